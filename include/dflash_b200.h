@@ -205,6 +205,130 @@ dfl_status dfl_argmax_top2_static(int32_t device, const float* logits_dev, int32
                                   uint64_t vocab, uint64_t ld, int32_t* argmax_dev,
                                   float* gap_dev, void* stream);
 
+/* ---- operators for a batch of requests that continue one prompt ----------
+ * No counterpart in the reference, which runs one sequence: the parts of a decoding step of many requests
+ * (best-of-n sampling, agents behind one system prompt) that depend on the batch, over the caller's own device
+ * buffers.  All three work like dfl_argmax_top2_static: they make `device` the calling thread's current device
+ * and leave it so, check their arguments, enqueue on `stream` (a cudaStream_t, NULL = the default stream) and
+ * return without waiting; they allocate nothing, keep nothing between calls and may be captured into a graph.
+ * Strides are in elements and not negative; the innermost dimension is contiguous; a stride of a dimension with
+ * one entry (or none) is not read.  A workspace belongs to the call from its enqueueing until the stream has
+ * passed it: calls that can overlap, and graphs that can be replayed at once, need one each.  Inputs of a call
+ * do not overlap its outputs except where that is said. */
+
+/* Per-head RMS norm of queries and keys, rotation by position, and the store of K and V rows, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight            (weight f32 [head_dim]; NULL = ones)
+ *   pair (j, j + rotary_dim / 2), j < rotary_dim / 2, turns by positions[axis(j)] * theta^(-2 j / rotary_dim)
+ * dimensions from rotary_dim on keep y (the layout of the model's own attention layers).  With several axes
+ * (time, height, width) sections[a] frequencies belong to axis a and their sum is rotary_dim / 2: one block of
+ * frequencies behind the other, or (interleaved) frequency j to axis a = j mod n_axes while j < n_axes *
+ * sections[a], and to axis 0 otherwise.  Angles are exact for every int32 position (negative ones too).
+ * kv_rows != NULL: token t's K and V rows go to row kv_rows[t] of k_out / v_out; tokens whose row is negative or
+ * at least n_kv_out_rows store none (their query is still written); no two tokens may name the same row.
+ * kv_rows == NULL: row t, and n_kv_out_rows is at least n_tokens.  v == NULL or n_kv_heads == 0: no V rows.
+ * An output may be its own input's buffer when types and strides are the same and kv_rows is NULL.
+ * src_dtype, dst_dtype: DFL_F32, DFL_F16 or DFL_BF16; head_dim 2..512, rotary_dim even and at most head_dim; theta >= 1;
+ * sums and angles in f32 or better, one rounding to dst_dtype.  n_tokens == 0 enqueues nothing. */
+#define DFL_MAX_ROPE_AXES 3
+typedef struct dfl_qk_norm_rope_args {
+    int32_t src_dtype, dst_dtype;
+    uint32_t n_tokens, n_q_heads, n_kv_heads, head_dim, rotary_dim;
+    uint32_t n_axes; /* 1..3 */
+    uint32_t sections[DFL_MAX_ROPE_AXES];
+    int32_t interleaved;
+    double theta;
+    float eps;
+    uint32_t _pad;
+    const void* q; /* [n_tokens][n_q_heads][head_dim] */
+    const void* k; /* [n_tokens][n_kv_heads][head_dim] */
+    const void* v;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const float* q_weight;
+    const float* k_weight;
+    const int32_t* positions; /* [n_axes][n_tokens] */
+    int64_t position_axis_stride;
+    const int64_t* kv_rows; /* [n_tokens] or NULL */
+    uint64_t n_kv_out_rows;
+    void* q_out; /* [n_tokens][n_q_heads][head_dim] */
+    void* k_out; /* [n_kv_out_rows][n_kv_heads][head_dim] */
+    void* v_out;
+    int64_t q_out_token_stride, q_out_head_stride, k_out_row_stride, k_out_head_stride, v_out_row_stride, v_out_head_stride;
+} dfl_qk_norm_rope_args;
+dfl_status dfl_qk_norm_rope(int32_t device, const dfl_qk_norm_rope_args* args, void* stream);
+
+/* Attention of a batch over one shared prefix and each request's own rows.  Request b's query i (i < q_len[b],
+ * or n_tokens when q_len is NULL) is its i-th newest-but-last token: it sees every prefix key and the own keys
+ * j <= own_len[b] - q_len[b] + i, the block's own rows being the last of own_len[b].  Query head h reads KV head
+ * h / (n_q_heads / n_kv_heads).  out = softmax(scale q k) v over what a row sees; a row that sees nothing, or
+ * whose scores are all -inf, is zero.  Output rows i >= q_len[b] are left as they were.  Lengths are read on
+ * the device (own_len is clamped to [0, own_capacity], q_len to [0, n_tokens]), so a captured call follows
+ * them.  Cache rows behind own_len, and the queries of absent tokens, may hold anything; a NaN or infinity in a V
+ * row that exists may reach every row of the request (a prefix row: of the batch) in the heads that read it.
+ * dtype: DFL_F16 or DFL_BF16 for all tensors; head_dim 64, 128 or 256; n_q_heads a multiple of n_kv_heads, at
+ * most 64 query heads a KV head; prefix_len and own_capacity below 2^30; addresses and strides multiples of 16
+ * bytes.  own_len may be NULL when own_capacity is 0.  Scores, softmax and sums in f32; the weights of a tile
+ * are rounded to dtype for the product with V, as is the result.  batch, n_tokens 0: enqueues nothing. */
+typedef struct dfl_prefix_attention_args {
+    int32_t dtype;
+    uint32_t batch, n_tokens, n_q_heads, n_kv_heads, head_dim;
+    float scale;
+    uint32_t _pad;
+    uint64_t prefix_len, own_capacity;
+    const void* q; /* [batch][n_tokens][n_q_heads][head_dim] */
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    const void* prefix_k; /* [prefix_len][n_kv_heads][head_dim] */
+    const void* prefix_v;
+    int64_t prefix_k_row_stride, prefix_k_head_stride, prefix_v_row_stride, prefix_v_head_stride;
+    const void* own_k; /* [batch][own_capacity][n_kv_heads][head_dim] */
+    const void* own_v;
+    int64_t own_k_batch_stride, own_k_row_stride, own_k_head_stride, own_v_batch_stride, own_v_row_stride, own_v_head_stride;
+    const int32_t* own_len; /* [batch] */
+    const int32_t* q_len;   /* [batch] or NULL */
+    void* out;              /* [batch][n_tokens][n_q_heads][head_dim] */
+    int64_t out_batch_stride, out_token_stride, out_head_stride;
+    void* workspace; /* 256-byte aligned */
+    uint64_t workspace_bytes;
+} dfl_prefix_attention_args;
+/* Bytes of workspace the call needs: depends on device, sizes and capacity, not on the lengths on the device. */
+dfl_status dfl_prefix_attention_workspace(int32_t device, const dfl_prefix_attention_args* args, uint64_t* bytes_out);
+dfl_status dfl_prefix_attention(int32_t device, const dfl_prefix_attention_args* args, void* stream);
+
+/* Verification of drafted tokens against the target's probabilities from given random numbers, on the device
+ * (dfl_accept_prefix is the host's, with its own generator and filters).  Row i of request b's logits
+ * [n_drafts + 1][vocab] is the target's distribution behind its first i drafts: p_i = softmax(logits / T), T =
+ * temperature[b] (NULL = 1); T == 0 puts all mass on the largest logit, ties to the lowest token.  Draft i
+ * (i < n_draft[b], NULL = n_drafts) stands while u_accept[b][i] * q_i(d_i) < p_i(d_i), where q_i is
+ * draft_probs[b][i] or, when that is NULL, all mass on the draft.  Behind the last draft that stands one token
+ * is drawn: from the residual max(p - q, 0) of the first refused draft (from p itself should that be empty),
+ * or from p of the last row when all stand - the lowest token whose cumulated mass exceeds u_sample[b] times
+ * the whole.  n_accepted_out[b] = drafts that stand; tokens_out[b] = those drafts, the drawn token, then -1.
+ * Where a row that the decision reads is no distribution (a NaN or +inf logit, all -inf, a negative or NaN
+ * temperature), n_accepted_out[b] = -1 - row and every token is -1.  A draft outside [0, vocab) does not stand.
+ * u in [0, 1); draft_probs finite and not negative.  The sums that draw a token are in 64 bits, so the token is
+ * the one that the definition gives.  n_drafts 0..DFL_MAX_VERIFY_DRAFTS, 1 <= vocab < 2^31; dtype of the logits: DFL_F32,
+ * DFL_F16 or DFL_BF16. */
+#define DFL_MAX_VERIFY_DRAFTS 255
+typedef struct dfl_verify_drafts_args {
+    int32_t dtype;
+    uint32_t batch, n_drafts, _pad;
+    uint64_t vocab;
+    const void* logits; /* [batch][n_drafts + 1][vocab] */
+    int64_t logits_batch_stride, logits_row_stride;
+    const float* draft_probs; /* [batch][n_drafts][vocab] or NULL */
+    int64_t probs_batch_stride, probs_row_stride;
+    const int32_t* drafts; /* [batch][n_drafts] contiguous, as the rest below */
+    const int32_t* n_draft;    /* [batch] or NULL */
+    const float* temperature;  /* [batch] or NULL */
+    const float* u_accept;     /* [batch][n_drafts] */
+    const float* u_sample;     /* [batch] */
+    int32_t* n_accepted_out;   /* [batch] */
+    int32_t* tokens_out;       /* [batch][n_drafts + 1] */
+    void* workspace;           /* 256-byte aligned */
+    uint64_t workspace_bytes;
+} dfl_verify_drafts_args;
+dfl_status dfl_verify_drafts_workspace(int32_t device, const dfl_verify_drafts_args* args, uint64_t* bytes_out);
+dfl_status dfl_verify_drafts(int32_t device, const dfl_verify_drafts_args* args, void* stream);
+
 /* ---- the CPU-runnable verify/accept case: two chained few-row GEMMs + greedy acceptance ---
  * logits = head(x W1^T); argmax per row; greedy prefix accept against drafts.
  * Device-resident pipeline object so the timed region has no allocation. */

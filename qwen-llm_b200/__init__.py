@@ -952,3 +952,7 @@ def make_device_tensor_table(entries):
             arr[i].on_device = 0
             keep.append((nm, raw))
     return arr, keep
+
+
+# operators for a batch of requests over one prompt (torch CUDA tensors)
+from .batch_ops import prefix_attention, qk_norm_rope, verify_drafts  # noqa: E402,F401

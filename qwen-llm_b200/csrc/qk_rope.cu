@@ -1,0 +1,241 @@
+// Norms of queries and keys for each head, rotation by position (one to three axes) and the store of the K and V rows, in one pass.
+//
+//   y = x * rsqrt(mean(x^2) + eps) * w;   (y_j, y_{j+h}) turns by pos[axis(j)] * theta^(-j/h),  h = rotary_dim / 2
+//
+// Bound: every element is read once and written once, a few dozen instructions an eight-element chunk: HBM.  A warp takes a token (or,
+// when there are fewer tokens than warps to fill the machine, a share of a token's heads), so the angles of a token are computed
+// once and reach the lanes through the warp's own piece of shared memory.
+//
+// Angles.  pos * frequency in f32 is off by 0.06 rad at position 1e6.  Here the frequency is a fraction of a turn in 64-bit fixed
+// point, F = 2^64 theta^(-j/h) / 2 pi, made on the host in extended precision; pos * F modulo 2^64 is the angle modulo one
+// turn (the wrap of the integer product drops the whole turns), off by at most 2^-27 turns at position 2^31.  Its upper 32 bits become f32.
+#include <cmath>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace dfl {
+dfl_status use_device(int device);
+namespace {
+
+constexpr int ROPE_MAX_DIM = 512;
+constexpr int ROPE_WARPS = 8;
+
+struct RopeParams {
+    const void *q, *k, *v;
+    void *q_out, *k_out, *v_out;
+    const float *qw, *kw;
+    const int32_t* pos;
+    const int64_t* rows;
+    int64_t q_t, q_h, k_t, k_h, v_t, v_h, qo_t, qo_h, ko_t, ko_h, vo_t, vo_h, pos_axis;
+    uint64_t n_rows;
+    uint32_t n_tokens, n_q, n_kv, dim, half, n_heads;   // n_heads: q, k and v heads of a token
+    uint32_t parts;                                     // warps that share a token's heads
+    float eps;
+    uint64_t turn[ROPE_MAX_DIM / 2];                    // fraction of a turn per position, 2^-64
+    uint8_t axis[ROPE_MAX_DIM / 2];
+};
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T> struct __align__(4 * sizeof(T)) Quad { T v[4]; };
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&x)[4]) {
+    const Quad<T> r = *reinterpret_cast<const Quad<T>*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = to_f<T>(r.v[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
+    Quad<T> r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = from_f<T>(x[i]);
+    *reinterpret_cast<Quad<T>*>(p) = r;
+}
+
+// cos and sin of one frequency at a token
+__device__ __forceinline__ float2 turn_of(const RopeParams& p, const uint64_t* turn, const uint8_t* axis, uint32_t j, uint32_t token) {
+    const int64_t pos = p.pos[axis[j] * p.pos_axis + token];
+    const uint64_t angle = (uint64_t)pos * turn[j];
+    float2 r;
+    sincospif((float)(int32_t)(angle >> 32) * 0x1p-31f, &r.y, &r.x);   // half turns in [-1, 1)
+    return r;
+}
+
+template <typename S, typename D>
+struct HeadRef {
+    const S* src;
+    D* dst;          // null: nothing is stored
+    const float* w;  // null: ones
+    bool normed;
+};
+template <typename S, typename D>
+__device__ __forceinline__ HeadRef<S, D> head_of(const RopeParams& p, uint32_t h, uint32_t token, int64_t row) {
+    HeadRef<S, D> r;
+    if (h < p.n_q) {
+        r.src = static_cast<const S*>(p.q) + token * p.q_t + h * p.q_h;
+        r.dst = static_cast<D*>(p.q_out) + token * p.qo_t + h * p.qo_h;
+        r.w = p.qw;
+        r.normed = true;
+    } else if (h < p.n_q + p.n_kv) {
+        h -= p.n_q;
+        r.src = static_cast<const S*>(p.k) + token * p.k_t + h * p.k_h;
+        r.dst = row >= 0 ? static_cast<D*>(p.k_out) + row * p.ko_t + h * p.ko_h : nullptr;
+        r.w = p.kw;
+        r.normed = true;
+    } else {
+        h -= p.n_q + p.n_kv;
+        r.src = static_cast<const S*>(p.v) + token * p.v_t + h * p.v_h;
+        r.dst = row >= 0 ? static_cast<D*>(p.v_out) + row * p.vo_t + h * p.vo_h : nullptr;
+        r.w = nullptr;
+        r.normed = false;
+    }
+    return r;
+}
+__device__ __forceinline__ int64_t row_of(const RopeParams& p, uint32_t token) {
+    const int64_t row = p.rows ? p.rows[token] : (int64_t)token;
+    return (uint64_t)row < p.n_rows ? row : -1;   // a negative row is a large unsigned one
+}
+
+// Any head width and alignment: a lane per element, partners through shared memory.
+template <typename S, typename D>
+__global__ void __launch_bounds__(32 * ROPE_WARPS) qk_norm_rope_any_kernel(const __grid_constant__ RopeParams p) {
+    __shared__ uint64_t turn[ROPE_MAX_DIM / 2];
+    __shared__ uint8_t axis[ROPE_MAX_DIM / 2];
+    __shared__ float y[ROPE_WARPS][ROPE_MAX_DIM];
+    for (uint32_t j = threadIdx.x; j < p.half; j += blockDim.x) turn[j] = p.turn[j], axis[j] = p.axis[j];
+    pdl_prologue();
+    __syncthreads();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t n_items = (uint64_t)p.n_tokens * p.parts;
+    for (uint64_t item = (uint64_t)blockIdx.x * ROPE_WARPS + warp; item < n_items; item += (uint64_t)gridDim.x * ROPE_WARPS) {
+        const uint32_t token = (uint32_t)(item / p.parts), part = (uint32_t)(item % p.parts);
+        const int64_t row = row_of(p, token);
+        for (uint32_t h = part; h < p.n_heads; h += p.parts) {
+            const HeadRef<S, D> r = head_of<S, D>(p, h, token, row);
+            float sum = 0.f;
+            for (uint32_t j = lane; j < p.dim; j += 32) {
+                const float x = to_f<S>(r.src[j]);
+                y[warp][j] = x;
+                sum += x * x;
+            }
+            sum = warp_sum(sum);
+            __syncwarp();
+            if (r.dst) {
+                const float norm = r.normed ? rsqrtf(sum / (float)p.dim + p.eps) : 1.f;
+                for (uint32_t j = lane; j < p.dim; j += 32) {
+                    const uint32_t f = j < p.half ? j : j - p.half;
+                    float out = y[warp][j] * norm * (r.w ? r.w[j] : 1.f);
+                    if (r.normed && j < 2 * p.half) {
+                        const float2 t = turn_of(p, turn, axis, f, token);
+                        const uint32_t o = j < p.half ? j + p.half : f;
+                        const float other = y[warp][o] * norm * (r.w ? r.w[o] : 1.f);
+                        out = j < p.half ? out * t.x - other * t.y : out * t.x + other * t.y;
+                    }
+                    r.dst[j] = from_f<D>(out);
+                }
+            }
+            __syncwarp();
+        }
+    }
+}
+
+bool dtype_ok(int32_t d) { return d == DFL_F32 || d == DFL_F16 || d == DFL_BF16; }
+
+template <typename S, typename D>
+cudaError_t launch_typed(const RopeParams& p, cudaStream_t st) {
+    const uint64_t items = (uint64_t)p.n_tokens * p.parts;
+    const uint64_t blocks = (items + ROPE_WARPS - 1) / ROPE_WARPS, most = (uint64_t)sm_count() * 8;
+    return launch_k(qk_norm_rope_any_kernel<S, D>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(32 * ROPE_WARPS), 0, st, p);
+}
+template <typename S>
+cudaError_t launch_src(const RopeParams& p, int32_t dst, cudaStream_t st) {
+    if (dst == DFL_F32) return launch_typed<S, float>(p, st);
+    if (dst == DFL_F16) return launch_typed<S, __half>(p, st);
+    return launch_typed<S, __nv_bfloat16>(p, st);
+}
+
+}  // namespace
+}  // namespace dfl
+
+extern "C" dfl_status dfl_qk_norm_rope(int32_t device, const dfl_qk_norm_rope_args* a, void* stream) {
+    using namespace dfl;
+    if (!a) return fail(DFL_ERR_BAD_ARG, "qk_norm_rope: null arguments");
+    if (!dtype_ok(a->src_dtype) || !dtype_ok(a->dst_dtype)) return fail(DFL_ERR_UNSUPPORTED, "qk_norm_rope: dtypes are f32, f16 and bf16");
+    if (a->head_dim < 2 || a->head_dim > ROPE_MAX_DIM || a->rotary_dim > a->head_dim || a->rotary_dim % 2)
+        return fail(DFL_ERR_BAD_SHAPE, "qk_norm_rope: need 2 <= head_dim <= 512 and an even rotary_dim <= head_dim");
+    if (a->n_axes < 1 || a->n_axes > DFL_MAX_ROPE_AXES) return fail(DFL_ERR_BAD_ARG, "qk_norm_rope: n_axes is 1, 2 or 3");
+    if (a->n_tokens > 0x7fffffffu || a->n_q_heads > 65536 || a->n_kv_heads > 65536) return fail(DFL_ERR_BAD_SHAPE, "qk_norm_rope: too many tokens or heads");
+    if (!(a->theta >= 1.0) || !std::isfinite(a->theta)) return fail(DFL_ERR_BAD_ARG, "qk_norm_rope: theta must be finite and at least 1");
+    if (!(a->eps >= 0.f) || !std::isfinite(a->eps)) return fail(DFL_ERR_BAD_ARG, "qk_norm_rope: eps must be finite and not negative");
+    const uint32_t half = a->rotary_dim / 2;
+    uint64_t sum = 0;
+    for (uint32_t i = 0; i < a->n_axes; ++i) {
+        sum += a->sections[i];
+        if (a->interleaved && i > 0 && a->sections[i] > 0 && (uint64_t)(a->sections[i] - 1) * a->n_axes + i >= half)
+            return fail(DFL_ERR_BAD_SHAPE, "qk_norm_rope: an interleaved section reaches beyond rotary_dim / 2 frequencies");
+    }
+    if (sum != half) return fail(DFL_ERR_BAD_SHAPE, "qk_norm_rope: the sections' sum must be rotary_dim / 2");
+    for (int64_t s : {a->q_token_stride, a->q_head_stride, a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, a->q_out_token_stride,
+                      a->q_out_head_stride, a->k_out_row_stride, a->k_out_head_stride, a->v_out_row_stride, a->v_out_head_stride, a->position_axis_stride})
+        if (s < 0) return fail(DFL_ERR_BAD_SHAPE, "qk_norm_rope: negative stride");
+    const bool has_v = a->v != nullptr && a->n_kv_heads > 0;
+    if (a->n_tokens > 0) {
+        if (a->n_q_heads && (!a->q || !a->q_out)) return fail(DFL_ERR_BAD_ARG, "qk_norm_rope: q and q_out are needed");
+        if (a->n_kv_heads && (!a->k || !a->k_out)) return fail(DFL_ERR_BAD_ARG, "qk_norm_rope: k and k_out are needed");
+        if (has_v && !a->v_out) return fail(DFL_ERR_BAD_ARG, "qk_norm_rope: v without v_out");
+        if (half && !a->positions) return fail(DFL_ERR_BAD_ARG, "qk_norm_rope: positions are needed");
+        if (a->n_kv_heads && !a->kv_rows && a->n_kv_out_rows < a->n_tokens) return fail(DFL_ERR_BAD_SHAPE, "qk_norm_rope: fewer output rows than tokens");
+    }
+    DFL_CHECK(use_device(device));
+    RopeParams p = {};
+    p.q = a->q, p.k = a->k, p.v = a->v, p.q_out = a->q_out, p.k_out = a->k_out, p.v_out = a->v_out;
+    p.qw = a->q_weight, p.kw = a->k_weight, p.pos = a->positions, p.rows = a->kv_rows;
+    const bool one_q = a->n_q_heads <= 1, one_k = a->n_kv_heads <= 1, one_t = a->n_tokens <= 1, one_r = a->n_kv_out_rows <= 1;
+    p.q_t = one_t ? 0 : a->q_token_stride, p.q_h = one_q ? 0 : a->q_head_stride;
+    p.k_t = one_t ? 0 : a->k_token_stride, p.k_h = one_k ? 0 : a->k_head_stride;
+    p.v_t = one_t ? 0 : a->v_token_stride, p.v_h = one_k ? 0 : a->v_head_stride;
+    p.qo_t = one_t ? 0 : a->q_out_token_stride, p.qo_h = one_q ? 0 : a->q_out_head_stride;
+    p.ko_t = one_r ? 0 : a->k_out_row_stride, p.ko_h = one_k ? 0 : a->k_out_head_stride;
+    p.vo_t = one_r ? 0 : a->v_out_row_stride, p.vo_h = one_k ? 0 : a->v_out_head_stride;
+    p.pos_axis = a->n_axes <= 1 ? 0 : a->position_axis_stride;
+    p.n_rows = a->n_kv_out_rows;
+    p.n_tokens = a->n_tokens, p.n_q = a->n_q_heads, p.n_kv = a->n_kv_heads, p.dim = a->head_dim, p.half = half;
+    p.n_heads = a->n_q_heads + a->n_kv_heads * (has_v ? 2u : 1u);
+    p.eps = a->eps;
+    if (p.n_tokens == 0 || p.n_heads == 0) return DFL_OK;
+    uint32_t upto = 0, owner = 0;
+    const long double step = half ? powl((long double)a->theta, -1.0L / half) : 1.0L;
+    long double turns = 1.0L / 6.283185307179586476925286766559L;   // at most 0.16: theta is at least one
+    for (uint32_t j = 0; j < half; ++j) {
+        p.turn[j] = (uint64_t)(turns * 0x1p64L);
+        turns *= step;   // 2^-64 of itself off a step: after 255 steps and 2^31 positions 2^-27 turns
+        if (a->interleaved) {
+            const uint32_t ax = j % a->n_axes;
+            p.axis[j] = (uint8_t)(j < (uint64_t)a->n_axes * a->sections[ax] ? ax : 0);
+        } else {
+            while (j >= upto + a->sections[owner]) upto += a->sections[owner++];
+            p.axis[j] = (uint8_t)owner;
+        }
+    }
+    // a token's heads are shared out until the machine has eight warps an SM
+    const uint64_t wanted = (uint64_t)sm_count() * 8;
+    const uint64_t parts = (wanted + p.n_tokens - 1) / p.n_tokens;
+    p.parts = (uint32_t)(parts < p.n_heads ? parts : p.n_heads);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (a->src_dtype == DFL_F32) e = launch_src<float>(p, a->dst_dtype, st);
+    else if (a->src_dtype == DFL_F16) e = launch_src<__half>(p, a->dst_dtype, st);
+    else e = launch_src<__nv_bfloat16>(p, a->dst_dtype, st);
+    DFL_CUDA(e);
+    count_launch();
+    return DFL_OK;
+}
