@@ -1,11 +1,56 @@
 // Attention of a batch of requests over one shared prefix and each request's own rows.
+//
+//   o_r = sum_j softmax(scale q_r k_j) v_j   over the prefix keys and the own keys up to the row's position
+//
+// A row is one query head of one token; the rows of a KV head lie one behind the other as r = (request * n + token) * group + g.
+// A work item is a tile of rows against a run of key tiles (128 keys each):
+//   * prefix items take rows ACROSS requests, so one tile of prefix K / V from memory serves up to 256 rows: for the batch the prefix is read
+//     once per 256 rows and not once a request;
+//   * own items take the rows of one request against its own keys;
+//   * fused items (requests with enough rows of their own to fill tiles) run over the prefix and then over the own keys and write the
+//     result themselves.
+// Items that see only a part of a row's keys leave (maximum, sum, unscaled output) in the workspace and a second kernel joins the parts.  Key
+// runs are split until the items fill the machine, so a few rows over a long prefix use every SM.
+//
+// One persistent CTA an SM; S = Q K^T and O += P V on the tensor cores (tcgen05, both accumulators and P in tensor memory), K and V tiles by
+// TMA into a ring.  Two warpgroups of softmax threads (thread = row), one MMA issuer, one producer.  Up to a head width of 128 the
+// warpgroups have a row tile each (or, when the item has at most 128 rows, every other key tile of the same rows), so one's products run
+// under the other's exponentials; at 256 the output takes half of tensor memory, and one warpgroup works on two score buffers in turn.
+// Step t uses score buffer t & 1 throughout: S(t) is issued behind PV(t - 2), which read that buffer's P.
+#include <cuda.h>
+
 #include <cmath>
 
-#include "common.cuh"
+#include "tcgen05_prims.cuh"
 
 namespace dfl {
 dfl_status use_device(int device);
 namespace {
+
+using namespace ts;
+
+constexpr int BA_KEYS = 128;             // keys of a tile
+constexpr int BA_ROWS = 128;             // rows of a tile
+constexpr int BA_THREADS = 384;          // 2 x 4 softmax warps, MMA issue, producer, two idle warps that make a warpgroup of the last four
+// A softmax thread holds a row of 128 scores: of the 168 registers a thread of the launch the last warpgroup gives most away (2 x 216 + 72 = 3 x 168).
+constexpr int BA_REGS_SOFTMAX = 216, BA_REGS_REST = 72;
+constexpr int BA_BOX = BA_KEYS * 128;    // one TMA box: 128 keys x 64 dimensions of 16 bits, 128-byte swizzle
+constexpr float BA_RESCALE = 8.f;        // a row's reference maximum moves when it is passed by 2^8: weights stay below 2^(8 + bias)
+
+template <int D>
+struct BaCfg {
+    static constexpr int UNIT = D < 128 ? D : 128;                // dimensions of a ring slot
+    static constexpr int UNITS = D / UNIT;                        // slots of a K or V tile
+    static constexpr int SLOT = BA_KEYS * UNIT * 2;
+    static constexpr int SLOTS = D == 64 ? 8 : 5;
+    static constexpr int TILES = D <= 128 ? 2 : 1;                // row tiles of a CTA
+    static constexpr int Q_BYTES = BA_ROWS * D * 2;
+    static constexpr int OFF_RING = TILES * Q_BYTES;
+    static constexpr int OFF_BAR = OFF_RING + SLOTS * SLOT;
+    static constexpr int SMEM = OFF_BAR + 256 + 1024;             // barriers, alignment of the base
+    static constexpr uint32_t TM_S = 0, TM_O = 256;               // columns: two score buffers, the accumulators
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+};
 
 struct BatchAttnParams {
     const void *q, *pk, *pv, *ok, *ov;
@@ -15,6 +60,16 @@ struct BatchAttnParams {
     uint32_t batch, n, n_q, n_kv, group;
     int32_t prefix, cap;
     float scale;
+    // the plan
+    uint32_t rows;                       // of a KV head: batch * n * group
+    uint32_t p_items, items;             // prefix items first
+    uint32_t p_blocks, p_splits, p_run;  // row blocks, splits of the keys, key tiles of a split
+    uint32_t o_blocks, o_splits, o_run;  // of one request
+    uint32_t prefix_tiles;
+    int32_t fused, direct, p_pair, o_pair;   // p_pair / o_pair: the warpgroups share a row tile and take the key tiles in turn
+    uint32_t p_parts, parts;             // parts a row may have in the workspace, the prefix's first
+    float2* part_ml;                     // [parts][n_kv][rows] reference maximum, sum
+    float* part_o;                       // [parts][n_kv][rows][D]
 };
 
 __device__ __forceinline__ int own_len_of(const BatchAttnParams& p, uint32_t b) {
@@ -26,41 +81,516 @@ __device__ __forceinline__ int q_len_of(const BatchAttnParams& p, uint32_t b) {
     return v < 0 ? 0 : v > (int)p.n ? (int)p.n : v;
 }
 
-// A warp a query: its dimensions over the lanes, one key at a time.
+template <typename T> struct Pair16;
+template <> struct Pair16<__half> {
+    static constexpr uint32_t FMT = 0;   // operand format of the instruction descriptor
+    static constexpr float BIAS = 7.f;   // weights up to 2^15: the small ones stay normal numbers for seven more powers of two
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+template <> struct Pair16<__nv_bfloat16> {
+    static constexpr uint32_t FMT = 1;
+    static constexpr float BIAS = 0.f;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// 128-byte swizzle, 8-row groups 1024 bytes apart.  K-major: `lbo` unused.  MN-major: `lbo` bytes between blocks of 64 along MN.
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr, uint32_t lbo) {
+    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+                 "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+                 "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+                 : "memory");
+}
+
+// Barriers of a step: by its warpgroup, 0 and 1 when both work; one that works alone has 0 for its even and 2 for its odd steps.  A parity wait only
+// tells a phase from the one before to a party that has seen every phase: none has a barrier that another warpgroup's steps go by.
+__device__ __forceinline__ int bar_of(bool two, int t) { return (t & 1) == 0 ? 0 : two ? 1 : 2; }
+
+// What every role works out alike from an item's number.
+struct Item {
+    uint32_t h, row0, row_end;   // rows row0.. of the KV head's, below row_end
+    uint32_t b;                  // the request of its own keys
+    int p0, p1, o0, o1;          // tiles of the prefix, of the own keys
+    uint32_t part;               // where its rows' parts go
+    int own, q_len;              // lengths of the request (own items)
+    bool pair;                   // the warpgroups share the rows
+    bool two;                    // both warpgroups work
+    int tiles, steps;
+};
+template <int D>
+__device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx) {
+    constexpr uint32_t BLOCK = BaCfg<D>::TILES * BA_ROWS;
+    Item it;
+    it.o0 = it.o1 = it.p0 = it.p1 = 0;
+    it.own = it.q_len = 0;
+    it.b = 0;
+    if (idx < p.p_items) {   // the row blocks of one split and head side by side: they read the same keys
+        const uint32_t block = idx % p.p_blocks, rest = idx / p.p_blocks, split = rest / p.n_kv;
+        it.h = rest % p.n_kv;
+        it.pair = p.p_pair != 0;
+        it.row0 = block * (it.pair ? BA_ROWS : BLOCK);
+        it.row_end = p.rows;
+        it.p0 = (int)(split * p.p_run);
+        it.p1 = min((int)p.prefix_tiles, it.p0 + (int)p.p_run);
+        it.part = split * (it.pair ? 2u : 1u);
+    } else {                 // the later rows of a request see more keys: they go first
+        idx -= p.p_items;
+        const uint32_t bh = idx % (p.batch * p.n_kv), rest = idx / (p.batch * p.n_kv), split = rest % p.o_splits;
+        const uint32_t block = p.o_blocks - 1 - rest / p.o_splits, per = p.n * p.group;
+        it.h = bh % p.n_kv;
+        it.b = bh / p.n_kv;
+        it.pair = p.o_pair != 0;
+        const uint32_t first = block * (it.pair ? BA_ROWS : BLOCK);
+        it.row0 = it.b * per + first;
+        it.own = own_len_of(p, it.b);
+        it.q_len = q_len_of(p, it.b);
+        const uint32_t there = (uint32_t)it.q_len * p.group;
+        it.row_end = it.b * per + (first < there ? min(there, per) : first);
+        // keys that the block's last row sees
+        const uint32_t last = min(first + (it.pair ? BA_ROWS : BLOCK), there);
+        const int seen = last > first ? min(it.own, max(0, it.own - it.q_len + (int)((last - 1) / p.group) + 1)) : 0;
+        const int pre = p.fused ? (int)p.prefix_tiles : 0, all = pre + (seen + BA_KEYS - 1) / BA_KEYS;
+        const int t0 = (int)(split * p.o_run), t1 = min(all, t0 + (int)p.o_run);
+        it.p0 = min(t0, pre), it.p1 = min(max(t1, it.p0), pre);
+        it.o0 = max(t0 - pre, 0), it.o1 = max(t1 - pre, it.o0);
+        it.part = p.p_parts + split * (it.pair ? 2u : 1u);
+    }
+    it.two = BaCfg<D>::TILES == 2 && (it.pair || it.row_end > it.row0 + BA_ROWS);
+    it.tiles = it.row_end > it.row0 ? (it.p1 - it.p0) + (it.o1 - it.o0) : 0;
+    it.steps = it.two && !it.pair ? 2 * it.tiles : it.tiles;
+    return it;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) batch_attn_row_kernel(const __grid_constant__ BatchAttnParams p) {
+__global__ void __launch_bounds__(BA_THREADS, 1)
+batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_constant__ CUtensorMap map_pk, const __grid_constant__ CUtensorMap map_pv,
+                     const __grid_constant__ CUtensorMap map_ok, const __grid_constant__ CUtensorMap map_ov) {
+    using C = BaCfg<D>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* ring = smem + C::OFF_RING;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+    uint64_t* empty = full + C::SLOTS;
+    uint64_t* q_full = empty + C::SLOTS;
+    uint64_t* s_full = q_full + 2;
+    uint64_t* p_full = s_full + 3;
+    uint64_t* pv_done = p_full + 3;
+    uint64_t* tail = pv_done + 3;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int err;   // a wait has run out: what is left is filled with NaN
+
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::SLOTS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 4);
+        for (int i = 0; i < 3; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&pv_done[i], 1);
+        }
+        mbar_init(tail, 1);
+        err = 0;
+        mbar_fence_init();
+    }
+    if (warp == 8) tmem_alloc(&tmem_slot, 512);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    pdl_prologue();
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BA_REGS_SOFTMAX));
+        // ================= softmax: thread = row =================
+        const int wg = warp >> 2, row = 32 * (warp & 3) + lane;
+        const uint32_t tm_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t tm_o = tm_lane + C::TM_O + (C::TILES == 2 ? (uint32_t)(wg * D) : 0u);
+        const float c = p.scale * 1.4426950408889634f;
+        uint8_t* q_rows = smem + wg * C::Q_BYTES + (warp & 3) * 32 * 128;   // this warp's rows of each block of 64 dimensions
+        uint32_t even = 0, odd = 0, alone = 0;   // uses of the barriers so far
+        for (uint32_t idx = blockIdx.x; idx < p.items; idx += gridDim.x) {
+            const Item it = item_of<D>(p, idx);
+            if (wg > 0 && !it.two) continue;
+            const uint32_t base0 = even, base1 = it.two ? odd : alone;
+            even += (uint32_t)(it.steps + 1) / 2;
+            (it.two ? odd : alone) += (uint32_t)it.steps / 2;
+            auto parity = [&](int t) { return ((t & 1 ? base1 : base0) + (uint32_t)(t >> 1)) & 1u; };
+            const uint32_t r = it.row0 + (it.two && !it.pair ? wg * BA_ROWS : 0) + row;
+            const bool there = r < it.row_end;
+            const uint32_t per = p.n * p.group, b = r / per, rem = r - b * per, tok = rem / p.group, g = rem - tok * p.group, head = it.h * p.group + g;
+            const int sees = min(it.own, max(0, it.own - it.q_len + (int)tok + 1));   // own items
+            const int first = it.two ? wg : 0, stride = it.two ? 2 : 1;
+            bool ok = *reinterpret_cast<volatile int*>(&err) == 0;
+            const bool active = __any_sync(0xffffffffu, there);
+            const bool stored = there && (!p.direct || (int)tok < q_len_of(p, b));
+            float m = -INFINITY, l = 0.f;
+            if (first < it.steps && ok) {
+                // the rows of Q into the operand layout: row r, 16-byte chunk k at chunk k ^ (r & 7)
+                const int64_t off = there ? b * p.q_b + tok * p.q_t + head * p.q_h : 0;
+                constexpr int CH = D / 8;   // chunks of a row
+#pragma unroll 4
+                for (int i = lane; i < 32 * CH; i += 32) {
+                    const int rr = i / CH, k = i % CH;
+                    const int64_t o = __shfl_sync(0xffffffffu, off, rr);
+                    const bool v = __shfl_sync(0xffffffffu, (int)there, rr) != 0;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (v) x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + o + k * 8);
+                    *reinterpret_cast<uint4*>(q_rows + (k >> 3) * BA_BOX + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) = x;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[wg]);
+            }
+            for (int t = first; t < it.steps && ok; t += stride) {
+                const int x = t & 1, tile = it.two && !it.pair ? t >> 1 : t;
+                ok = mbar_wait_warp_inline(&s_full[bar_of(it.two, t)], parity(t), &err, DEV_ERR_WAIT_FULL);
+                if (!ok) break;
+                fence_after_sync();
+                if (active) {
+                    const uint32_t tm_s = tm_lane + C::TM_S + 128u * (uint32_t)x;
+                    float s[128];
+                    tmem_ld32(tm_s, *reinterpret_cast<float(*)[32]>(s));
+                    tmem_ld32(tm_s + 32, *reinterpret_cast<float(*)[32]>(s + 32));
+                    tmem_ld32(tm_s + 64, *reinterpret_cast<float(*)[32]>(s + 64));
+                    tmem_ld32(tm_s + 96, *reinterpret_cast<float(*)[32]>(s + 96));
+                    wait_ld();
+                    const int n_p = it.p1 - it.p0;
+                    const int limit = tile < n_p ? p.prefix - (it.p0 + tile) * BA_KEYS : sees - (it.o0 + tile - n_p) * BA_KEYS;
+                    if (__any_sync(0xffffffffu, limit < BA_KEYS)) {
+#pragma unroll
+                        for (int j = 0; j < 128; ++j) s[j] = j < limit ? s[j] : -INFINITY;
+                    }
+                    float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int j = 4; j < 128; j += 4) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], s[j + k]);
+                    }
+                    const float t4 = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    const bool moves = m == -INFINITY ? t4 > -INFINITY : (t4 - m) * c > BA_RESCALE;
+                    if (__any_sync(0xffffffffu, moves)) {
+                        const float f = moves ? (m == -INFINITY ? 0.f : ex2((m - t4) * c)) : 1.f;
+                        if (t >= first + stride) {   // the accumulator holds earlier tiles: their products have to be done
+                            ok = mbar_wait_warp_inline(&pv_done[bar_of(it.two, t - stride)], parity(t - stride), &err, DEV_ERR_WAIT_DRAIN);
+                            if (!ok) break;
+                            fence_after_sync();
+#pragma unroll
+                            for (int j = 0; j < D; j += 16) {
+                                float o[16];
+                                uint32_t u[16];
+                                tmem_ld16(tm_o + j, o);
+                                wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(o[k] * f);
+                                tmem_st16(tm_o + j, u);
+                            }
+                        }
+                        l *= f;
+                        if (moves) m = t4;
+                    }
+                    const float mc = m == -INFINITY ? 0.f : m * c - Pair16<T>::BIAS;
+                    const uint64_t c2 = pack2(c, c), mc2 = pack2(-mc, -mc);
+                    uint64_t sum2[2] = {0, 0};
+#pragma unroll
+                    for (int j = 0; j < 64; j += 32) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            float a, e;
+                            unpack2(fma2(pack2(s[2 * (j + k)], s[2 * (j + k) + 1]), c2, mc2), a, e);
+                            a = ex2(a), e = ex2(e);
+                            sum2[k & 1] = add2(sum2[k & 1], pack2(a, e));
+                            w[k] = Pair16<T>::pack(a, e);
+                        }
+                        tmem_st32(tm_s + j, w);
+                    }
+                    float a, e;
+                    unpack2(add2(sum2[0], sum2[1]), a, e);
+                    l += a + e;
+                    wait_st();
+                }
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[bar_of(it.two, t)]);
+            }
+            // the last products of this warpgroup's accumulator
+            const int last = it.steps > first ? first + (it.steps - 1 - first) / stride * stride : -1;
+            if (last >= 0 && ok) {
+                ok = mbar_wait_warp_inline(&pv_done[bar_of(it.two, last)], parity(last), &err, DEV_ERR_WAIT_DRAIN);
+                fence_after_sync();
+            }
+            if (!ok) l = __int_as_float(0x7fffffff);
+            const bool holds = last >= 0 && ok;   // the accumulator has something
+            if (!active) continue;
+            const uint32_t row_w = r - lane;      // the warp's first row
+            __syncwarp();
+            if (p.direct) {
+                const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+                const int64_t off = there ? b * p.o_b + tok * p.o_t + head * p.o_h : 0;
+#pragma unroll 1
+                for (int k = 0; k < D / 64; ++k) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float o[32];
+                        if (holds) {
+                            tmem_ld32(tm_o + 64 * k + 32 * j, o);
+                            wait_ld();
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int at = 8 * i + 2 * e;
+                                w[e] = Pair16<T>::pack(holds && l != 0.f ? o[at] * inv : inv, holds && l != 0.f ? o[at + 1] * inv : inv);
+                            }
+                            *reinterpret_cast<uint4*>(q_rows + lane * 128 + (((4 * j + i) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int rr = 4 * i + (lane >> 3), ch = lane & 7;
+                        const int64_t o = __shfl_sync(0xffffffffu, off, rr);
+                        const uint4 w = *reinterpret_cast<const uint4*>(q_rows + rr * 128 + ((ch ^ (rr & 7)) << 4));
+                        if (__shfl_sync(0xffffffffu, (int)stored, rr)) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + o + 64 * k + 8 * ch) = w;
+                    }
+                    __syncwarp();
+                }
+            } else {
+                const uint64_t base = ((uint64_t)(it.part + (it.pair ? wg : 0)) * p.n_kv + it.h) * p.rows;
+                if (there) p.part_ml[base + r] = make_float2(m, l);
+                if (!holds) continue;   // a part without mass is not read
+                float* dst = p.part_o + (base + row_w) * D;
+#pragma unroll 1
+                for (int k = 0; k < D / 32; ++k) {
+                    float o[32];
+                    tmem_ld32(tm_o + 32 * k, o);
+                    wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<float4*>(q_rows + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int rr = 4 * i + (lane >> 3), ch = lane & 7;
+                        const float4 w = *reinterpret_cast<const float4*>(q_rows + rr * 128 + ((ch ^ (rr & 7)) << 4));
+                        if (row_w + rr < it.row_end) *reinterpret_cast<float4*>(dst + (uint64_t)rr * D + 32 * k + 4 * ch) = w;
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BA_REGS_REST));
+    }
+    if (warp == 8) {
+        // ================= MMA issue =================
+        constexpr uint32_t FMT = (Pair16<T>::FMT << 7) | (Pair16<T>::FMT << 10);
+        constexpr uint32_t ID_S = instr_desc(128) | FMT, ID_O = instr_desc(C::UNIT) | FMT | (1u << 16);   // V lies key by key: N-major
+        const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(smem);
+        uint32_t even = 0, odd = 0, alone = 0, q_uses[2] = {0, 0}, seq = 0;
+        bool ok = true;
+        for (uint32_t idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
+            const Item it = item_of<D>(p, idx);
+            const bool in_step = it.two && !it.pair;   // both warpgroups use a key tile
+            auto k_seq = [&](int tile) { return seq + C::UNITS * (uint32_t)(in_step ? 2 * tile : tile == 0 ? 0 : 2 * tile - 1); };
+            auto v_seq = [&](int tile) { return seq + C::UNITS * (uint32_t)(in_step ? 2 * tile + 1 : tile == it.tiles - 1 ? 2 * tile + 1 : 2 * tile + 2); };
+            for (int t = 0; t < it.steps + 2 && ok; ++t) {
+                const int x = t & 1;
+                if (t >= 2) {   // O += P V of step t - 2
+                    const int tp = t - 2, tile = in_step ? tp >> 1 : tp;
+                    ok = mbar_wait_warp(&p_full[bar_of(it.two, tp)], ((x ? (it.two ? odd : alone) : even) + (uint32_t)(tp >> 1)) & 1u, &err, DEV_ERR_WAIT_FULL);
+                    const uint32_t acc = it.two ? (uint32_t)x : 0u;
+                    const bool fresh = tp < (it.two ? 2 : 1), frees = !in_step || x == 1;
+                    for (int u = 0; u < C::UNITS && ok; ++u) {
+                        const uint32_t q = v_seq(tile) + u, slot = q % C::SLOTS;
+                        ok = mbar_wait_warp(&full[slot], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_FULL);
+                        if (!ok) break;
+                        fence_after_sync();
+                        if (elect_one()) {
+                            const uint32_t v_a = ring_a + slot * C::SLOT;
+#pragma unroll
+                            for (int j = 0; j < BA_KEYS / 16; ++j)
+                                mma_ts_rt(tmem + C::TM_O + acc * D + u * C::UNIT, tmem + C::TM_S + 128u * (uint32_t)x + 8u * j, swizzled_desc(v_a + 2048u * j, BA_BOX), ID_O,
+                                          fresh && j == 0 ? 0u : 1u);
+                            if (frees) mma_commit(&empty[slot]);
+                            if (u == C::UNITS - 1) mma_commit(&pv_done[bar_of(it.two, t)]);
+                        }
+                        __syncwarp();
+                    }
+                    if (!ok) break;
+                }
+                if (t < it.steps) {   // S = Q K^T
+                    const int tile = in_step ? t >> 1 : t, rt = it.two ? x : 0;
+                    if (t < (it.two ? 2 : 1)) {
+                        ok = mbar_wait_warp(&q_full[rt], q_uses[rt] & 1u, &err, DEV_ERR_WAIT_FULL);
+                        ++q_uses[rt];
+                        if (!ok) break;
+                    }
+                    const bool frees = !in_step || x == 1;
+                    for (int u = 0; u < C::UNITS && ok; ++u) {
+                        const uint32_t q = k_seq(tile) + u, slot = q % C::SLOTS;
+                        ok = mbar_wait_warp(&full[slot], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_FULL);
+                        if (!ok) break;
+                        fence_after_sync();
+                        if (elect_one()) {
+                            const uint32_t k_a = ring_a + slot * C::SLOT, a = q_a + rt * C::Q_BYTES + u * (C::UNIT / 64) * BA_BOX;
+#pragma unroll
+                            for (int j = 0; j < C::UNIT / 16; ++j) {
+                                const uint32_t at = (uint32_t)(j >> 2) * BA_BOX + (uint32_t)(j & 3) * 32u;
+                                mma_ss(tmem + C::TM_S + 128u * (uint32_t)x, swizzled_desc(a + at, 16), swizzled_desc(k_a + at, 16), ID_S, u > 0 || j > 0 ? 1u : 0u);
+                            }
+                            if (frees) mma_commit(&empty[slot]);
+                            if (u == C::UNITS - 1) mma_commit(&s_full[bar_of(it.two, t)]);
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+            even += (uint32_t)(it.steps + 1) / 2;
+            (it.two ? odd : alone) += (uint32_t)it.steps / 2;
+            seq += 2u * C::UNITS * (uint32_t)it.tiles;
+        }
+    } else if (warp == 9) {
+        // ================= producer =================
+        uint32_t seq = 0, tails = 0;
+        bool ok = true;
+        for (uint32_t idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
+            const Item it = item_of<D>(p, idx);
+            const bool in_step = it.two && !it.pair;
+            const int n_p = it.p1 - it.p0;
+            auto load = [&](int tile, bool is_v) {
+                const bool pre = tile < n_p;
+                const int key = (pre ? it.p0 + tile : it.o0 + tile - n_p) * BA_KEYS;
+                const int valid = pre ? BA_KEYS : it.own - key;   // behind the prefix and the capacity TMA itself fills in zeros
+                const bool cut = is_v && valid < BA_KEYS && it.own < p.cap;
+                const CUtensorMap* map = pre ? (is_v ? &map_pv : &map_pk) : (is_v ? &map_ov : &map_ok);
+                for (int u = 0; u < C::UNITS && ok; ++u, ++seq) {
+                    const uint32_t slot = seq % C::SLOTS;
+                    if (seq >= (uint32_t)C::SLOTS) ok = mbar_wait_warp(&empty[slot], (seq / C::SLOTS - 1) & 1u, &err, DEV_ERR_WAIT_EMPTY);
+                    if (!ok) break;
+                    uint64_t* bar = cut ? tail : &full[slot];
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(bar, C::SLOT);
+#pragma unroll
+                        for (int j = 0; j < C::UNIT / 64; ++j) {
+                            uint8_t* dst = ring + slot * C::SLOT + j * BA_BOX;
+                            const int x = u * C::UNIT + 64 * j;
+                            if (pre) tma_load_3d(dst, map, x, (int)it.h, key, bar);
+                            else tma_load_4d(dst, map, x, (int)it.h, key, (int)it.b, bar);
+                        }
+                    }
+                    __syncwarp();
+                    if (cut) {   // rows behind the request's last: a weight of zero times whatever they hold has to be zero
+                        ok = mbar_wait_warp(tail, tails & 1u, &err, DEV_ERR_WAIT_FULL);
+                        ++tails;
+                        if (!ok) break;
+                        for (int j = 0; j < C::UNIT / 64; ++j)
+                            for (int i = valid * 8 + lane; i < BA_KEYS * 8; i += 32)
+                                *reinterpret_cast<uint4*>(ring + slot * C::SLOT + j * BA_BOX + i * 16) = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&full[slot]);
+                    }
+                }
+            };
+            if (in_step) {
+                for (int i = 0; i < it.tiles && ok; ++i) {
+                    load(i, false);
+                    load(i, true);
+                }
+            } else if (it.tiles > 0) {
+                load(0, false);
+                for (int i = 0; i < it.tiles && ok; ++i) {
+                    if (i + 1 < it.tiles) load(i + 1, false);
+                    load(i, true);
+                }
+            }
+        }
+        // nothing may still be in flight into this CTA's shared memory when it leaves
+        for (uint32_t q = seq > (uint32_t)C::SLOTS ? seq - C::SLOTS : 0; q < seq; ++q)
+            mbar_wait_warp(&full[q % C::SLOTS], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_DRAIN);
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == 8) {
+        fence_after_sync();
+        tmem_free(tmem, 512);
+    }
+}
+
+// Joins the parts of a row: a warp a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) batch_attn_join_kernel(const __grid_constant__ BatchAttnParams p) {
     pdl_prologue();
     constexpr int E = D / 32;
-    const uint64_t r = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const uint64_t idx = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const uint32_t lane = threadIdx.x & 31;
-    if (r >= (uint64_t)p.batch * p.n * p.n_q) return;
-    const uint32_t h = (uint32_t)(r % p.n_q), i = (uint32_t)(r / p.n_q % p.n), b = (uint32_t)(r / p.n_q / p.n), kvh = h / p.group;
-    const int rows = q_len_of(p, b), own = own_len_of(p, b);
-    if ((int)i >= rows) return;
-    const int seen = min(own, max(0, own - rows + (int)i + 1));
-    float q[E], o[E] = {}, m = -INFINITY, l = 0.f;
-    const T* qp = static_cast<const T*>(p.q) + b * p.q_b + i * p.q_t + h * p.q_h + lane * E;
-    for (int e = 0; e < E; ++e) q[e] = (float)qp[e] * p.scale;
-    for (int64_t j = 0; j < (int64_t)p.prefix + seen; ++j) {
-        const T *k, *v;
-        if (j < p.prefix) {
-            k = static_cast<const T*>(p.pk) + j * p.pk_r + kvh * p.pk_h;
-            v = static_cast<const T*>(p.pv) + j * p.pv_r + kvh * p.pv_h;
-        } else {
-            k = static_cast<const T*>(p.ok) + b * p.ok_b + (j - p.prefix) * p.ok_r + kvh * p.ok_h;
-            v = static_cast<const T*>(p.ov) + b * p.ov_b + (j - p.prefix) * p.ov_r + kvh * p.ov_h;
-        }
-        float s = 0.f;
-        for (int e = 0; e < E; ++e) s += q[e] * (float)k[lane * E + e];
-        s = warp_sum(s);
-        if (s == -INFINITY) continue;
-        const float top = fmaxf(m, s), f = m == -INFINITY ? 0.f : expf(m - top), w = expf(s - top);
-        l = l * f + w;
-        for (int e = 0; e < E; ++e) o[e] = o[e] * f + w * (float)v[lane * E + e];
-        m = top;
+    if (idx >= (uint64_t)p.rows * p.n_kv) return;
+    const uint32_t h = (uint32_t)(idx / p.rows), r = (uint32_t)(idx % p.rows), per = p.n * p.group, b = r / per, rem = r - b * per, tok = rem / p.group;
+    const int q_len = q_len_of(p, b);
+    if ((int)tok >= q_len) return;
+    // the parts that were written: all of the prefix's; of the own keys those that begin ahead of the last key the row's block sees
+    uint32_t n = p.p_parts;
+    if (p.o_splits > 0) {
+        const int own = own_len_of(p, b);
+        const uint32_t block = (p.o_pair || D > 128 ? BA_ROWS : 2 * BA_ROWS), first = rem / block * block, last = min(first + block, (uint32_t)q_len * p.group);
+        const int seen = min(own, max(0, own - q_len + (int)((last - 1) / p.group) + 1));
+        const uint32_t tiles = (p.fused ? p.prefix_tiles : 0u) + (uint32_t)(seen + BA_KEYS - 1) / BA_KEYS;
+        n += (tiles + p.o_run - 1) / p.o_run * (p.o_pair ? 2u : 1u);
     }
-    T* dst = static_cast<T*>(p.out) + b * p.o_b + i * p.o_t + h * p.o_h + lane * E;
-    for (int e = 0; e < E; ++e) dst[e] = (T)(l == 0.f ? 0.f : o[e] / l);
+    const float c = p.scale * 1.4426950408889634f;
+    const uint64_t at = (uint64_t)h * p.rows + r, step = (uint64_t)p.n_kv * p.rows;
+    float top = -INFINITY;
+    for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[i * step + at].x);
+    top = warp_max(top);
+    float l = 0.f, o[E] = {};
+    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+        float w = 0.f, li = 0.f;
+        if (i0 + lane < n) {
+            const float2 ml = p.part_ml[(i0 + lane) * step + at];
+            w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : ex2((ml.x - top) * c);   // a NaN sum without a maximum: the item gave up
+            li = w * ml.y;
+            if (ml.x == -INFINITY) li = ml.y;
+        }
+        l += warp_sum(li);
+        const unsigned some = __ballot_sync(0xffffffffu, w != 0.f);
+        for (unsigned left = some; left; left &= left - 1) {
+            const int i = __ffs(left) - 1;
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            if (!(wi == wi)) continue;
+            const float* src = p.part_o + ((i0 + i) * step + at) * D + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += wi * src[e];
+        }
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    T* dst = static_cast<T*>(p.out) + b * p.o_b + tok * p.o_t + (h * p.group + rem - tok * p.group) * p.o_h + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = Pair16<T>::pack(l == 0.f ? 0.f : o[e] * inv, l == 0.f ? 0.f : o[e + 1] * inv);
 }
 
 dfl_status check(const dfl_prefix_attention_args* a, BatchAttnParams* p) {
@@ -96,16 +626,117 @@ dfl_status check(const dfl_prefix_attention_args* a, BatchAttnParams* p) {
     p->batch = a->batch, p->n = a->n_tokens, p->n_q = a->n_q_heads, p->n_kv = a->n_kv_heads, p->group = a->n_q_heads / a->n_kv_heads;
     p->prefix = (int32_t)a->prefix_len, p->cap = (int32_t)a->own_capacity;
     p->scale = a->scale;
+    // every key has a place of its own for the copy engine: an expanded dimension has not
+    if ((a->prefix_len > 1 && (!p->pk_r || !p->pv_r)) || (pre && heads && (!p->pk_h || !p->pv_h)) || (a->own_capacity > 1 && (!p->ok_r || !p->ov_r)) ||
+        (own && heads && (!p->ok_h || !p->ov_h)) || (own && a->batch > 1 && (!p->ok_b || !p->ov_b)))
+        return fail(DFL_ERR_BAD_SHAPE, "prefix_attention: a stride of K or V is zero");
     return DFL_OK;
 }
 
+// How the work is cut.  Times in microseconds, measured on B200: a key tile against two row tiles 1.2, against one 0.6 (head width 128), an item's
+// start and end 4, a byte of a part written and read again 1 / 4e6.
+uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+void plan(const dfl_prefix_attention_args* a, BatchAttnParams* p, int sms) {
+    const uint32_t D = a->head_dim, block = D <= 128 ? 2 * BA_ROWS : BA_ROWS, per = p->n * p->group;
+    p->rows = p->batch * per;
+    p->prefix_tiles = ceil_div((uint64_t)p->prefix, BA_KEYS);
+    const uint32_t own_tiles = ceil_div((uint64_t)p->cap, BA_KEYS);
+    const double tile1 = 0.6 * D / 128.0, start = 4.0, part_us = 8.0 * D / 4e6;
+    // requests that fill their row blocks to four fifths take prefix and own keys in one go
+    const uint32_t o_block = D <= 128 && per <= BA_ROWS ? BA_ROWS : block;
+    const uint32_t o_blocks = ceil_div(per, o_block);
+    p->fused = 5ull * per >= 4ull * o_blocks * o_block && p->prefix_tiles > 0 && own_tiles > 0;
+    auto splits_for = [&](uint64_t items, uint32_t tiles, double tile_us, double part_cost) {
+        if (items > 64ull * sms) return 1u;
+        uint32_t best = 1u;
+        double best_us = 1e30;
+        for (uint32_t s = 1; s <= tiles && s <= 64; ++s) {
+            const uint32_t run = ceil_div(tiles, s);
+            if (ceil_div(tiles, run) != s) continue;
+            const double us = ceil_div(items * s, (uint64_t)sms) * (run * tile_us + start) + s * part_cost;
+            if (us < best_us * 0.98) best_us = us, best = s;
+        }
+        return best;
+    };
+    p->p_items = p->p_blocks = p->p_splits = p->p_run = p->p_parts = 0;
+    p->o_blocks = p->o_splits = p->o_run = 0;
+    p->p_pair = D <= 128 && p->rows <= BA_ROWS;
+    p->o_pair = D <= 128 && per <= BA_ROWS;
+    const double part_cost = (double)p->rows * p->n_kv * part_us;
+    if (p->prefix_tiles > 0 && !p->fused) {
+        p->p_blocks = ceil_div(p->rows, p->p_pair ? BA_ROWS : block);
+        const uint64_t items = (uint64_t)p->p_blocks * p->n_kv;
+        const double tile_us = D <= 128 && !p->p_pair ? 2 * tile1 : tile1;
+        p->p_splits = splits_for(items, p->prefix_tiles, tile_us, part_cost * (p->p_pair ? 2 : 1));
+        p->p_run = ceil_div(p->prefix_tiles, p->p_splits);
+        p->p_items = (uint32_t)(items * p->p_splits);
+        p->p_parts = p->p_splits * (p->p_pair ? 2 : 1);
+    }
+    uint64_t o_items = 0;
+    if (own_tiles > 0 || p->prefix_tiles == 0) {
+        const uint32_t tiles = own_tiles + (p->fused ? p->prefix_tiles : 0);
+        p->o_blocks = o_blocks;
+        const uint64_t items = (uint64_t)p->batch * p->n_kv * o_blocks;
+        const double tile_us = D <= 128 && !p->o_pair ? 2 * tile1 : tile1;
+        p->o_splits = tiles > 0 ? splits_for(items, tiles, tile_us, part_cost * (p->o_pair ? 2 : 1)) : 1;
+        p->o_run = tiles > 0 ? ceil_div(tiles, p->o_splits) : 1;
+        o_items = items * p->o_splits;
+    }
+    p->items = p->p_items + (uint32_t)o_items;
+    p->parts = p->p_parts + p->o_splits * (p->o_pair ? 2 : 1);
+    p->direct = p->parts == 1;
+}
+
+uint64_t ml_bytes(const BatchAttnParams& p) { return ((uint64_t)p.parts * p.n_kv * p.rows * sizeof(float2) + 255) / 256 * 256; }
+uint64_t workspace_bytes(const BatchAttnParams& p, uint32_t dim) {
+    return p.direct ? 0 : ml_bytes(p) + (uint64_t)p.parts * p.n_kv * p.rows * dim * sizeof(float);
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_fn() {
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) f = nullptr;
+        cudaGetLastError();
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+// boxes of 128 rows x 64 dimensions of one head; dimensions (dim, head, row[, request])
+dfl_status make_map(CUtensorMap* map, const void* base, int32_t dtype, uint32_t dim, uint32_t heads, uint64_t rows, uint32_t batch, int64_t head_stride, int64_t row_stride,
+                    int64_t batch_stride, int rank) {
+    const EncodeTiled encode = encode_fn();
+    if (!encode) return fail(DFL_ERR_CUDA, "prefix_attention: the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t own = (cuuint64_t)dim * 2;   // stands in for the stride of a dimension with one entry
+    const cuuint64_t dims[4] = {dim, heads, rows, batch};
+    const cuuint64_t strides[3] = {heads > 1 ? (cuuint64_t)head_stride * 2 : own, rows > 1 ? (cuuint64_t)row_stride * 2 : own, batch > 1 ? (cuuint64_t)batch_stride * 2 : own};
+    const cuuint32_t box[4] = {64, 1, BA_KEYS, 1}, unit[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, dtype == DFL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides,
+                              box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(DFL_ERR_BAD_SHAPE, "prefix_attention: cuTensorMapEncodeTiled refused the layout (" + std::to_string((int)r) + ")");
+    return DFL_OK;
+}
+
+template <typename T, int D>
+dfl_status launch(const BatchAttnParams& p, const CUtensorMap (&m)[4], int sms, cudaStream_t st) {
+    DFL_CUDA(cudaFuncSetAttribute(batch_attn_t5_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, BaCfg<D>::SMEM));
+    const uint32_t grid = p.items < (uint32_t)sms ? p.items : (uint32_t)sms;
+    DFL_CUDA(launch_k(batch_attn_t5_kernel<T, D>, dim3(grid), dim3(BA_THREADS), BaCfg<D>::SMEM, st, p, m[0], m[1], m[2], m[3]));
+    count_launch();
+    if (!p.direct) {
+        DFL_CUDA(launch_k(batch_attn_join_kernel<T, D>, dim3(ceil_div((uint64_t)p.rows * p.n_kv, 8)), dim3(256), 0, st, p));
+        count_launch();
+    }
+    return DFL_OK;
+}
 template <typename T>
-cudaError_t launch_rows(const BatchAttnParams& p, uint32_t dim, cudaStream_t st) {
-    const uint64_t rows = (uint64_t)p.batch * p.n * p.n_q;
-    const dim3 grid((unsigned)((rows + 7) / 8));
-    if (dim == 64) return launch_k(batch_attn_row_kernel<T, 64>, grid, dim3(256), 0, st, p);
-    if (dim == 128) return launch_k(batch_attn_row_kernel<T, 128>, grid, dim3(256), 0, st, p);
-    return launch_k(batch_attn_row_kernel<T, 256>, grid, dim3(256), 0, st, p);
+dfl_status launch_dim(const BatchAttnParams& p, const CUtensorMap (&m)[4], uint32_t dim, int sms, cudaStream_t st) {
+    if (dim == 64) return launch<T, 64>(p, m, sms, st);
+    if (dim == 128) return launch<T, 128>(p, m, sms, st);
+    return launch<T, 256>(p, m, sms, st);
 }
 
 }  // namespace
@@ -113,9 +744,14 @@ cudaError_t launch_rows(const BatchAttnParams& p, uint32_t dim, cudaStream_t st)
 
 extern "C" dfl_status dfl_prefix_attention_workspace(int32_t device, const dfl_prefix_attention_args* a, uint64_t* bytes_out) {
     using namespace dfl;
-    if (!a || !bytes_out) return fail(DFL_ERR_BAD_ARG, "prefix_attention_workspace: null argument");
-    (void)device;
+    if (!bytes_out) return fail(DFL_ERR_BAD_ARG, "prefix_attention_workspace: null argument");
+    BatchAttnParams p;
+    DFL_CHECK(check(a, &p));
+    DFL_CHECK(use_device(device));
     *bytes_out = 0;
+    if (a->batch == 0 || a->n_tokens == 0) return DFL_OK;
+    plan(a, &p, sm_count());
+    *bytes_out = workspace_bytes(p, a->head_dim);
     return DFL_OK;
 }
 
@@ -125,8 +761,23 @@ extern "C" dfl_status dfl_prefix_attention(int32_t device, const dfl_prefix_atte
     DFL_CHECK(check(a, &p));
     DFL_CHECK(use_device(device));
     if (a->batch == 0 || a->n_tokens == 0) return DFL_OK;
+    const int sms = sm_count();
+    plan(a, &p, sms);
+    const uint64_t need = workspace_bytes(p, a->head_dim);
+    if (need && (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 256)) return fail(DFL_ERR_BAD_ARG, "prefix_attention: the workspace must be 256-byte aligned");
+    if (a->workspace_bytes < need)
+        return fail(DFL_ERR_BAD_SHAPE, "prefix_attention: the workspace has " + std::to_string(a->workspace_bytes) + " of " + std::to_string(need) + " bytes");
+    p.part_ml = static_cast<float2*>(a->workspace);
+    p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + ml_bytes(p));
+    CUtensorMap m[4] = {};
+    if (p.prefix > 0) {
+        DFL_CHECK(make_map(&m[0], p.pk, a->dtype, a->head_dim, p.n_kv, p.prefix, 1, p.pk_h, p.pk_r, 0, 3));
+        DFL_CHECK(make_map(&m[1], p.pv, a->dtype, a->head_dim, p.n_kv, p.prefix, 1, p.pv_h, p.pv_r, 0, 3));
+    }
+    if (p.cap > 0) {
+        DFL_CHECK(make_map(&m[2], p.ok, a->dtype, a->head_dim, p.n_kv, p.cap, p.batch, p.ok_h, p.ok_r, p.ok_b, 4));
+        DFL_CHECK(make_map(&m[3], p.ov, a->dtype, a->head_dim, p.n_kv, p.cap, p.batch, p.ov_h, p.ov_r, p.ov_b, 4));
+    }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    DFL_CUDA(a->dtype == DFL_F16 ? launch_rows<__half>(p, a->head_dim, st) : launch_rows<__nv_bfloat16>(p, a->head_dim, st));
-    count_launch();
-    return DFL_OK;
+    return a->dtype == DFL_F16 ? launch_dim<__half>(p, m, a->head_dim, sms, st) : launch_dim<__nv_bfloat16>(p, m, a->head_dim, sms, st);
 }

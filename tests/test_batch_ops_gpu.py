@@ -220,6 +220,10 @@ ATTN = [
     (1, 1, 8, 8, 128, 20000, 1000, "f16", "rows"),
     (3, 257, 3, 1, 128, 0, 300, "bf16", "rows"),
     (7, 9, 7, 7, 64, 65, 10, "f16", "heads"),
+    # several items to a CTA, row blocks with both halves and with one in turn
+    (40, 150, 16, 8, 64, 200, 170, "bf16", "rows"),
+    (30, 77, 16, 8, 128, 300, 200, "f16", "rows"),
+    (50, 20, 32, 4, 256, 257, 150, "bf16", "rows"),
 ]
 
 
