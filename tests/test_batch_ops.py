@@ -114,28 +114,33 @@ REFUSED = [
 ]
 
 
+def entry_point(name):
+    f = C.CFUNCTYPE(C.c_int32, C.c_int32, C.c_void_p, C.c_void_p)
+    return f((name, pkg.lib()))
+
+
 @pytest.mark.parametrize("make,entry,change,status", REFUSED, ids=["%s-%s" % (e[4:], "-".join(c)) for _, e, c, _ in REFUSED])
 def test_refused_before_anything_runs(make, entry, change, status):
     with pytest.raises(pkg.DflError) as e:
-        pkg.check(getattr(pkg.lib(), entry)(C.c_int32(0), C.byref(make(**change)), None))
+        pkg.check(entry_point(entry)(0, C.byref(make(**change)), None))
     assert e.value.name == status and entry[4:] in str(e.value)
 
 
 @pytest.mark.parametrize("make,entry", [(rope_args, "dfl_qk_norm_rope"), (attn_args, "dfl_prefix_attention"), (verify_args, "dfl_verify_drafts")])
 def test_null_arguments_and_no_device(make, entry):
     with pytest.raises(pkg.DflError) as e:
-        pkg.check(getattr(pkg.lib(), entry)(C.c_int32(0), None, None))
+        pkg.check(entry_point(entry)(0, None, None))
     assert e.value.name == "BAD_ARG"
     if pkg.device_count() == 0:
         with pytest.raises(pkg.DflError) as e:
-            pkg.check(getattr(pkg.lib(), entry)(C.c_int32(0), C.byref(make()), None))
+            pkg.check(entry_point(entry)(0, C.byref(make()), None))
         assert e.value.name == "NO_DEVICE"
 
 
 def test_wrappers_refuse_what_they_can_see():
     torch = pytest.importorskip("torch")
     q = torch.zeros(2, 4, 64)
-    with pytest.raises(ValueError, match="q: on cpu"):
+    with pytest.raises(ValueError, match="q: on cpu, expected a CUDA device"):
         pkg.qk_norm_rope(q, q, torch.zeros(2, dtype=torch.int32), theta=1e4)
     with pytest.raises(ValueError, match="q: shape"):
         pkg.prefix_attention(q, q, q)
