@@ -45,26 +45,38 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <typename T> struct __align__(4 * sizeof(T)) Quad { T v[4]; };
+// four elements as they lie in memory; unpacked only when they are used, so loads in flight hold no more registers than bytes
+template <typename T> struct Quad;
+template <> struct Quad<float> {
+    float4 r;
+    __device__ __forceinline__ void get(float (&x)[4]) const { x[0] = r.x, x[1] = r.y, x[2] = r.z, x[3] = r.w; }
+    static __device__ __forceinline__ Quad of(const float (&x)[4]) { return Quad{make_float4(x[0], x[1], x[2], x[3])}; }
+};
+template <> struct Quad<__half> {
+    uint2 r;
+    __device__ __forceinline__ void get(float (&x)[4]) const {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+    }
+    static __device__ __forceinline__ Quad of(const float (&x)[4]) {
+        const __half2 a = __floats2half2_rn(x[0], x[1]), b = __floats2half2_rn(x[2], x[3]);
+        return Quad{make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b))};
+    }
+};
+template <> struct Quad<__nv_bfloat16> {
+    uint2 r;
+    __device__ __forceinline__ void get(float (&x)[4]) const {
+        x[0] = __uint_as_float(r.x << 16), x[1] = __uint_as_float(r.x & 0xffff0000u), x[2] = __uint_as_float(r.y << 16), x[3] = __uint_as_float(r.y & 0xffff0000u);
+    }
+    static __device__ __forceinline__ Quad of(const float (&x)[4]) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+        return Quad{make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b))};
+    }
+};
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&x)[4]) {
-    const Quad<T> r = *reinterpret_cast<const Quad<T>*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = to_f<T>(r.v[i]);
-}
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
-    Quad<T> r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = from_f<T>(x[i]);
-    *reinterpret_cast<Quad<T>*>(p) = r;
-}
-
-// cos and sin of one frequency at a token
-__device__ __forceinline__ float2 turn_of(const RopeParams& p, const uint64_t* turn, const uint8_t* axis, uint32_t j, uint32_t token) {
-    const int64_t pos = p.pos[axis[j] * p.pos_axis + token];
-    const uint64_t angle = (uint64_t)pos * turn[j];
+// cos and sin of one frequency at a position
+__device__ __forceinline__ float2 turn_of(int32_t pos, uint64_t turn) {
+    const uint64_t angle = (uint64_t)(int64_t)pos * turn;
     float2 r;
     sincospif((float)(int32_t)(angle >> 32) * 0x1p-31f, &r.y, &r.x);   // half turns in [-1, 1)
     return r;
@@ -135,7 +147,7 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) qk_norm_rope_any_kernel(const
                     const uint32_t f = j < p.half ? j : j - p.half;
                     float out = y[warp][j] * norm * (r.w ? r.w[j] : 1.f);
                     if (r.normed && j < 2 * p.half) {
-                        const float2 t = turn_of(p, turn, axis, f, token);
+                        const float2 t = turn_of(p.pos[axis[f] * p.pos_axis + token], turn[f]);
                         const uint32_t o = j < p.half ? j + p.half : f;
                         const float other = y[warp][o] * norm * (r.w ? r.w[o] : 1.f);
                         out = j < p.half ? out * t.x - other * t.y : out * t.x + other * t.y;
@@ -148,16 +160,139 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) qk_norm_rope_any_kernel(const
     }
 }
 
+// Head widths of 64, 128 and 256: L lanes a head, eight elements a lane in two runs of four that turn together (j and j + half), so no value
+// crosses lanes but the sum of squares.  What bounds it is how much is in flight: U heads' loads a lane group, 64 registers for 32 warps an
+// SM, the next token's positions fetched ahead.
+template <typename S, typename D, int L, bool NORM, int U>
+__device__ __forceinline__ void rope_heads(const S* src, int64_t src_h, D* dst, int64_t dst_h, uint32_t n, uint32_t h0, uint32_t step, uint32_t g, uint32_t c0, uint32_t c1,
+                                           const float* w, float eps, const float (&cs)[4], const float (&sn)[4]) {
+    float wa[4] = {1.f, 1.f, 1.f, 1.f}, wb[4] = {1.f, 1.f, 1.f, 1.f};
+    if (NORM && w && h0 < n) {
+        const float4 x = *reinterpret_cast<const float4*>(w + c0), y = *reinterpret_cast<const float4*>(w + c1);
+        wa[0] = x.x, wa[1] = x.y, wa[2] = x.z, wa[3] = x.w, wb[0] = y.x, wb[1] = y.y, wb[2] = y.z, wb[3] = y.w;
+    }
+    src += (h0 + g) * src_h + c0;
+    dst += (h0 + g) * dst_h + c0;
+    src_h *= step, dst_h *= step, c1 -= c0;
+#pragma unroll 1
+    for (; h0 < n; h0 += U * step, src += U * src_h) {   // h0: the first lane group's head
+        Quad<S> x0[U], x1[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (h0 + u * step + g < n) {
+                x0[u] = *reinterpret_cast<const Quad<S>*>(src + u * src_h);
+                x1[u] = *reinterpret_cast<const Quad<S>*>(src + u * src_h + c1);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (h0 + u * step >= n) break;   // for the whole warp
+            float a[4], b[4];
+            x0[u].get(a);
+            x1[u].get(b);
+            if (NORM) {
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += a[e] * a[e] + b[e] * b[e];
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const float norm = rsqrtf(sum * (1.f / (8 * L)) + eps);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = a[e] * norm * wa[e], z = b[e] * norm * wb[e];
+                    a[e] = y * cs[e] - z * sn[e];
+                    b[e] = z * cs[e] + y * sn[e];
+                }
+            }
+            if (h0 + u * step + g < n) {
+                *reinterpret_cast<Quad<D>*>(dst) = Quad<D>::of(a);
+                *reinterpret_cast<Quad<D>*>(dst + c1) = Quad<D>::of(b);
+                dst += dst_h;
+            }
+        }
+    }
+}
+
+template <typename S, typename D, int L>
+__global__ void __launch_bounds__(32 * ROPE_WARPS, 4) qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
+    constexpr int MAXH = L * 4, PER = (MAXH + 31) / 32;   // frequencies, of a lane
+    __shared__ uint64_t turn[MAXH];
+    __shared__ uint8_t axis[MAXH];
+    __shared__ __align__(16) float2 table[ROPE_WARPS][MAXH];
+    for (uint32_t j = threadIdx.x; j < p.half; j += blockDim.x) turn[j] = p.turn[j], axis[j] = p.axis[j];
+    pdl_prologue();
+    __syncthreads();
+    constexpr uint32_t G = 32 / L;
+    constexpr int U = sizeof(S) == 4 ? 2 : 4;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane / L, i = lane % L;
+    const bool turns = 4 * i < p.half;
+    const uint32_t c0 = turns ? 4 * i : 2 * p.half + 8 * (i - p.half / 4), c1 = turns ? p.half + 4 * i : c0 + 4;
+    // a token's heads in units of one a lane group, q's, k's and v's one behind the other; a warp has every `parts`-th unit
+    const uint32_t uq = (p.n_q + G - 1) / G, uk = (p.n_kv + G - 1) / G;
+    const uint64_t n_items = (uint64_t)p.n_tokens * p.parts, hop = (uint64_t)gridDim.x * ROPE_WARPS;
+    uint64_t item = (uint64_t)blockIdx.x * ROPE_WARPS + warp;
+    int32_t pos[PER];
+    auto fetch = [&](uint64_t it) {
+        const uint32_t token = (uint32_t)(it / p.parts);
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (lane + 32 * k < p.half) pos[k] = p.pos[axis[lane + 32 * k] * p.pos_axis + token];
+    };
+    if (item < n_items) fetch(item);
+    for (; item < n_items; item += hop) {
+        const uint32_t token = (uint32_t)(item / p.parts), part = (uint32_t)(item - (uint64_t)token * p.parts);
+        const int64_t row = p.n_kv ? row_of(p, token) : -1;
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (lane + 32 * k < p.half) table[warp][lane + 32 * k] = turn_of(pos[k], turn[lane + 32 * k]);
+        if (item + hop < n_items) fetch(item + hop);
+        __syncwarp();
+        float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {};
+        if (turns) {
+            const float4 a = *reinterpret_cast<const float4*>(&table[warp][4 * i]), b = *reinterpret_cast<const float4*>(&table[warp][4 * i + 2]);
+            cs[0] = a.x, sn[0] = a.y, cs[1] = a.z, sn[1] = a.w, cs[2] = b.x, sn[2] = b.y, cs[3] = b.z, sn[3] = b.w;
+        }
+        __syncwarp();
+        const uint32_t sk = (part + p.parts - uq % p.parts) % p.parts, sv = (sk + p.parts - uk % p.parts) % p.parts;   // first units of k and v
+        rope_heads<S, D, L, true, U>(static_cast<const S*>(p.q) + token * p.q_t, p.q_h, static_cast<D*>(p.q_out) + token * p.qo_t, p.qo_h, p.n_q, part * G, p.parts * G, g,
+                                     c0, c1, p.qw, p.eps, cs, sn);
+        if (row >= 0) {
+            rope_heads<S, D, L, true, U>(static_cast<const S*>(p.k) + token * p.k_t, p.k_h, static_cast<D*>(p.k_out) + row * p.ko_t, p.ko_h, p.n_kv, sk * G, p.parts * G, g,
+                                         c0, c1, p.kw, p.eps, cs, sn);
+            if (p.v) rope_heads<S, D, L, false, U>(static_cast<const S*>(p.v) + token * p.v_t, p.v_h, static_cast<D*>(p.v_out) + row * p.vo_t, p.vo_h, p.n_kv, sv * G, p.parts * G, g,
+                                                   c0, c1, nullptr, 0.f, cs, sn);
+        }
+    }
+}
+
 bool dtype_ok(int32_t d) { return d == DFL_F32 || d == DFL_F16 || d == DFL_BF16; }
 
+// every address the quad kernel forms is a multiple of four elements
 template <typename S, typename D>
-cudaError_t launch_typed(const RopeParams& p, cudaStream_t st) {
-    const uint64_t items = (uint64_t)p.n_tokens * p.parts;
-    const uint64_t blocks = (items + ROPE_WARPS - 1) / ROPE_WARPS, most = (uint64_t)sm_count() * 8;
-    return launch_k(qk_norm_rope_any_kernel<S, D>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(32 * ROPE_WARPS), 0, st, p);
+bool in_quads(const RopeParams& p) {
+    auto src = [&](const void* x, int64_t a, int64_t b) { return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(S)) == 0 && a % 4 == 0 && b % 4 == 0; };
+    auto dst = [&](const void* x, int64_t a, int64_t b) { return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(D)) == 0 && a % 4 == 0 && b % 4 == 0; };
+    const bool kv = p.n_kv > 0, v = p.n_heads > p.n_q + p.n_kv;
+    return p.half % 4 == 0 && (p.dim == 64 || p.dim == 128 || p.dim == 256) && (!p.n_q || (src(p.q, p.q_t, p.q_h) && dst(p.q_out, p.qo_t, p.qo_h))) &&
+           (!kv || (src(p.k, p.k_t, p.k_h) && dst(p.k_out, p.ko_t, p.ko_h))) && (!v || (src(p.v, p.v_t, p.v_h) && dst(p.v_out, p.vo_t, p.vo_h))) &&
+           reinterpret_cast<uintptr_t>(p.qw) % 16 == 0 && reinterpret_cast<uintptr_t>(p.kw) % 16 == 0;
+}
+template <typename S, typename D>
+cudaError_t launch_typed(RopeParams& p, cudaStream_t st) {
+    const bool quads = in_quads<S, D>(p);
+    // a token's heads are shared out over warps until the machine has eight warps an SM, but a warp keeps a load for each of its lane groups
+    const uint64_t wanted = (uint64_t)sm_count() * 8, parts = (wanted + p.n_tokens - 1) / p.n_tokens;
+    const uint32_t groups = quads ? 256 / p.dim : 1, most_parts = (p.n_q + groups - 1) / groups + (p.n_heads - p.n_q + groups - 1) / groups;
+    p.parts = (uint32_t)(parts < most_parts ? parts : most_parts);
+    const uint64_t items = (uint64_t)p.n_tokens * p.parts, blocks = (items + ROPE_WARPS - 1) / ROPE_WARPS, most = (uint64_t)sm_count() * 4;
+    const dim3 grid((unsigned)(blocks < most ? blocks : most)), block(32 * ROPE_WARPS);
+    if (!quads) return launch_k(qk_norm_rope_any_kernel<S, D>, grid, block, 0, st, p);
+    if (p.dim == 64) return launch_k(qk_norm_rope_kernel<S, D, 8>, grid, block, 0, st, p);
+    if (p.dim == 128) return launch_k(qk_norm_rope_kernel<S, D, 16>, grid, block, 0, st, p);
+    return launch_k(qk_norm_rope_kernel<S, D, 32>, grid, block, 0, st, p);
 }
 template <typename S>
-cudaError_t launch_src(const RopeParams& p, int32_t dst, cudaStream_t st) {
+cudaError_t launch_src(RopeParams& p, int32_t dst, cudaStream_t st) {
     if (dst == DFL_F32) return launch_typed<S, float>(p, st);
     if (dst == DFL_F16) return launch_typed<S, __half>(p, st);
     return launch_typed<S, __nv_bfloat16>(p, st);
@@ -197,7 +332,7 @@ extern "C" dfl_status dfl_qk_norm_rope(int32_t device, const dfl_qk_norm_rope_ar
     }
     DFL_CHECK(use_device(device));
     RopeParams p = {};
-    p.q = a->q, p.k = a->k, p.v = a->v, p.q_out = a->q_out, p.k_out = a->k_out, p.v_out = a->v_out;
+    p.q = a->q, p.k = a->k, p.v = has_v ? a->v : nullptr, p.q_out = a->q_out, p.k_out = a->k_out, p.v_out = a->v_out;
     p.qw = a->q_weight, p.kw = a->k_weight, p.pos = a->positions, p.rows = a->kv_rows;
     const bool one_q = a->n_q_heads <= 1, one_k = a->n_kv_heads <= 1, one_t = a->n_tokens <= 1, one_r = a->n_kv_out_rows <= 1;
     p.q_t = one_t ? 0 : a->q_token_stride, p.q_h = one_q ? 0 : a->q_head_stride;
@@ -226,10 +361,6 @@ extern "C" dfl_status dfl_qk_norm_rope(int32_t device, const dfl_qk_norm_rope_ar
             p.axis[j] = (uint8_t)owner;
         }
     }
-    // a token's heads are shared out until the machine has eight warps an SM
-    const uint64_t wanted = (uint64_t)sm_count() * 8;
-    const uint64_t parts = (wanted + p.n_tokens - 1) / p.n_tokens;
-    p.parts = (uint32_t)(parts < p.n_heads ? parts : p.n_heads);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (a->src_dtype == DFL_F32) e = launch_src<float>(p, a->dst_dtype, st);

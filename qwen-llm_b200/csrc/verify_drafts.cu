@@ -49,42 +49,86 @@ template <> __device__ __forceinline__ float logit<__nv_bfloat16>(const void* ba
 
 __device__ __forceinline__ float temperature_of(const VerifyParams& p, uint32_t b) { return p.temperature ? p.temperature[b] : 1.f; }
 
-// the larger maximum first, the lower index among equals; sums are brought to it
-__device__ __forceinline__ Piece merge(const Piece& a, const Piece& b, float c) {
-    const bool a_first = a.top > b.top || (a.top == b.top && a.first < b.first);
-    const Piece &x = a_first ? a : b, &y = a_first ? b : a;
-    return Piece{x.top, x.sum + (y.top == -INFINITY ? y.sum : y.sum * exp2f((y.top - x.top) * c)), x.first, 0};
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// the logits of a 16-byte piece, -inf where there is none
+template <typename T> __device__ __forceinline__ void unpack_logits(const uint4& w, bool in, float* x);
+template <> __device__ __forceinline__ void unpack_logits<float>(const uint4& w, bool in, float* x) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = in ? __uint_as_float(u[e]) : -INFINITY;
+}
+template <> __device__ __forceinline__ void unpack_logits<__half>(const uint4& w, bool in, float* x) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+        x[2 * e] = in ? f.x : -INFINITY, x[2 * e + 1] = in ? f.y : -INFINITY;
+    }
+}
+template <> __device__ __forceinline__ void unpack_logits<__nv_bfloat16>(const uint4& w, bool in, float* x) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[2 * e] = in ? __uint_as_float(u[e] << 16) : -INFINITY, x[2 * e + 1] = in ? __uint_as_float(u[e] & 0xffff0000u) : -INFINITY;
 }
 
-// grid pieces x batch x rows, rows outermost
+// 32 logits a thread in 16-byte pieces, all in flight at once; what lies beside the aligned range of the row (at most seven logits at either end)
+// belongs to the first and the last piece.  Grid pieces x batch x rows, rows outermost.
 template <typename T>
 __global__ void __launch_bounds__(ST_THREADS) verify_pieces_kernel(const __grid_constant__ VerifyParams p) {
     pdl_prologue();
+    constexpr int VE = 16 / sizeof(T), NV = 32 / VE;   // logits of a vector, vectors of a thread
     __shared__ Piece warps[ST_THREADS / 32];
     const uint32_t piece = blockIdx.x % p.n_pieces, b = blockIdx.x / p.n_pieces % p.batch, r = blockIdx.x / p.n_pieces / p.batch;
-    const uint32_t lo = piece * p.piece, hi = min(p.vocab, lo + p.piece);
     const float t = temperature_of(p, b), c = t > 0.f ? fminf(1.44269504f / t, 3e38f) : 1.f;   // finite: 0 * c has to stay 0
-    const int64_t row = b * p.x_b + r * p.x_r;
-    Piece a{-INFINITY, 0.f, 0x7fffffff, 0};
-    for (uint32_t i = lo + threadIdx.x; i < hi; i += ST_THREADS) {
-        const float x = logit<T>(p.logits, row + i);
-        if (x != x || x == INFINITY) a.sum = NAN;
-        else if (x > a.top) a = Piece{x, a.sum * exp2f((a.top - x) * c) + 1.f, (int32_t)i, 0};
-        else if (x != -INFINITY) a.sum += exp2f((x - a.top) * c);
-    }
+    const T* row = static_cast<const T*>(p.logits) + b * p.x_b + r * p.x_r;
+    const uint32_t head = min(p.vocab, (uint32_t)((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T)));   // logits ahead of the first vector
+    const uint32_t n_vec = (p.vocab - head) / VE, v0 = piece * (p.piece / VE), v1 = piece + 1 == p.n_pieces ? n_vec : min(n_vec, v0 + p.piece / VE);
+    float x[32], extra = -INFINITY;
+    uint32_t extra_at = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Piece y;
-        y.top = __shfl_xor_sync(0xffffffffu, a.top, o);
-        y.sum = __shfl_xor_sync(0xffffffffu, a.sum, o);
-        y.first = __shfl_xor_sync(0xffffffffu, a.first, o);
-        a = merge(a, y, c);
+    for (int j = 0; j < NV; ++j) {
+        const uint32_t v = v0 + threadIdx.x + j * ST_THREADS;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        const bool in = v < v1;
+        if (in) w = __ldcs(reinterpret_cast<const uint4*>(row + head) + v);
+        unpack_logits<T>(w, in, &x[j * VE]);
+    }
+    if (piece == 0 && threadIdx.x < head) extra_at = threadIdx.x, extra = logit<T>(row, extra_at);
+    if (piece + 1 == p.n_pieces && threadIdx.x >= 32 && threadIdx.x - 32 < p.vocab - head - n_vec * VE) {
+        extra_at = head + n_vec * VE + threadIdx.x - 32;
+        extra = logit<T>(row, extra_at);
+    }
+    float top = extra;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) top = fmaxf(top, x[j]);
+    const float mine = top;
+    top = warp_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = ex2((extra - base) * c);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) sum += ex2((x[j] - base) * c);   // NaN for a NaN and for +inf
+    Piece a{top, warp_sum(sum), 0x7fffffff, 0};
+    if (t == 0.f) {   // greedy: the first index of the maximum
+        if (mine == top) {
+            if (extra == top) a.first = (int32_t)extra_at;
+#pragma unroll
+            for (int j = 31; j >= 0; --j)
+                if (x[j] == top) a.first = min(a.first, (int32_t)(head + (v0 + threadIdx.x + (j / VE) * ST_THREADS) * VE + j % VE));
+        }
+        a.first = __reduce_min_sync(0xffffffffu, a.first);
     }
     if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = a;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < ST_THREADS / 32; ++w) a = merge(a, warps[w], c);
-        p.pieces[((uint64_t)b * p.rows + r) * p.n_pieces + piece] = a;
+    if (threadIdx.x < 32) {
+        a = threadIdx.x < ST_THREADS / 32 ? warps[threadIdx.x] : Piece{-INFINITY, 0.f, 0x7fffffff, 0};
+        const float all = warp_max(a.top);
+        a.sum = warp_sum(a.top == -INFINITY ? a.sum : a.sum * ex2((a.top - all) * c));
+        a.first = __reduce_min_sync(0xffffffffu, a.top == all ? a.first : 0x7fffffff);
+        if (threadIdx.x == 0) p.pieces[((uint64_t)b * p.rows + r) * p.n_pieces + piece] = Piece{all, a.sum, a.first, 0};
     }
 }
 
@@ -265,9 +309,7 @@ struct Split {
     uint32_t piece, n_pieces;
 };
 Split split_of(const dfl_verify_drafts_args* a) {
-    // pieces of 16 K logits; of 4 K while that leaves the machine short of CTAs
-    const uint64_t rows = (uint64_t)a->batch * (a->n_drafts + 1);
-    const uint32_t piece = rows * ((a->vocab + 16383) / 16384) < 592 ? 4096 : 16384;
+    constexpr uint32_t piece = ST_THREADS * 32;
     return Split{piece, (uint32_t)((a->vocab + piece - 1) / piece)};
 }
 
