@@ -160,122 +160,182 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) qk_norm_rope_any_kernel(const
     }
 }
 
-// Head widths of 64, 128 and 256: L lanes a head, eight elements a lane in two runs of four that turn together (j and j + half), so no value
-// crosses lanes but the sum of squares.  What bounds it is how much is in flight: U heads' loads a lane group, 64 registers for 32 warps an
-// SM, the next token's positions fetched ahead.
-template <typename S, typename D, int L, bool NORM, int U>
-__device__ __forceinline__ void rope_heads(const S* src, int64_t src_h, D* dst, int64_t dst_h, uint32_t n, uint32_t h0, uint32_t step, uint32_t g, uint32_t c0, uint32_t c1,
-                                           const float* w, float eps, const float (&cs)[4], const float (&sn)[4]) {
-    float wa[4] = {1.f, 1.f, 1.f, 1.f}, wb[4] = {1.f, 1.f, 1.f, 1.f};
-    if (NORM && w && h0 < n) {
-        const float4 x = *reinterpret_cast<const float4*>(w + c0), y = *reinterpret_cast<const float4*>(w + c1);
-        wa[0] = x.x, wa[1] = x.y, wa[2] = x.z, wa[3] = x.w, wb[0] = y.x, wb[1] = y.y, wb[2] = y.z, wb[3] = y.w;
-    }
-    src += (h0 + g) * src_h + c0;
-    dst += (h0 + g) * dst_h + c0;
-    src_h *= step, dst_h *= step, c1 -= c0;
-#pragma unroll 1
-    for (; h0 < n; h0 += U * step, src += U * src_h) {   // h0: the first lane group's head
-        Quad<S> x0[U], x1[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (h0 + u * step + g < n) {
-                x0[u] = *reinterpret_cast<const Quad<S>*>(src + u * src_h);
-                x1[u] = *reinterpret_cast<const Quad<S>*>(src + u * src_h + c1);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (h0 + u * step >= n) break;   // for the whole warp
-            float a[4], b[4];
-            x0[u].get(a);
-            x1[u].get(b);
-            if (NORM) {
-                float sum = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum += a[e] * a[e] + b[e] * b[e];
-#pragma unroll
-                for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                const float norm = rsqrtf(sum * (1.f / (8 * L)) + eps);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float y = a[e] * norm * wa[e], z = b[e] * norm * wb[e];
-                    a[e] = y * cs[e] - z * sn[e];
-                    b[e] = z * cs[e] + y * sn[e];
-                }
-            }
-            if (h0 + u * step + g < n) {
-                *reinterpret_cast<Quad<D>*>(dst) = Quad<D>::of(a);
-                *reinterpret_cast<Quad<D>*>(dst + c1) = Quad<D>::of(b);
-                dst += dst_h;
-            }
-        }
-    }
+// Head widths of 64, 128 and 256.  A token's heads go by in units of 32 lanes x 8 elements (G heads of L lanes), q's, k's and v's one behind the
+// other; a warp has every `parts`-th unit of its tokens.  What bounds it is how much is in flight: a warp keeps three stages of 2 KB of units on
+// their way into its own piece of shared memory (16-byte asynchronous copies, across the borders of tokens), 24 warps an SM.
+// A lane takes two runs of four elements that turn together (j and j + half), so no value crosses lanes but the sum of squares; weight and angle
+// are one factor, made once a token, and everything runs on pairs of f32.
+constexpr int ROPE_STAGES = 4, ROPE_STAGE_BYTES = 2048;
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
 template <typename S, typename D, int L>
-__global__ void __launch_bounds__(32 * ROPE_WARPS, 4) qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(32 * ROPE_WARPS, 3) qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
     constexpr int MAXH = L * 4, PER = (MAXH + 31) / 32;   // frequencies, of a lane
+    constexpr uint32_t G = 32 / L, DIM = 8 * L;
+    constexpr int UNIT = 256 * sizeof(S), U = ROPE_STAGE_BYTES / UNIT, CHUNK = 16 / sizeof(S);   // bytes of a unit, units of a stage, elements of a copy
+    extern __shared__ __align__(128) uint8_t stages[];   // [warps][stages][U units]
     __shared__ uint64_t turn[MAXH];
     __shared__ uint8_t axis[MAXH];
     __shared__ __align__(16) float2 table[ROPE_WARPS][MAXH];
     for (uint32_t j = threadIdx.x; j < p.half; j += blockDim.x) turn[j] = p.turn[j], axis[j] = p.axis[j];
     pdl_prologue();
     __syncthreads();
-    constexpr uint32_t G = 32 / L;
-    constexpr int U = sizeof(S) == 4 ? 2 : 4;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane / L, i = lane % L;
     const bool turns = 4 * i < p.half;
     const uint32_t c0 = turns ? 4 * i : 2 * p.half + 8 * (i - p.half / 4), c1 = turns ? p.half + 4 * i : c0 + 4;
-    // a token's heads in units of one a lane group, q's, k's and v's one behind the other; a warp has every `parts`-th unit
-    const uint32_t uq = (p.n_q + G - 1) / G, uk = (p.n_kv + G - 1) / G;
+    uint8_t* ring = stages + warp * (ROPE_STAGES * ROPE_STAGE_BYTES);
     const uint64_t n_items = (uint64_t)p.n_tokens * p.parts, hop = (uint64_t)gridDim.x * ROPE_WARPS;
-    uint64_t item = (uint64_t)blockIdx.x * ROPE_WARPS + warp;
+    const uint32_t uq = (p.n_q + G - 1) / G, uk = (p.n_kv + G - 1) / G, kinds = p.v ? 3 : p.n_kv ? 2 : 1;
+
+    // a walk over the units: item (token and share), kind (q, k, v), first head
+    struct Walk {
+        uint64_t item;
+        uint32_t token, kind, h, n;   // n: heads of the kind
+    };
+    const uint32_t step = p.parts * G;
+    auto settle = [&](Walk& w) {      // on to a kind and an item that has units
+        while (w.h >= w.n) {
+            if (++w.kind < kinds) {
+                const uint32_t before = w.kind == 1 ? uq : uq + uk, part = (uint32_t)(w.item - (uint64_t)w.token * p.parts);
+                w.n = p.n_kv;
+                w.h = (part + p.parts - before % p.parts) % p.parts * G;
+            } else {
+                w.item += hop;
+                if (w.item >= n_items) return;
+                w.token = (uint32_t)(w.item / p.parts);
+                w.kind = 0;
+                w.n = p.n_q;
+                w.h = (uint32_t)(w.item - (uint64_t)w.token * p.parts) * G;
+            }
+        }
+    };
+    auto start = [&]() {
+        Walk w;
+        w.item = (uint64_t)blockIdx.x * ROPE_WARPS + warp;
+        w.kind = 0, w.n = p.n_q, w.token = 0, w.h = 0;
+        if (w.item < n_items) {
+            w.token = (uint32_t)(w.item / p.parts);
+            w.h = (uint32_t)(w.item - (uint64_t)w.token * p.parts) * G;
+            settle(w);
+        }
+        return w;
+    };
+    Walk in = start(), at = in;
+    uint32_t slot_in = 0, slot_at = 0;
+    auto issue = [&]() {
+        if (in.item < n_items) {
+            const S* src = in.kind == 0 ? static_cast<const S*>(p.q) + in.token * p.q_t : in.kind == 1 ? static_cast<const S*>(p.k) + in.token * p.k_t : static_cast<const S*>(p.v) + in.token * p.v_t;
+            const int64_t hs = in.kind == 0 ? p.q_h : in.kind == 1 ? p.k_h : p.v_h;
+#pragma unroll
+            for (int j = 0; j < ROPE_STAGE_BYTES / 512; ++j) {   // 16 bytes a lane at a time
+                const uint32_t e = (lane + 32 * j) * CHUNK, u = e / 256, h = in.h + u * step + e % 256 / DIM;   // element of the stage, its unit and head
+                if (h < in.n) copy16(ring + slot_in * ROPE_STAGE_BYTES + (lane + 32 * j) * 16, src + h * hs + e % DIM);
+            }
+            in.h += U * step;
+            settle(in);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        slot_in = slot_in + 1 == ROPE_STAGES ? 0 : slot_in + 1;
+    };
     int32_t pos[PER];
-    auto fetch = [&](uint64_t it) {
-        const uint32_t token = (uint32_t)(it / p.parts);
+    auto fetch = [&](uint64_t item) {
+        const uint32_t token = (uint32_t)(item / p.parts);
 #pragma unroll
         for (int k = 0; k < PER; ++k)
             if (lane + 32 * k < p.half) pos[k] = p.pos[axis[lane + 32 * k] * p.pos_axis + token];
     };
-    if (item < n_items) fetch(item);
-    for (; item < n_items; item += hop) {
-        const uint32_t token = (uint32_t)(item / p.parts), part = (uint32_t)(item - (uint64_t)token * p.parts);
-        const int64_t row = p.n_kv ? row_of(p, token) : -1;
+    if (at.item < n_items) fetch(at.item);
+    for (int s = 0; s < ROPE_STAGES - 1; ++s) issue();
+    uint64_t now = ~0ull;        // the item whose angles are in the registers
+    uint32_t kind_now = 3;       // and the kind whose factors are
+    int64_t row = -1;
+    uint64_t f_ac[2], f_bs[2], f_bc[2], f_as[2];   // w_a cos, w_b sin, w_b cos, w_a sin
+    while (at.item < n_items) {
+        issue();
+        if (at.item != now) {
+            now = at.item;
+            kind_now = 3;
 #pragma unroll
-        for (int k = 0; k < PER; ++k)
-            if (lane + 32 * k < p.half) table[warp][lane + 32 * k] = turn_of(pos[k], turn[lane + 32 * k]);
-        if (item + hop < n_items) fetch(item + hop);
-        __syncwarp();
-        float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {};
-        if (turns) {
-            const float4 a = *reinterpret_cast<const float4*>(&table[warp][4 * i]), b = *reinterpret_cast<const float4*>(&table[warp][4 * i + 2]);
-            cs[0] = a.x, sn[0] = a.y, cs[1] = a.z, sn[1] = a.w, cs[2] = b.x, sn[2] = b.y, cs[3] = b.z, sn[3] = b.w;
+            for (int k = 0; k < PER; ++k)
+                if (lane + 32 * k < p.half) table[warp][lane + 32 * k] = turn_of(pos[k], turn[lane + 32 * k]);
+            row = p.n_kv ? row_of(p, at.token) : -1;
+            if (now + hop < n_items) fetch(now + hop);
+            __syncwarp();
         }
-        __syncwarp();
-        const uint32_t sk = (part + p.parts - uq % p.parts) % p.parts, sv = (sk + p.parts - uk % p.parts) % p.parts;   // first units of k and v
-        rope_heads<S, D, L, true, U>(static_cast<const S*>(p.q) + token * p.q_t, p.q_h, static_cast<D*>(p.q_out) + token * p.qo_t, p.qo_h, p.n_q, part * G, p.parts * G, g,
-                                     c0, c1, p.qw, p.eps, cs, sn);
-        if (row >= 0) {
-            rope_heads<S, D, L, true, U>(static_cast<const S*>(p.k) + token * p.k_t, p.k_h, static_cast<D*>(p.k_out) + row * p.ko_t, p.ko_h, p.n_kv, sk * G, p.parts * G, g,
-                                         c0, c1, p.kw, p.eps, cs, sn);
-            if (p.v) rope_heads<S, D, L, false, U>(static_cast<const S*>(p.v) + token * p.v_t, p.v_h, static_cast<D*>(p.v_out) + row * p.vo_t, p.vo_h, p.n_kv, sv * G, p.parts * G, g,
-                                                   c0, c1, nullptr, 0.f, cs, sn);
+        if (at.kind != kind_now && at.kind < 2) {
+            const float* w = at.kind == 0 ? p.qw : p.kw;
+            float4 wa = make_float4(1.f, 1.f, 1.f, 1.f), wb = wa, t0 = make_float4(1.f, 0.f, 1.f, 0.f), t1 = t0;
+            if (w) wa = *reinterpret_cast<const float4*>(w + c0), wb = *reinterpret_cast<const float4*>(w + c1);
+            if (turns) t0 = *reinterpret_cast<const float4*>(&table[warp][4 * i]), t1 = *reinterpret_cast<const float4*>(&table[warp][4 * i + 2]);
+            f_ac[0] = pack2(wa.x * t0.x, wa.y * t0.z), f_ac[1] = pack2(wa.z * t1.x, wa.w * t1.z);
+            f_bs[0] = pack2(-wb.x * t0.y, -wb.y * t0.w), f_bs[1] = pack2(-wb.z * t1.y, -wb.w * t1.w);
+            f_bc[0] = pack2(wb.x * t0.x, wb.y * t0.z), f_bc[1] = pack2(wb.z * t1.x, wb.w * t1.z);
+            f_as[0] = pack2(wa.x * t0.y, wa.y * t0.w), f_as[1] = pack2(wa.z * t1.y, wa.w * t1.w);
         }
+        kind_now = at.kind;
+        asm volatile("cp.async.wait_group %0;" ::"n"(ROPE_STAGES - 1) : "memory");
+        __syncwarp();
+        const S* st = reinterpret_cast<const S*>(ring + slot_at * ROPE_STAGE_BYTES) + g * DIM;
+        D* dst = at.kind == 0 ? static_cast<D*>(p.q_out) + at.token * p.qo_t : at.kind == 1 ? static_cast<D*>(p.k_out) + row * p.ko_t : static_cast<D*>(p.v_out) + row * p.vo_t;
+        const int64_t ds = at.kind == 0 ? p.qo_h : at.kind == 1 ? p.ko_h : p.vo_h;
+        const bool stored = at.kind == 0 || row >= 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t h = at.h + u * step + g;
+            if (at.h + u * step >= at.n) break;   // for the whole warp
+            Quad<S> ra = *reinterpret_cast<const Quad<S>*>(st + u * 256 + c0), rb = *reinterpret_cast<const Quad<S>*>(st + u * 256 + c1);
+            float a[4], b[4];
+            ra.get(a);
+            rb.get(b);
+            if (at.kind < 2) {
+                uint64_t a2[2] = {pack2(a[0], a[1]), pack2(a[2], a[3])}, b2[2] = {pack2(b[0], b[1]), pack2(b[2], b[3])};
+                float s0, s1;
+                unpack2(fma2(b2[1], b2[1], fma2(b2[0], b2[0], fma2(a2[1], a2[1], mul2(a2[0], a2[0])))), s0, s1);
+                float sum = s0 + s1;
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const float norm = rsqrtf(sum * (1.f / DIM) + p.eps);
+                const uint64_t n2 = pack2(norm, norm);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint64_t x = mul2(fma2(a2[e], f_ac[e], mul2(b2[e], f_bs[e])), n2), y = mul2(fma2(b2[e], f_bc[e], mul2(a2[e], f_as[e])), n2);
+                    unpack2(x, a[2 * e], a[2 * e + 1]);
+                    unpack2(y, b[2 * e], b[2 * e + 1]);
+                }
+            }
+            if (stored && h < at.n) {
+                *reinterpret_cast<Quad<D>*>(dst + h * ds + c0) = Quad<D>::of(a);
+                *reinterpret_cast<Quad<D>*>(dst + h * ds + c1) = Quad<D>::of(b);
+            }
+        }
+        at.h += U * step;
+        settle(at);
+        slot_at = slot_at + 1 == ROPE_STAGES ? 0 : slot_at + 1;
+        __syncwarp();   // the slot is free, the table read
     }
 }
 
 bool dtype_ok(int32_t d) { return d == DFL_F32 || d == DFL_F16 || d == DFL_BF16; }
 
-// every address the quad kernel forms is a multiple of four elements
+// every address the quad kernel forms is a multiple of 16 bytes where it reads, of four elements where it writes
 template <typename S, typename D>
 bool in_quads(const RopeParams& p) {
-    auto src = [&](const void* x, int64_t a, int64_t b) { return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(S)) == 0 && a % 4 == 0 && b % 4 == 0; };
+    constexpr int chunk = 16 / sizeof(S);
+    auto src = [&](const void* x, int64_t a, int64_t b) { return reinterpret_cast<uintptr_t>(x) % 16 == 0 && a % chunk == 0 && b % chunk == 0; };
     auto dst = [&](const void* x, int64_t a, int64_t b) { return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(D)) == 0 && a % 4 == 0 && b % 4 == 0; };
     const bool kv = p.n_kv > 0, v = p.n_heads > p.n_q + p.n_kv;
     return p.half % 4 == 0 && (p.dim == 64 || p.dim == 128 || p.dim == 256) && (!p.n_q || (src(p.q, p.q_t, p.q_h) && dst(p.q_out, p.qo_t, p.qo_h))) &&
            (!kv || (src(p.k, p.k_t, p.k_h) && dst(p.k_out, p.ko_t, p.ko_h))) && (!v || (src(p.v, p.v_t, p.v_h) && dst(p.v_out, p.vo_t, p.vo_h))) &&
            reinterpret_cast<uintptr_t>(p.qw) % 16 == 0 && reinterpret_cast<uintptr_t>(p.kw) % 16 == 0;
+}
+template <typename S, typename D, int L>
+cudaError_t launch_quads(const RopeParams& p, dim3 grid, cudaStream_t st) {
+    constexpr int smem = ROPE_WARPS * ROPE_STAGES * ROPE_STAGE_BYTES;
+    const cudaError_t e = cudaFuncSetAttribute(qk_norm_rope_kernel<S, D, L>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return e != cudaSuccess ? e : launch_k(qk_norm_rope_kernel<S, D, L>, grid, dim3(32 * ROPE_WARPS), smem, st, p);
 }
 template <typename S, typename D>
 cudaError_t launch_typed(RopeParams& p, cudaStream_t st) {
@@ -284,12 +344,12 @@ cudaError_t launch_typed(RopeParams& p, cudaStream_t st) {
     const uint64_t wanted = (uint64_t)sm_count() * 8, parts = (wanted + p.n_tokens - 1) / p.n_tokens;
     const uint32_t groups = quads ? 256 / p.dim : 1, most_parts = (p.n_q + groups - 1) / groups + (p.n_heads - p.n_q + groups - 1) / groups;
     p.parts = (uint32_t)(parts < most_parts ? parts : most_parts);
-    const uint64_t items = (uint64_t)p.n_tokens * p.parts, blocks = (items + ROPE_WARPS - 1) / ROPE_WARPS, most = (uint64_t)sm_count() * 4;
+    const uint64_t items = (uint64_t)p.n_tokens * p.parts, blocks = (items + ROPE_WARPS - 1) / ROPE_WARPS, most = (uint64_t)sm_count() * 3;
     const dim3 grid((unsigned)(blocks < most ? blocks : most)), block(32 * ROPE_WARPS);
     if (!quads) return launch_k(qk_norm_rope_any_kernel<S, D>, grid, block, 0, st, p);
-    if (p.dim == 64) return launch_k(qk_norm_rope_kernel<S, D, 8>, grid, block, 0, st, p);
-    if (p.dim == 128) return launch_k(qk_norm_rope_kernel<S, D, 16>, grid, block, 0, st, p);
-    return launch_k(qk_norm_rope_kernel<S, D, 32>, grid, block, 0, st, p);
+    if (p.dim == 64) return launch_quads<S, D, 8>(p, grid, st);
+    if (p.dim == 128) return launch_quads<S, D, 16>(p, grid, st);
+    return launch_quads<S, D, 32>(p, grid, st);
 }
 template <typename S>
 cudaError_t launch_src(RopeParams& p, int32_t dst, cudaStream_t st) {

@@ -22,8 +22,10 @@ namespace {
 
 constexpr int ST_THREADS = 512;
 constexpr int DRAW_CLUSTER = 8;
-constexpr int DRAW_THREADS = 512;
+constexpr int DRAW_THREADS = 256;
 constexpr int DRAW_WARPS = DRAW_THREADS / 32;
+constexpr int DRAW_SEGMENTS = 32;   // sums that a warp keeps of its run of the row, at most
+constexpr int STOP_BASE = DFL_MAX_VERIFY_DRAFTS + 1;
 
 struct Piece {   // of one row: maximum, sum of exp((x - max) / T), first index of the maximum
     float top, sum;
@@ -36,7 +38,8 @@ struct VerifyParams {
     const int32_t *drafts, *n_draft;
     const float *temperature, *u_accept, *u_sample;
     int32_t *n_accepted, *tokens;
-    Piece* pieces;   // [batch][rows][n_pieces]
+    Piece* pieces;       // [batch][rows][n_pieces]
+    uint32_t* tickets;   // [batch][rows] pieces done, then [batch] STOP_BASE - (the row that decides), 0 while it is not known; or null
     int64_t x_b, x_r, q_b, q_r;
     uint32_t batch, rows, n_pieces, piece;   // rows = drafts + 1
     uint32_t vocab;
@@ -75,6 +78,72 @@ template <> __device__ __forceinline__ void unpack_logits<__nv_bfloat16>(const u
     for (int e = 0; e < 4; ++e) x[2 * e] = in ? __uint_as_float(u[e] << 16) : -INFINITY, x[2 * e + 1] = in ? __uint_as_float(u[e] & 0xffff0000u) : -INFINITY;
 }
 
+// 2^(u / 32) for u <= 0 in 64 bits: u = k + r with |r| <= 1/2, 2^(k / 32) from a table of 32 entries (entry i in lane i's `tab`: the whole warp calls)
+// and an exponent, 2^(r / 32) by its series to r^5 (the next term is 2e-16).  Twelve double-precision instructions; zero below 2^-1000.
+__device__ __forceinline__ double pow2_32nd(double u, double tab) {
+    constexpr double L = 0.02166084939249829;   // ln 2 / 32
+    constexpr double MAGIC = 6755399441055744.0;   // 1.5 * 2^52: the sum's low word is the nearest integer
+    const double kd = u + MAGIC;
+    const int k = __double2loint(kd);
+    const double r = u - (kd - MAGIC);
+    double e = L * L * L * L * L / 120.0;
+    e = fma(e, r, L * L * L * L / 24.0);
+    e = fma(e, r, L * L * L / 6.0);
+    e = fma(e, r, L * L / 2.0);
+    e = fma(e, r, L);
+    e = fma(e, r, 1.0);
+    e *= __shfl_sync(0xffffffffu, tab, k & 31);
+    const double scaled = __hiloint2double(__double2hiint(e) + (int)((uint32_t)(k >> 5) << 20), __double2loint(e));
+    return u > -32000.0 ? scaled : 0.0;
+}
+__device__ __forceinline__ double pow2_table() { return exp2((double)(threadIdx.x & 31) * 0.03125); }
+
+struct Row {
+    float top;
+    int32_t first;
+    int stands;   // the draft behind this row's tokens: 1 stands, 0 does not (or there is none), -1 the row is no distribution
+};
+// by a whole warp: puts a row's pieces together and tests its draft.  Both kernels come to the same answer: no product in it is left to the
+// compiler to fuse or not.
+template <typename T>
+__device__ __forceinline__ Row row_of(const VerifyParams& p, uint32_t b, uint32_t r, int n, float t, double scale, double tab) {
+    const Piece* pc = p.pieces + ((uint64_t)b * p.rows + r) * p.n_pieces;
+    const uint32_t lane = threadIdx.x & 31;
+    // the draft's probabilities are on their way meanwhile
+    const int d = (int)r < n ? p.drafts[(uint64_t)b * (p.rows - 1) + r] : -1;
+    const bool tested = d >= 0 && (uint32_t)d < p.vocab;
+    const float x = tested ? logit<T>(p.logits, b * p.x_b + r * p.x_r + d) : 0.f, u = tested ? p.u_accept[(uint64_t)b * (p.rows - 1) + r] : 0.f;
+    const float q = tested && p.probs ? p.probs[b * p.q_b + r * p.q_r + d] : 1.f;
+    float top = -INFINITY;
+    for (uint32_t i = lane; i < p.n_pieces; i += 32) top = fmaxf(top, __ldcg(&pc[i].top));
+    top = warp_max(top);
+    double sum = 0.0;
+    int first = 0x7fffffff;
+    for (uint32_t i0 = 0; i0 < p.n_pieces; i0 += 32) {
+        Piece y{-INFINITY, 0.f, 0x7fffffff, 0};
+        if (i0 + lane < p.n_pieces) {
+            const int4 w = __ldcg(reinterpret_cast<const int4*>(&pc[i0 + lane]));
+            y = Piece{__int_as_float(w.x), __int_as_float(w.y), w.z, 0};
+        }
+        if (y.top == top) first = min(first, y.first);
+        const double f = pow2_32nd(__dmul_rn((double)y.top - (double)top, scale), tab);
+        sum = fma((double)y.sum, y.top == -INFINITY ? 1.0 : f, sum);   // a piece without a maximum adds its NaN, if it met one
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    first = __reduce_min_sync(0xffffffffu, first);
+    const double w = pow2_32nd(__dmul_rn((double)x - (double)top, scale), tab);
+    const double pd = t > 0.f ? w / sum : (d == first ? 1.0 : 0.0);
+    const bool ok = t >= 0.f && t < INFINITY && top > -INFINITY && top < INFINITY && sum == sum;
+    return Row{top, first, !ok ? -1 : tested && (double)u * (double)q < pd ? 1 : 0};
+}
+// what the exponent of a weight is multiplied by: 2^(u / 32) = e^((x - top) / T)
+__device__ __forceinline__ double scale_of(float t) { return t > 0.f ? 32.0 * 1.4426950408889634 / (double)t : 0.0; }
+__device__ __forceinline__ int drafts_of(const VerifyParams& p, uint32_t b) {
+    const int K = (int)p.rows - 1, n = p.n_draft ? p.n_draft[b] : K;
+    return n < 0 ? 0 : n > K ? K : n;
+}
+
 // 32 logits a thread in 16-byte pieces, all in flight at once; what lies beside the aligned range of the row (at most seven logits at either end)
 // belongs to the first and the last piece.  Grid pieces x batch x rows, rows outermost.
 template <typename T>
@@ -83,6 +152,10 @@ __global__ void __launch_bounds__(ST_THREADS) verify_pieces_kernel(const __grid_
     constexpr int VE = 16 / sizeof(T), NV = 32 / VE;   // logits of a vector, vectors of a thread
     __shared__ Piece warps[ST_THREADS / 32];
     const uint32_t piece = blockIdx.x % p.n_pieces, b = blockIdx.x / p.n_pieces % p.batch, r = blockIdx.x / p.n_pieces / p.batch;
+    // rows that the decision cannot read: behind the last draft that exists, and behind a row that is known to decide
+    const int n = drafts_of(p, b);
+    uint32_t* stop = p.tickets ? p.tickets + (uint64_t)p.batch * p.rows + b : nullptr;
+    if ((int)r > n || (stop && STOP_BASE - (int)r < (int)*reinterpret_cast<volatile uint32_t*>(stop))) return;
     const float t = temperature_of(p, b), c = t > 0.f ? fminf(1.44269504f / t, 3e38f) : 1.f;   // finite: 0 * c has to stay 0
     const T* row = static_cast<const T*>(p.logits) + b * p.x_b + r * p.x_r;
     const uint32_t head = min(p.vocab, (uint32_t)((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T)));   // logits ahead of the first vector
@@ -128,36 +201,20 @@ __global__ void __launch_bounds__(ST_THREADS) verify_pieces_kernel(const __grid_
         const float all = warp_max(a.top);
         a.sum = warp_sum(a.top == -INFINITY ? a.sum : a.sum * ex2((a.top - all) * c));
         a.first = __reduce_min_sync(0xffffffffu, a.top == all ? a.first : 0x7fffffff);
-        if (threadIdx.x == 0) p.pieces[((uint64_t)b * p.rows + r) * p.n_pieces + piece] = Piece{all, a.sum, a.first, 0};
+        uint32_t done = 0;
+        if (threadIdx.x == 0) {
+            p.pieces[((uint64_t)b * p.rows + r) * p.n_pieces + piece] = Piece{all, a.sum, a.first, 0};
+            if (stop) {
+                __threadfence();
+                done = atomicAdd(&p.tickets[(uint64_t)b * p.rows + r], 1u) + 1;
+            }
+        }
+        if (stop && __shfl_sync(0xffffffffu, done, 0) == p.n_pieces) {   // the row's last piece: spare the rows behind it if its draft falls
+            __threadfence();
+            const Row row = row_of<T>(p, b, r, n, t, scale_of(t), pow2_table());
+            if (threadIdx.x == 0 && row.stands != 1) atomicMax(stop, (uint32_t)(STOP_BASE - (int)r));
+        }
     }
-}
-
-struct Row {
-    double sum;     // f32-accurate
-    float top;
-    int32_t first;
-    bool ok;        // a distribution
-};
-// by a whole warp
-__device__ __forceinline__ Row row_of(const VerifyParams& p, uint32_t b, uint32_t r, double inv_t, float t) {
-    const Piece* pc = p.pieces + ((uint64_t)b * p.rows + r) * p.n_pieces;
-    const uint32_t lane = threadIdx.x & 31;
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < p.n_pieces; i += 32) top = fmaxf(top, __ldcg(&pc[i].top));
-    top = warp_max(top);
-    double sum = 0.0;
-    int first = 0x7fffffff;
-    for (uint32_t i = lane; i < p.n_pieces; i += 32) {
-        const float pt = __ldcg(&pc[i].top), ps = __ldcg(&pc[i].sum);
-        if (pt == top) first = min(first, __ldcg(&pc[i].first));
-        sum += pt == -INFINITY ? (double)ps : (double)ps * exp(((double)pt - (double)top) * inv_t);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-    }
-    return Row{sum, top, first, t >= 0.f && t < INFINITY && top > -INFINITY && sum == sum};
 }
 
 // Adds up one value a CTA of the cluster, in rank order: what the ranks before this one hold, and the whole.
@@ -174,143 +231,191 @@ __device__ __forceinline__ void cluster_sum(cg::cluster_group& cluster, double* 
     *whole = w;
 }
 
+// four logits from `at` on, of those below `end`; the others -inf
+template <typename T>
+__device__ __forceinline__ void load4(const T* row, uint32_t at, uint32_t end, bool vec, float (&x)[4]) {
+    if (vec && at + 4 <= end) {
+        if (sizeof(T) == 4) {
+            const float4 w = __ldg(reinterpret_cast<const float4*>(row + at));
+            x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+        } else {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(row + at));
+            float y[8];
+            unpack_logits<T>(make_uint4(w.x, w.y, 0, 0), true, y);
+            x[0] = y[0], x[1] = y[1], x[2] = y[2], x[3] = y[3];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = at + e < end ? logit<T>(row, at + e) : -INFINITY;
+    }
+}
+__device__ __forceinline__ double warp_sum64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
 template <typename T>
 __global__ void __cluster_dims__(DRAW_CLUSTER, 1, 1) __launch_bounds__(DRAW_THREADS) verify_draw_kernel(const __grid_constant__ VerifyParams p) {
     pdl_prologue();
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ double slots[3][DRAW_CLUSTER];
     __shared__ double warp_sums[DRAW_WARPS];
-    __shared__ int stands[DFL_MAX_VERIFY_DRAFTS + 1];
-    __shared__ int found, taken_s;
+    __shared__ double segments[DRAW_WARPS][DRAW_SEGMENTS];
+    __shared__ Row rows[DFL_MAX_VERIFY_DRAFTS + 1];
+    __shared__ int found;
     const uint32_t b = blockIdx.x / DRAW_CLUSTER, rank = cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int K = (int)p.rows - 1;
-    int n = p.n_draft ? p.n_draft[b] : K;
-    n = n < 0 ? 0 : n > K ? K : n;
+    const int K = (int)p.rows - 1, n = drafts_of(p, b);
     const float t = temperature_of(p, b);
-    const double inv_t = t > 0.f ? 1.0 / (double)t : 0.0;
+    const double scale = scale_of(t), tab = pow2_table();
     if (threadIdx.x == 0) found = -1;
-    cluster.sync();   // every CTA of the cluster has started
-    // a warp a draft: does it stand (1), not (0), or is its row no distribution (-1)
-    for (int r = (int)warp; r <= n; r += DRAW_WARPS) {
-        const Row row = row_of(p, b, r, inv_t, t);
-        if (lane == 0) {
-            int s = row.ok ? 0 : -1;
-            if (row.ok && r < n) {
-                const int d = p.drafts[(int64_t)b * K + r];
-                if (d >= 0 && (uint32_t)d < p.vocab) {
-                    const double x = (double)logit<T>(p.logits, b * p.x_b + r * p.x_r + d);
-                    const double pd = t > 0.f ? exp((x - (double)row.top) * inv_t) / row.sum : (d == row.first ? 1.0 : 0.0);
-                    const double qd = p.probs ? (double)p.probs[b * p.q_b + r * p.q_r + d] : 1.0;
-                    s = (double)p.u_accept[(int64_t)b * K + r] * qd < pd ? 1 : 0;
-                }
-            }
-            stands[r] = s;
+    cluster.barrier_arrive();
+    // a warp a row, four rows a warp at a time until one decides
+    int taken = 0;
+    for (int r0 = 0; r0 <= n; r0 += DRAW_WARPS) {
+        if (r0 + (int)warp <= n) {
+            const Row row = row_of<T>(p, b, r0 + warp, n, t, scale, tab);
+            if (lane == 0) rows[r0 + warp] = row;
         }
+        __syncthreads();
+        const int end = min(n, r0 + DRAW_WARPS - 1);
+        while (taken < end && rows[taken].stands == 1) ++taken;
+        if (rows[taken].stands != 1 || taken == n) break;
+        ++taken;
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int r = 0;
-        while (r < n && stands[r] == 1) ++r;
-        taken_s = stands[r] < 0 ? -1 - r : r;
-    }
-    __syncthreads();
-    const int taken = taken_s;
-    int token = -1;
-    if (taken >= 0) {
-        const Row row = row_of(p, b, taken, inv_t, t);
-        const bool refused = taken < n;
-        const int d = refused ? p.drafts[(int64_t)b * K + taken] : -1;
-        const int64_t x_row = b * p.x_b + taken * p.x_r, q_row = b * p.q_b + taken * p.q_r;
-        if (t == 0.f) {
-            token = row.first;
-        } else {
-            // the row in vocabulary order over the cluster's warps, a run of tokens each
-            const uint32_t n_warps = DRAW_CLUSTER * DRAW_WARPS, per = ((p.vocab + n_warps - 1) / n_warps + 31) / 32 * 32;
-            const uint64_t lo64 = (uint64_t)(rank * DRAW_WARPS + warp) * per;
-            const uint32_t lo = (uint32_t)(lo64 < p.vocab ? lo64 : p.vocab), hi = (uint32_t)(lo64 + per < p.vocab ? lo64 + per : p.vocab);
-            const double top = (double)row.top;
-            double z = 1.0;
-            int mode = refused ? (p.probs ? 2 : 1) : 0;   // 0 w, 1 w without the draft, 2 max(p - q, 0)
-            auto weight = [&](uint32_t i) -> double {
-                const double w = exp(((double)logit<T>(p.logits, x_row + i) - top) * inv_t);
-                if (mode == 0) return w;
-                if (mode == 1) return (int)i == d ? 0.0 : w;
-                return fmax(w / z - (double)p.probs[q_row + i], 0.0);
-            };
-            double before = 0.0, whole = 0.0, in_cta = 0.0, mine = 0.0;
-            auto sum_up = [&](int slot) {
-                mine = 0.0;
-                for (uint32_t i = lo + lane; i < hi; i += 32) mine += weight(i);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-                __syncthreads();
-                if (lane == 0) warp_sums[warp] = mine;
-                __syncthreads();
-                double cta = 0.0;
-                in_cta = 0.0;
-                for (int w = 0; w < DRAW_WARPS; ++w) {
-                    if (w == (int)warp) in_cta = cta;
-                    cta += warp_sums[w];
-                }
-                cluster_sum(cluster, slots[slot], cta, &before, &whole);
-            };
+    const Row row = rows[taken];
+    const bool refused = taken < n, ok = row.stands >= 0;
+    cluster.barrier_wait();   // every CTA of the cluster has started
+    if (ok && t > 0.f) {
+        const int d = refused ? p.drafts[(uint64_t)b * K + taken] : -1;
+        const T* x_row = static_cast<const T*>(p.logits) + b * p.x_b + taken * p.x_r;
+        const float* q_row = p.probs + b * p.q_b + taken * p.q_r;
+        const bool x_vec = reinterpret_cast<uintptr_t>(x_row) % (4 * sizeof(T)) == 0, q_vec = reinterpret_cast<uintptr_t>(q_row) % 16 == 0;
+        // the row in vocabulary order over the cluster's warps: a run of `count` segments of `seg` tokens each
+        constexpr uint32_t N_WARPS = DRAW_CLUSTER * DRAW_WARPS;
+        const uint32_t blocks = (p.vocab + 127) / 128, per = (blocks + N_WARPS - 1) / N_WARPS, seg_blocks = (per + DRAW_SEGMENTS - 1) / DRAW_SEGMENTS;
+        const uint32_t b0 = min(blocks, (rank * DRAW_WARPS + warp) * per), b1 = min(blocks, b0 + per);   // blocks of 128 tokens, four a lane
+        const double top = (double)row.top;
+        double z = 1.0;
+        int mode = refused ? (p.probs ? 2 : 1) : 0;   // 0 w, 1 w without the draft, 2 max(p - q, 0)
+        auto weights = [&](uint32_t block, double (&w)[4]) {
+            const uint32_t at = block * 128 + lane * 4;
+            float x[4], q[4];
+            load4<T>(x_row, at, p.vocab, x_vec, x);
             if (mode == 2) {
-                mode = 0;
-                sum_up(0);
-                z = whole;
-                mode = 2;
+                if (at < p.vocab) load4<float>(q_row, at, p.vocab, q_vec, q);
+                else q[0] = q[1] = q[2] = q[3] = 0.f;
             }
-            sum_up(1);
-            if (!(whole > 0.0)) {   // nothing is left of p beside q
-                mode = 0;
-                sum_up(2);
-            }
-            // inside [0, whole) even if u is not inside [0, 1); the runs share that range out without gap or overlap, their ends being the
-            // same sums as the next ones' starts
-            double target = fmax((double)p.u_sample[b] * whole, 0.0);
-            if (!(target < whole)) target = __longlong_as_double(__double_as_longlong(whole) - 1);
-            const double start = before + in_cta, end = before + (in_cta + mine);
-            if (start <= target && end > target) {
-                double run = start;
-                int hit = -1, last = -1;
-                for (uint32_t i0 = lo; i0 < hi && hit < 0; i0 += 32) {
-                    const uint32_t i = i0 + lane;
-                    const double w = i < hi ? weight(i) : 0.0;
-                    double upto = w;
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const double y = __shfl_up_sync(0xffffffffu, upto, o);
-                        if ((int)lane >= o) upto += y;
-                    }
-                    const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && run + upto > target), some = __ballot_sync(0xffffffffu, w > 0.0);
-                    if (some) last = (int)i0 + 31 - __clz(some);
-                    if (over) hit = (int)i0 + __ffs(over) - 1;
-                    run += __shfl_sync(0xffffffffu, upto, 31);
-                }
-                if (lane == 0) found = hit >= 0 ? hit : last;
+            for (int e = 0; e < 4; ++e) {
+                w[e] = pow2_32nd(__dmul_rn((double)x[e] - top, scale), tab);
+                if (mode == 1 && (int)(at + e) == d) w[e] = 0.0;
+                if (mode == 2) w[e] = at + e < p.vocab ? fmax(fma(w[e], z, -(double)q[e]), 0.0) : 0.0;
             }
+        };
+        double before = 0.0, whole = 0.0, in_cta = 0.0, mine = 0.0;
+        auto sum_up = [&](int slot) {
+            mine = 0.0;
+            for (uint32_t s = 0, bl = b0; bl < b1; ++s) {
+                double sum = 0.0;
+                for (uint32_t k = 0; k < seg_blocks && bl < b1; ++k, ++bl) {
+                    double w[4];
+                    weights(bl, w);
+                    sum += (w[0] + w[1]) + (w[2] + w[3]);
+                }
+                sum = warp_sum64(sum);
+                if (lane == 0) segments[warp][s] = sum;
+                mine += sum;
+            }
+            __syncthreads();   // warp_sums of an earlier call are read
+            if (lane == 0) warp_sums[warp] = mine;
+            __syncthreads();
+            double cta = 0.0;
+            in_cta = 0.0;
+            for (int w = 0; w < DRAW_WARPS; ++w) {
+                if (w == (int)warp) in_cta = cta;
+                cta += warp_sums[w];
+            }
+            cluster_sum(cluster, slots[slot], cta, &before, &whole);
+        };
+        if (mode == 2) {
+            mode = 0;
+            sum_up(0);
+            z = 1.0 / whole;
+            mode = 2;
+        }
+        sum_up(1);
+        if (!(whole > 0.0)) {   // nothing is left of p beside q
+            mode = 0;
+            sum_up(2);
+        }
+        // inside [0, whole) even if u is not inside [0, 1); the runs share that range out without gap or overlap, their ends being the
+        // same sums as the next ones' starts
+        double target = fmax((double)p.u_sample[b] * whole, 0.0);
+        if (!(target < whole)) target = __longlong_as_double(__double_as_longlong(whole) - 1);
+        const double start = before + in_cta, end = before + (in_cta + mine);
+        if (start <= target && end > target) {
+            double upto = start;
+            uint32_t s = 0, bl = b0;
+            while (bl + seg_blocks < b1 && !(upto + segments[warp][s] > target)) upto += segments[warp][s++], bl += seg_blocks;
+            int hit = -1, last = -1;
+            for (; bl < b1 && hit < 0; ++bl) {
+                double w[4];
+                weights(bl, w);
+                double own = (w[0] + w[1]) + (w[2] + w[3]), sum = own;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double y = __shfl_up_sync(0xffffffffu, sum, o);
+                    if ((int)lane >= o) sum += y;
+                }
+                double run = upto + (sum - own);
+                int at = -1, some = -1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    run += w[e];
+                    if (w[e] > 0.0) {
+                        some = (int)(bl * 128 + lane * 4 + e);
+                        if (at < 0 && run > target) at = some;
+                    }
+                }
+                const unsigned over = __ballot_sync(0xffffffffu, at >= 0);
+                last = max(last, __reduce_max_sync(0xffffffffu, some));
+                if (over) hit = __shfl_sync(0xffffffffu, at, __ffs(over) - 1);
+                upto += __shfl_sync(0xffffffffu, sum, 31);
+            }
+            if (lane == 0) found = hit >= 0 ? hit : last;   // none by a rounding: the run's last token with any mass
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        if (found >= 0) p.tokens[(uint64_t)b * p.rows + taken] = found;   // one run of the cluster's holds the target
-        if (rank == 0) {
-            p.n_accepted[b] = taken;
-            if (token >= 0) p.tokens[(uint64_t)b * p.rows + taken] = token;
+    if (threadIdx.x == 0 && found >= 0) p.tokens[(uint64_t)b * p.rows + taken] = found;   // one run of the cluster's holds the target
+    if (rank == 0) {
+        if (threadIdx.x == 0) {
+            p.n_accepted[b] = ok ? taken : -1 - taken;
+            if (!ok || t == 0.f) p.tokens[(uint64_t)b * p.rows + taken] = ok ? row.first : -1;
         }
-    }
-    if (rank == 0)
         for (int i = threadIdx.x; i <= K; i += DRAW_THREADS)
-            if (i != taken) p.tokens[(uint64_t)b * p.rows + i] = i < taken ? p.drafts[(int64_t)b * K + i] : -1;
+            if (i != taken) p.tokens[(uint64_t)b * p.rows + i] = ok && i < taken ? p.drafts[(uint64_t)b * K + i] : -1;
+    }
     cluster.sync();   // nobody leaves while its sums are read
 }
 
 struct Split {
     uint32_t piece, n_pieces;
+    bool tickets;
+    uint64_t piece_bytes, ticket_bytes;
 };
 Split split_of(const dfl_verify_drafts_args* a) {
     constexpr uint32_t piece = ST_THREADS * 32;
-    return Split{piece, (uint32_t)((a->vocab + piece - 1) / piece)};
+    Split s;
+    s.piece = piece;
+    s.n_pieces = (uint32_t)((a->vocab + piece - 1) / piece);
+    const uint64_t rows = (uint64_t)a->batch * (a->n_drafts + 1);
+    // Rows behind a draft that falls are spared where they start late enough to know: with more pieces than run at once.  The counters have to be
+    // cleared, a launch of 2 us.
+    s.tickets = a->n_drafts > 0 && rows * s.n_pieces > 2000;
+    s.piece_bytes = (rows * s.n_pieces * sizeof(Piece) + 255) / 256 * 256;
+    s.ticket_bytes = s.tickets ? (rows + a->batch) * sizeof(uint32_t) : 0;
+    return s;
 }
 
 dfl_status check(const dfl_verify_drafts_args* a, bool pointers) {
@@ -345,7 +450,8 @@ extern "C" dfl_status dfl_verify_drafts_workspace(int32_t device, const dfl_veri
     if (!bytes_out) return fail(DFL_ERR_BAD_ARG, "verify_drafts_workspace: null argument");
     (void)device;   // the same on every one
     DFL_CHECK(check(a, false));
-    *bytes_out = (uint64_t)a->batch * (a->n_drafts + 1) * split_of(a).n_pieces * sizeof(Piece);
+    const Split s = split_of(a);
+    *bytes_out = s.piece_bytes + s.ticket_bytes;
     return DFL_OK;
 }
 
@@ -368,6 +474,10 @@ extern "C" dfl_status dfl_verify_drafts(int32_t device, const dfl_verify_drafts_
     const Split s = split_of(a);
     p.batch = a->batch, p.rows = a->n_drafts + 1, p.vocab = (uint32_t)a->vocab, p.piece = s.piece, p.n_pieces = s.n_pieces;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (s.tickets) {
+        p.tickets = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a->workspace) + s.piece_bytes);
+        DFL_CUDA(cudaMemsetAsync(p.tickets, 0, s.ticket_bytes, st));
+    }
     DFL_CUDA(a->dtype == DFL_F32 ? launch<float>(p, st) : a->dtype == DFL_F16 ? launch<__half>(p, st) : launch<__nv_bfloat16>(p, st));
     count_launch(2);
     return DFL_OK;
