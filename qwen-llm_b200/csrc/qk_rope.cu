@@ -10,7 +10,6 @@
 // point, F = 2^64 theta^(-j/h) / 2 pi, made on the host in extended precision; pos * F modulo 2^64 is the angle modulo one
 // turn (the wrap of the integer product drops the whole turns), off by at most 2^-27 turns at position 2^31.  Its upper 32 bits become f32.
 #include <cmath>
-#include <type_traits>
 
 #include "common.cuh"
 

@@ -4,13 +4,14 @@
 //   w_t = exp((x_t - max x) / T), Z = sum w, p = w / Z;   draft d stands while u q(d) < p(d)
 //   drawn token = the lowest t with  sum_{s <= t} r_s > u sum r,   r = w without the refused draft | max(p - q, 0) | w
 //
-// Two launches.  The first reads every row once and leaves (max, sum, index of the first maximum) of each piece of it: bound by the bytes of the
-// logits, f32 sums.  In the second a cluster of eight CTAs a request puts the pieces together, decides, and goes over the one row that the
-// draw needs again, in 64 bits: a border between two tokens is met by a sum that is 1e-9 off once in a few thousand draws (vocabulary
-// 151 936), by one that is 1e-14 off practically never, and the token is to be the definition's.
+// Two launches.  The first reads every row that it cannot rule out once and leaves (max, sum, index of the first maximum) of each piece of it: bound
+// by the bytes of the logits, f32 sums.  In the second a cluster of one to sixteen CTAs a request puts the pieces together, decides, and goes over
+// the one row that the draw needs again, in 64 bits: a border between two tokens is met by a sum that is 1e-9 off once in a few thousand draws
+// (vocabulary 151 936), by one that is 1e-13 off practically never, and the token is to be the definition's.
 #include <cooperative_groups.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -20,9 +21,11 @@ namespace dfl {
 dfl_status use_device(int device);
 namespace {
 
-constexpr int ST_THREADS = 512;
-constexpr int DRAW_CLUSTER = 8;
-constexpr int DRAW_THREADS = 256;
+constexpr int ST_BYTES = 32768, ST_SLOTS = 6;   // the first kernel: bytes of a piece, pieces of the ring
+constexpr int ST_GROUPS = 2, ST_WARPS = 8, ST_FINISH = 6, ST_THREADS = 32 * (1 + ST_GROUPS * ST_WARPS + ST_FINISH);   // groups of warps that take the pieces in turn
+static_assert(ST_SLOTS % ST_FINISH == 0 && ST_SLOTS % ST_GROUPS == 0, "a slot always has the same group and the same finishing warp: who waits by parity has to see every phase");
+constexpr int DRAW_CLUSTER = 16;     // CTAs of a request, at most
+constexpr int DRAW_THREADS = 512;
 constexpr int DRAW_WARPS = DRAW_THREADS / 32;
 constexpr int DRAW_SEGMENTS = 32;   // sums that a warp keeps of its run of the row, at most
 constexpr int STOP_BASE = DFL_MAX_VERIFY_DRAFTS + 1;
@@ -41,7 +44,7 @@ struct VerifyParams {
     Piece* pieces;       // [batch][rows][n_pieces]
     uint32_t* tickets;   // [batch][rows] pieces done, then [batch] STOP_BASE - (the row that decides), 0 while it is not known; or null
     int64_t x_b, x_r, q_b, q_r;
-    uint32_t batch, rows, n_pieces, piece;   // rows = drafts + 1
+    uint32_t batch, rows, n_pieces;   // rows = drafts + 1
     uint32_t vocab;
 };
 
@@ -78,25 +81,58 @@ template <> __device__ __forceinline__ void unpack_logits<__nv_bfloat16>(const u
     for (int e = 0; e < 4; ++e) x[2 * e] = in ? __uint_as_float(u[e] << 16) : -INFINITY, x[2 * e + 1] = in ? __uint_as_float(u[e] & 0xffff0000u) : -INFINITY;
 }
 
-// 2^(u / 32) for u <= 0 in 64 bits: u = k + r with |r| <= 1/2, 2^(k / 32) from a table of 32 entries (entry i in lane i's `tab`: the whole warp calls)
-// and an exponent, 2^(r / 32) by its series to r^5 (the next term is 2e-16).  Twelve double-precision instructions; zero below 2^-1000.
-__device__ __forceinline__ double pow2_32nd(double u, double tab) {
-    constexpr double L = 0.02166084939249829;   // ln 2 / 32
-    constexpr double MAGIC = 6755399441055744.0;   // 1.5 * 2^52: the sum's low word is the nearest integer
-    const double kd = u + MAGIC;
-    const int k = __double2loint(kd);
-    const double r = u - (kd - MAGIC);
-    double e = L * L * L * L * L / 120.0;
-    e = fma(e, r, L * L * L * L / 24.0);
-    e = fma(e, r, L * L * L / 6.0);
-    e = fma(e, r, L * L / 2.0);
-    e = fma(e, r, L);
-    e = fma(e, r, 1.0);
-    e *= __shfl_sync(0xffffffffu, tab, k & 31);
-    const double scaled = __hiloint2double(__double2hiint(e) + (int)((uint32_t)(k >> 5) << 20), __double2loint(e));
-    return u > -32000.0 ? scaled : 0.0;
-}
+// A row's weights e^((x - top) / T) = 2^(u / 32), u = (x - top) scale <= 0, in 64 bits.  u = k + r with k an integer: 2^(k / 32) comes from a table of 32
+// entries (entry i in lane i's `tab`: the whole warp calls) and an exponent, 2^(r / 32) from its series to r^4, the r^5 term spread over the
+// lower ones as its Chebyshev polynomial says (within 1e-13 for |r| <= 1/2).  k is found in f32, where a place more or less does no harm.
+// Ten double-precision instructions a weight; they bound the draw (B200: 62 a clock and SM), so N weights go side by side: one chain takes
+// some 400 clocks.
+struct Expo {
+    double top, scale, tab;
+    float top_f, scale_f;
+};
 __device__ __forceinline__ double pow2_table() { return exp2((double)(threadIdx.x & 31) * 0.03125); }
+// 32 / (T ln 2); T = 0 is never asked for
+__device__ __forceinline__ double scale_of(float t) { return t > 0.f ? 32.0 * 1.4426950408889634 / (double)t : 0.0; }
+__device__ __forceinline__ Expo expo(float top, double scale, double tab) { return Expo{(double)top, scale, tab, top, fminf((float)scale, 3e38f)}; }
+template <int N>
+__device__ __forceinline__ void weights_of(const Expo& f, const float* x, double (&w)[N]) {
+    constexpr double L = 0.02166084939249829;   // ln 2 / 32
+    constexpr double C5 = L * L * L * L * L / 120.0, A2 = 0.25;   // |r| <= A
+    constexpr double C4 = L * L * L * L / 24.0, C3 = L * L * L / 6.0 + C5 * 1.25 * A2, C2 = L * L / 2.0, C1 = L - C5 * 0.3125 * A2 * A2;
+    constexpr int ZERO = 0x4b400000;            // the bits of 1.5 * 2^23; adding that leaves the nearest integer in a number's low bits
+    double e[N];
+    int k[N];                                   // ZERO + k
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        k[i] = __float_as_int(fmaxf(fmaf(x[i] - f.top_f, f.scale_f, 12582912.f), 12582912.f - 40000.f));
+        w[i] = (double)x[i] - f.top;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        w[i] = __dmul_rn(w[i], f.scale);
+        e[i] = __hiloint2double(0x43300000, k[i]) - (4503599627370496.0 + ZERO);   // 2^52 + bits less 2^52 + ZERO: k
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] -= e[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = fma(C4, w[i], C3);
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = fma(e[i], w[i], C2);
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = fma(e[i], w[i], C1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = fma(e[i], w[i], 1.0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] *= __shfl_sync(0xffffffffu, f.tab, k[i] & 31);
+#pragma unroll
+    for (int i = 0; i < N; ++i)   // (k >> 5) << 20 on the exponent: ZERO's own bits leave the word; zero below 2^-1000
+        w[i] = k[i] > ZERO - 32000 ? __hiloint2double(__double2hiint(e[i]) + ((k[i] & ~31) << 15), __double2loint(e[i])) : 0.0;
+}
+__device__ __forceinline__ double weight_of(const Expo& f, float x) {
+    double w[1];
+    weights_of<1>(f, &x, w);
+    return w[0];
+}
 
 struct Row {
     float top;
@@ -117,6 +153,7 @@ __device__ __forceinline__ Row row_of(const VerifyParams& p, uint32_t b, uint32_
     float top = -INFINITY;
     for (uint32_t i = lane; i < p.n_pieces; i += 32) top = fmaxf(top, __ldcg(&pc[i].top));
     top = warp_max(top);
+    const Expo ex = expo(top, scale, tab);
     double sum = 0.0;
     int first = 0x7fffffff;
     for (uint32_t i0 = 0; i0 < p.n_pieces; i0 += 32) {
@@ -126,114 +163,221 @@ __device__ __forceinline__ Row row_of(const VerifyParams& p, uint32_t b, uint32_
             y = Piece{__int_as_float(w.x), __int_as_float(w.y), w.z, 0};
         }
         if (y.top == top) first = min(first, y.first);
-        const double f = pow2_32nd(__dmul_rn((double)y.top - (double)top, scale), tab);
+        const double f = weight_of(ex, y.top);
         sum = fma((double)y.sum, y.top == -INFINITY ? 1.0 : f, sum);   // a piece without a maximum adds its NaN, if it met one
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     first = __reduce_min_sync(0xffffffffu, first);
-    const double w = pow2_32nd(__dmul_rn((double)x - (double)top, scale), tab);
+    const double w = weight_of(ex, x);
     const double pd = t > 0.f ? w / sum : (d == first ? 1.0 : 0.0);
     const bool ok = t >= 0.f && t < INFINITY && top > -INFINITY && top < INFINITY && sum == sum;
     return Row{top, first, !ok ? -1 : tested && (double)u * (double)q < pd ? 1 : 0};
 }
-// what the exponent of a weight is multiplied by: 2^(u / 32) = e^((x - top) / T)
-__device__ __forceinline__ double scale_of(float t) { return t > 0.f ? 32.0 * 1.4426950408889634 / (double)t : 0.0; }
 __device__ __forceinline__ int drafts_of(const VerifyParams& p, uint32_t b) {
     const int K = (int)p.rows - 1, n = p.n_draft ? p.n_draft[b] : K;
     return n < 0 ? 0 : n > K ? K : n;
 }
 
-// 32 logits a thread in 16-byte pieces, all in flight at once; what lies beside the aligned range of the row (at most seven logits at either end)
-// belongs to the first and the last piece.  Grid pieces x batch x rows, rows outermost.
+// Pieces of 32 KB go by bulk copy into a ring of six, one persistent CTA an SM: a producer warp, two groups of eight warps that find the pieces' maxima
+// and sums in turn, six warps that put a group's results together (counting a piece takes one of them as long as six pieces take to arrive: with two of
+// them 131 us for 350 MB, four 81, six 71).  So 192 KB an SM are under way whatever the warps do.  What lies beside the aligned range of a row (at most
+// seven logits at either end) belongs to the first and the last piece.  Pieces x batch x rows, the first rows of all requests first: when a row's last
+// piece is done its draft is tested, and where it falls the rows behind are spared.
+struct ItemInfo {   // what the producer found out about a piece
+    uint32_t b, r, piece, head, v0, n, tail;   // n vectors from v0 on, `head` logits ahead of the row's first vector, the last ones from `tail` on
+    float c;                                   // log2 e / T, finite: 0 * c has to stay 0
+    int32_t greedy, end;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(ST_THREADS) verify_pieces_kernel(const __grid_constant__ VerifyParams p) {
-    pdl_prologue();
-    constexpr int VE = 16 / sizeof(T), NV = 32 / VE;   // logits of a vector, vectors of a thread
-    __shared__ Piece warps[ST_THREADS / 32];
-    const uint32_t piece = blockIdx.x % p.n_pieces, b = blockIdx.x / p.n_pieces % p.batch, r = blockIdx.x / p.n_pieces / p.batch;
-    // rows that the decision cannot read: behind the last draft that exists, and behind a row that is known to decide
-    const int n = drafts_of(p, b);
-    uint32_t* stop = p.tickets ? p.tickets + (uint64_t)p.batch * p.rows + b : nullptr;
-    if ((int)r > n || (stop && STOP_BASE - (int)r < (int)*reinterpret_cast<volatile uint32_t*>(stop))) return;
-    const float t = temperature_of(p, b), c = t > 0.f ? fminf(1.44269504f / t, 3e38f) : 1.f;   // finite: 0 * c has to stay 0
-    const T* row = static_cast<const T*>(p.logits) + b * p.x_b + r * p.x_r;
-    const uint32_t head = min(p.vocab, (uint32_t)((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T)));   // logits ahead of the first vector
-    const uint32_t n_vec = (p.vocab - head) / VE, v0 = piece * (p.piece / VE), v1 = piece + 1 == p.n_pieces ? n_vec : min(n_vec, v0 + p.piece / VE);
-    float x[32], extra = -INFINITY;
-    uint32_t extra_at = 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const uint32_t v = v0 + threadIdx.x + j * ST_THREADS;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        const bool in = v < v1;
-        if (in) w = __ldcs(reinterpret_cast<const uint4*>(row + head) + v);
-        unpack_logits<T>(w, in, &x[j * VE]);
-    }
-    if (piece == 0 && threadIdx.x < head) extra_at = threadIdx.x, extra = logit<T>(row, extra_at);
-    if (piece + 1 == p.n_pieces && threadIdx.x >= 32 && threadIdx.x - 32 < p.vocab - head - n_vec * VE) {
-        extra_at = head + n_vec * VE + threadIdx.x - 32;
-        extra = logit<T>(row, extra_at);
-    }
-    float top = extra;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) top = fmaxf(top, x[j]);
-    const float mine = top;
-    top = warp_max(top);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = ex2((extra - base) * c);
-#pragma unroll
-    for (int j = 0; j < 32; ++j) sum += ex2((x[j] - base) * c);   // NaN for a NaN and for +inf
-    Piece a{top, warp_sum(sum), 0x7fffffff, 0};
-    if (t == 0.f) {   // greedy: the first index of the maximum
-        if (mine == top) {
-            if (extra == top) a.first = (int32_t)extra_at;
-#pragma unroll
-            for (int j = 31; j >= 0; --j)
-                if (x[j] == top) a.first = min(a.first, (int32_t)(head + (v0 + threadIdx.x + (j / VE) * ST_THREADS) * VE + j % VE));
+__global__ void __launch_bounds__(ST_THREADS, 1) verify_pieces_kernel(const __grid_constant__ VerifyParams p) {
+    constexpr uint32_t VE = 16 / sizeof(T), PIECE = ST_BYTES / sizeof(T);   // logits of 16 bytes, of a piece
+    extern __shared__ __align__(128) uint8_t ring[];   // [ST_SLOTS][ST_BYTES]
+    __shared__ uint64_t full[ST_SLOTS], parts_full[ST_SLOTS], empty[ST_SLOTS];
+    __shared__ Piece parts[ST_SLOTS][ST_WARPS];
+    __shared__ ItemInfo info[ST_SLOTS];
+    __shared__ int err;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST_SLOTS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&parts_full[i], ST_WARPS);
+            mbar_init(&empty[i], 1);
         }
-        a.first = __reduce_min_sync(0xffffffffu, a.first);
+        err = 0;
+        mbar_fence_init();
     }
-    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = a;
+    pdl_launch_dependents();
+    const double tab = pow2_table();
     __syncthreads();
-    if (threadIdx.x < 32) {
-        a = threadIdx.x < ST_THREADS / 32 ? warps[threadIdx.x] : Piece{-INFINITY, 0.f, 0x7fffffff, 0};
-        const float all = warp_max(a.top);
-        a.sum = warp_sum(a.top == -INFINITY ? a.sum : a.sum * ex2((a.top - all) * c));
-        a.first = __reduce_min_sync(0xffffffffu, a.top == all ? a.first : 0x7fffffff);
-        uint32_t done = 0;
-        if (threadIdx.x == 0) {
-            p.pieces[((uint64_t)b * p.rows + r) * p.n_pieces + piece] = Piece{all, a.sum, a.first, 0};
-            if (stop) {
-                __threadfence();
-                done = atomicAdd(&p.tickets[(uint64_t)b * p.rows + r], 1u) + 1;
+    pdl_wait();
+    const uint32_t items = p.n_pieces * p.batch * p.rows;
+    uint32_t* stops = p.tickets ? p.tickets + (uint64_t)p.batch * p.rows : nullptr;
+    auto row_ptr = [&](uint32_t b, uint32_t r) { return static_cast<const T*>(p.logits) + b * p.x_b + r * p.x_r; };
+    if (warp == 0) {
+        // ================= producer =================
+        // 32 of the CTA's items are looked at side by side, one a lane.  Not needed are rows behind the last draft that exists and rows behind one that is
+        // known to decide; that is looked up anew for every piece that is sent, while a slot of the ring is waited for.
+        bool ok = true, free = false;   // free: the next slot is
+        uint32_t seq = 0;
+        auto wait_slot = [&]() {
+            if (!free && seq >= ST_SLOTS) ok = mbar_wait_warp(&empty[seq % ST_SLOTS], (seq / ST_SLOTS - 1) & 1u, &err, DEV_ERR_WAIT_EMPTY);
+            free = true;
+        };
+        for (uint64_t base = blockIdx.x; base < items && ok; base += 32ull * gridDim.x) {
+            const uint64_t item = base + (uint64_t)lane * gridDim.x;
+            ItemInfo f = {};
+            bool need = item < items;
+            if (need) {
+                f.piece = (uint32_t)item % p.n_pieces, f.b = (uint32_t)item / p.n_pieces % p.batch, f.r = (uint32_t)item / p.n_pieces / p.batch;
+                need = (int)f.r <= drafts_of(p, f.b);
+                const T* row = row_ptr(f.b, f.r);
+                f.head = min(p.vocab, (uint32_t)((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T)));
+                const uint32_t n_vec = (p.vocab - f.head) / VE;
+                f.tail = f.head + n_vec * VE;
+                f.v0 = f.piece * (PIECE / VE);
+                f.n = f.v0 < n_vec ? min(n_vec - f.v0, PIECE / VE) : 0;
+                const float t = temperature_of(p, f.b);
+                f.c = t > 0.f ? fminf(1.44269504f / t, 3e38f) : 1.f;
+                f.greedy = t == 0.f;
+            }
+            while (true) {
+                uint32_t stop = 0;
+                if (stops && need) stop = *reinterpret_cast<volatile uint32_t*>(&stops[f.b]);
+                wait_slot();
+                if (!ok) break;
+                need = need && STOP_BASE - (int)f.r >= (int)stop;
+                const unsigned mask = __ballot_sync(0xffffffffu, need);
+                if (!mask) break;
+                const uint32_t slot = seq % ST_SLOTS;
+                if (lane == __ffs(mask) - 1) {
+                    need = false;
+                    info[slot] = f;
+                    if (f.n) {
+                        mbar_arrive_expect_tx(&full[slot], f.n * 16);
+                        bulk_g2s(ring + slot * ST_BYTES, row_ptr(f.b, f.r) + f.head + f.v0 * VE, f.n * 16, &full[slot]);
+                    } else {
+                        mbar_arrive(&full[slot]);
+                    }
+                }
+                __syncwarp();
+                free = false;
+                ++seq;
             }
         }
-        if (stop && __shfl_sync(0xffffffffu, done, 0) == p.n_pieces) {   // the row's last piece: spare the rows behind it if its draft falls
-            __threadfence();
-            const Row row = row_of<T>(p, b, r, n, t, scale_of(t), pow2_table());
-            if (threadIdx.x == 0 && row.stands != 1) atomicMax(stop, (uint32_t)(STOP_BASE - (int)r));
+        for (int k = 0; k < ST_FINISH && ok; ++k) {   // an end mark for each group and each of the last warps
+            wait_slot();
+            if (!ok) break;
+            if (lane == 0) {
+                info[seq % ST_SLOTS].end = 1;
+                mbar_arrive(&full[seq % ST_SLOTS]);
+            }
+            __syncwarp();
+            free = false;
+            ++seq;
+        }
+        for (uint32_t q = seq > ST_SLOTS ? seq - ST_SLOTS : 0; q < seq; ++q)   // nothing may still be in flight into this CTA's shared memory when it leaves
+            mbar_wait_warp(&full[q % ST_SLOTS], (q / ST_SLOTS) & 1u, &err, DEV_ERR_WAIT_DRAIN);
+    } else if (warp <= ST_GROUPS * ST_WARPS) {
+        // ================= maximum and sum =================
+        const uint32_t group = (warp - 1) / ST_WARPS, w = (warp - 1) % ST_WARPS;
+        for (uint32_t seq = group;; seq += ST_GROUPS) {
+            const uint32_t slot = seq % ST_SLOTS;
+            if (!mbar_wait_warp(&full[slot], (seq / ST_SLOTS) & 1u, &err, DEV_ERR_WAIT_FULL)) break;
+            const ItemInfo& f = info[slot];
+            if (f.end) break;
+            const float c = f.c;
+            const uint32_t n = f.n, v0 = f.v0, head = f.head;
+            const uint4* src = reinterpret_cast<const uint4*>(ring + slot * ST_BYTES);
+            constexpr int NV = ST_BYTES / 16 / (ST_WARPS * 32);
+            const uint32_t i0 = w * 32 + lane;
+            float x[NV * VE], extra = -INFINITY;
+            uint32_t extra_at = 0;
+            if (w == 0) {
+                const T* row = row_ptr(f.b, f.r);
+                if (f.piece == 0 && lane < (int)head) extra_at = lane, extra = logit<T>(row, extra_at);
+                if (f.piece + 1 == p.n_pieces && lane >= 16 && f.tail + lane - 16 < p.vocab) extra_at = f.tail + lane - 16, extra = logit<T>(row, extra_at);
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const uint32_t i = i0 + j * (ST_WARPS * 32);
+                unpack_logits<T>(i < n ? src[i] : make_uint4(0, 0, 0, 0), i < n, &x[j * VE]);
+            }
+            float top = extra;
+#pragma unroll
+            for (int j = 0; j < NV * (int)VE; ++j) top = fmaxf(top, x[j]);
+            const float mine = top;
+            top = warp_max(top);
+            const float ref = top == -INFINITY ? 0.f : top;
+            float sum = ex2((extra - ref) * c);
+#pragma unroll
+            for (int j = 0; j < NV * (int)VE; ++j) sum += ex2((x[j] - ref) * c);   // NaN for a NaN and for +inf
+            int first = 0x7fffffff;
+            if (f.greedy && mine == top) {   // the first index of the maximum
+                if (extra == top) first = (int)extra_at;
+#pragma unroll
+                for (int j = 0; j < NV * (int)VE; ++j)
+                    if (x[j] == top) first = min(first, (int)(head + (v0 + i0 + j / VE * (ST_WARPS * 32)) * VE + j % VE));
+            }
+            const Piece a{top, warp_sum(sum), __reduce_min_sync(0xffffffffu, first), 0};
+            if (lane == 0) {
+                parts[slot][w] = a;
+                mbar_arrive(&parts_full[slot]);
+            }
+        }
+    } else {
+        // ================= pieces put together =================
+        const uint32_t who = warp - 1 - ST_GROUPS * ST_WARPS;
+        for (uint32_t seq = who;; seq += ST_FINISH) {
+            const uint32_t slot = seq % ST_SLOTS, round = (seq / ST_SLOTS) & 1u;
+            if (!mbar_wait_warp(&full[slot], round, &err, DEV_ERR_WAIT_FULL)) break;
+            const ItemInfo f = info[slot];
+            if (f.end) break;
+            if (!mbar_wait_warp(&parts_full[slot], round, &err, DEV_ERR_WAIT_FULL)) break;
+            Piece y = lane < ST_WARPS ? parts[slot][lane] : Piece{-INFINITY, 0.f, 0x7fffffff, 0};
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[slot]);
+            const uint32_t piece = f.piece, b = f.b, r = f.r;
+            const float c = f.c;
+            const float all = warp_max(y.top);
+            y.sum = warp_sum(y.top == -INFINITY ? y.sum : y.sum * ex2((y.top - all) * c));
+            y.first = __reduce_min_sync(0xffffffffu, y.top == all ? y.first : 0x7fffffff);
+            uint32_t done = 0;
+            if (lane == 0) {
+                *reinterpret_cast<int4*>(&p.pieces[((uint64_t)b * p.rows + r) * p.n_pieces + piece]) = make_int4(__float_as_int(all), __float_as_int(y.sum), y.first, 0);
+                // releases this piece, acquires the others'
+                if (stops) asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(done) : "l"(&p.tickets[(uint64_t)b * p.rows + r]) : "memory");
+                ++done;
+            }
+            if (stops && __shfl_sync(0xffffffffu, done, 0) == p.n_pieces) {   // the row's last piece: spare the rows behind it if its draft falls
+                asm volatile("fence.acq_rel.gpu;" ::: "memory");
+                const float t = temperature_of(p, b);
+                const Row row = row_of<T>(p, b, r, drafts_of(p, b), t, scale_of(t), tab);
+                if (lane == 0 && row.stands != 1) atomicMax(&stops[b], (uint32_t)(STOP_BASE - (int)r));
+            }
         }
     }
+    __syncthreads();
+    if (err)   // a wait has run out: none of this CTA's rows is a distribution
+        for (uint64_t item = blockIdx.x + (uint64_t)threadIdx.x * gridDim.x; item < items; item += (uint64_t)blockDim.x * gridDim.x)
+            *reinterpret_cast<int4*>(&p.pieces[(item / p.n_pieces % p.batch * p.rows + item / p.n_pieces / p.batch) * p.n_pieces + item % p.n_pieces]) =
+                make_int4(0, 0x7fffffff, 0, 0);
 }
 
-// Adds up one value a CTA of the cluster, in rank order: what the ranks before this one hold, and the whole.
-__device__ __forceinline__ void cluster_sum(cg::cluster_group& cluster, double* slots, double mine, double* before, double* whole) {
-    const unsigned rank = cluster.block_rank();
-    if (threadIdx.x < DRAW_CLUSTER) cluster.map_shared_rank(slots, threadIdx.x)[rank] = mine;
-    cluster.sync();
-    double b = 0.0, w = 0.0;
-    for (unsigned i = 0; i < DRAW_CLUSTER; ++i) {
-        if (i == rank) b = w;
-        w += slots[i];
+// Running sums over lanes, this lane's included.
+__device__ __forceinline__ double warp_scan(double v, uint32_t lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, v, o);
+        if ((int)lane >= o) v += y;
     }
-    *before = b;
-    *whole = w;
+    return v;
 }
 
 // four logits from `at` on, of those below `end`; the others -inf
 template <typename T>
-__device__ __forceinline__ void load4(const T* row, uint32_t at, uint32_t end, bool vec, float (&x)[4]) {
+__device__ __forceinline__ void load4(const T* row, uint32_t at, uint32_t end, bool vec, float* x) {
     if (vec && at + 4 <= end) {
         if (sizeof(T) == 4) {
             const float4 w = __ldg(reinterpret_cast<const float4*>(row + at));
@@ -249,25 +393,22 @@ __device__ __forceinline__ void load4(const T* row, uint32_t at, uint32_t end, b
         for (int e = 0; e < 4; ++e) x[e] = at + e < end ? logit<T>(row, at + e) : -INFINITY;
     }
 }
-__device__ __forceinline__ double warp_sum64(double v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 template <typename T>
-__global__ void __cluster_dims__(DRAW_CLUSTER, 1, 1) __launch_bounds__(DRAW_THREADS) verify_draw_kernel(const __grid_constant__ VerifyParams p) {
-    pdl_prologue();
+__global__ void __launch_bounds__(DRAW_THREADS, 1) verify_draw_kernel(const __grid_constant__ VerifyParams p) {
+    pdl_launch_dependents();
+    const double tab = pow2_table();
+    pdl_wait();
     cg::cluster_group cluster = cg::this_cluster();
     __shared__ double slots[3][DRAW_CLUSTER];
     __shared__ double warp_sums[DRAW_WARPS];
     __shared__ double segments[DRAW_WARPS][DRAW_SEGMENTS];
     __shared__ Row rows[DFL_MAX_VERIFY_DRAFTS + 1];
     __shared__ int found;
-    const uint32_t b = blockIdx.x / DRAW_CLUSTER, rank = cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t size = cluster.num_blocks(), b = blockIdx.x / size, rank = cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int K = (int)p.rows - 1, n = drafts_of(p, b);
     const float t = temperature_of(p, b);
-    const double scale = scale_of(t), tab = pow2_table();
+    const float u_sample = p.u_sample[b];
+    const double scale = scale_of(t);
     if (threadIdx.x == 0) found = -1;
     cluster.barrier_arrive();
     // a warp a row, four rows a warp at a time until one decides
@@ -287,87 +428,110 @@ __global__ void __cluster_dims__(DRAW_CLUSTER, 1, 1) __launch_bounds__(DRAW_THRE
     const bool refused = taken < n, ok = row.stands >= 0;
     cluster.barrier_wait();   // every CTA of the cluster has started
     if (ok && t > 0.f) {
-        const int d = refused ? p.drafts[(uint64_t)b * K + taken] : -1;
+        int d = refused && !p.probs ? p.drafts[(uint64_t)b * K + taken] : -1;   // the token that has no weight
         const T* x_row = static_cast<const T*>(p.logits) + b * p.x_b + taken * p.x_r;
         const float* q_row = p.probs + b * p.q_b + taken * p.q_r;
         const bool x_vec = reinterpret_cast<uintptr_t>(x_row) % (4 * sizeof(T)) == 0, q_vec = reinterpret_cast<uintptr_t>(q_row) % 16 == 0;
         // the row in vocabulary order over the cluster's warps: a run of `count` segments of `seg` tokens each
-        constexpr uint32_t N_WARPS = DRAW_CLUSTER * DRAW_WARPS;
-        const uint32_t blocks = (p.vocab + 127) / 128, per = (blocks + N_WARPS - 1) / N_WARPS, seg_blocks = (per + DRAW_SEGMENTS - 1) / DRAW_SEGMENTS;
+        const uint32_t n_warps = size * DRAW_WARPS;
+        const uint32_t blocks = (p.vocab + 127) / 128, per = (blocks + n_warps - 1) / n_warps, seg_blocks = (per + 2 * DRAW_SEGMENTS - 1) / (2 * DRAW_SEGMENTS) * 2;
         const uint32_t b0 = min(blocks, (rank * DRAW_WARPS + warp) * per), b1 = min(blocks, b0 + per);   // blocks of 128 tokens, four a lane
-        const double top = (double)row.top;
+        const Expo ex = expo(row.top, scale, tab);
         double z = 1.0;
-        int mode = refused ? (p.probs ? 2 : 1) : 0;   // 0 w, 1 w without the draft, 2 max(p - q, 0)
-        auto weights = [&](uint32_t block, double (&w)[4]) {
+        // two kinds of weight: w, without the refused draft's (kind W), and max(p - q, 0) (kind R)
+        using W = std::false_type;
+        using R = std::true_type;
+        auto fetch = [&](auto kind, uint32_t block, float* x, float* q) {
             const uint32_t at = block * 128 + lane * 4;
-            float x[4], q[4];
             load4<T>(x_row, at, p.vocab, x_vec, x);
-            if (mode == 2) {
-                if (at < p.vocab) load4<float>(q_row, at, p.vocab, q_vec, q);
-                else q[0] = q[1] = q[2] = q[3] = 0.f;
-            }
+            if (kind.value) load4<float>(q_row, at, p.vocab, q_vec, q);   // behind the row nothing is read
+        };
+        // of N / 4 blocks one behind the other
+        auto weights = [&](auto kind, uint32_t block, const float* x, const float* q, auto& w) {
+            constexpr int N = sizeof(w) / sizeof(double);
+            const uint32_t at = block * 128 + lane * 4;
+            weights_of<N>(ex, x, w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                w[e] = pow2_32nd(__dmul_rn((double)x[e] - top, scale), tab);
-                if (mode == 1 && (int)(at + e) == d) w[e] = 0.0;
-                if (mode == 2) w[e] = at + e < p.vocab ? fmax(fma(w[e], z, -(double)q[e]), 0.0) : 0.0;
+            for (int i = 0; i < N; ++i) {
+                const uint32_t token = at + i / 4 * 128 + i % 4;
+                if (kind.value) w[i] = token < p.vocab ? fmax(fma(w[i], z, -(double)q[i]), 0.0) : 0.0;
+            }
+            if (!kind.value && d >= 0 && (uint32_t)d / 128 - block < N / 4) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) w[i] = (uint32_t)d == at + i / 4 * 128 + i % 4 ? 0.0 : w[i];
             }
         };
-        double before = 0.0, whole = 0.0, in_cta = 0.0, mine = 0.0;
-        auto sum_up = [&](int slot) {
-            mine = 0.0;
-            for (uint32_t s = 0, bl = b0; bl < b1; ++s) {
-                double sum = 0.0;
-                for (uint32_t k = 0; k < seg_blocks && bl < b1; ++k, ++bl) {
-                    double w[4];
-                    weights(bl, w);
-                    sum += (w[0] + w[1]) + (w[2] + w[3]);
+        double whole = 0.0, start = 0.0, end = 0.0;   // of the row, of the warp's run
+        auto sum_up = [&](auto kind, int slot) {
+            // two blocks at a time, the next two on their way; lanes are added up once a segment of an even number of blocks
+            double mine = 0.0;
+            float x[8], q[8], x_next[8], q_next[8];
+            fetch(kind, b0, x_next, q_next);
+            fetch(kind, b0 + 1, x_next + 4, q_next + 4);
+            double sum = 0.0;
+            uint32_t s = 0, in_seg = 0;
+            for (uint32_t bl = b0; bl < b1; bl += 2) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = x_next[i], q[i] = kind.value ? q_next[i] : 0.f;
+                fetch(kind, bl + 2, x_next, q_next);
+                fetch(kind, bl + 3, x_next + 4, q_next + 4);
+                double w[8];
+                weights(kind, bl, x, q, w);
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
+                if (bl + 1 < b1) sum += (w[4] + w[5]) + (w[6] + w[7]);
+                in_seg += 2;
+                if (in_seg == seg_blocks || bl + 2 >= b1) {
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane == 0) segments[warp][s] = sum;
+                    mine += sum;
+                    sum = 0.0;
+                    in_seg = 0;
+                    ++s;
                 }
-                sum = warp_sum64(sum);
-                if (lane == 0) segments[warp][s] = sum;
-                mine += sum;
             }
             __syncthreads();   // warp_sums of an earlier call are read
             if (lane == 0) warp_sums[warp] = mine;
             __syncthreads();
-            double cta = 0.0;
-            in_cta = 0.0;
-            for (int w = 0; w < DRAW_WARPS; ++w) {
-                if (w == (int)warp) in_cta = cta;
-                cta += warp_sums[w];
-            }
-            cluster_sum(cluster, slots[slot], cta, &before, &whole);
+            // Running sums of the CTA's warps, of the cluster's CTAs.  Every warp makes the same ones, and the end of a run is the same number as
+            // the next one's start, so the runs share [0, whole) out without gap or overlap.
+            const double in_cta = warp_scan(lane < DRAW_WARPS ? warp_sums[lane] : 0.0, lane);
+            const double in_all = __shfl_sync(0xffffffffu, in_cta, DRAW_WARPS - 1);
+            if (warp == 0 && lane < size) cluster.map_shared_rank(slots[slot], lane)[rank] = in_all;
+            cluster.sync();
+            const double in_row = warp_scan(lane < size ? slots[slot][lane] : 0.0, lane);
+            whole = __shfl_sync(0xffffffffu, in_row, size - 1);
+            const double before = rank ? __shfl_sync(0xffffffffu, in_row, rank - 1) : 0.0;
+            start = warp ? before + __shfl_sync(0xffffffffu, in_cta, warp - 1) : before;
+            end = warp + 1 < DRAW_WARPS ? before + __shfl_sync(0xffffffffu, in_cta, warp) : __shfl_sync(0xffffffffu, in_row, rank);
         };
-        if (mode == 2) {
-            mode = 0;
-            sum_up(0);
+        bool rest = refused && p.probs;   // drawn from the residual
+        if (rest) {
+            sum_up(W{}, 0);
             z = 1.0 / whole;
-            mode = 2;
+            sum_up(R{}, 1);
+            rest = whole > 0.0;            // nothing may be left of p beside q: then from p
         }
-        sum_up(1);
-        if (!(whole > 0.0)) {   // nothing is left of p beside q
-            mode = 0;
-            sum_up(2);
-        }
-        // inside [0, whole) even if u is not inside [0, 1); the runs share that range out without gap or overlap, their ends being the
-        // same sums as the next ones' starts
-        double target = fmax((double)p.u_sample[b] * whole, 0.0);
+        if (!rest) sum_up(W{}, 2);
+        // inside [0, whole) even if u is not inside [0, 1)
+        double target = fmax((double)u_sample * whole, 0.0);
         if (!(target < whole)) target = __longlong_as_double(__double_as_longlong(whole) - 1);
-        const double start = before + in_cta, end = before + (in_cta + mine);
         if (start <= target && end > target) {
             double upto = start;
             uint32_t s = 0, bl = b0;
             while (bl + seg_blocks < b1 && !(upto + segments[warp][s] > target)) upto += segments[warp][s++], bl += seg_blocks;
             int hit = -1, last = -1;
             for (; bl < b1 && hit < 0; ++bl) {
+                float x[4], q[4];
                 double w[4];
-                weights(bl, w);
-                double own = (w[0] + w[1]) + (w[2] + w[3]), sum = own;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double y = __shfl_up_sync(0xffffffffu, sum, o);
-                    if ((int)lane >= o) sum += y;
+                if (rest) {
+                    fetch(R{}, bl, x, q);
+                    weights(R{}, bl, x, q, w);
+                } else {
+                    fetch(W{}, bl, x, q);
+                    weights(W{}, bl, x, q, w);
                 }
+                const double own = (w[0] + w[1]) + (w[2] + w[3]), sum = warp_scan(own, lane);
                 double run = upto + (sum - own);
                 int at = -1, some = -1;
 #pragma unroll
@@ -400,19 +564,17 @@ __global__ void __cluster_dims__(DRAW_CLUSTER, 1, 1) __launch_bounds__(DRAW_THRE
 }
 
 struct Split {
-    uint32_t piece, n_pieces;
+    uint32_t n_pieces;
     bool tickets;
     uint64_t piece_bytes, ticket_bytes;
 };
 Split split_of(const dfl_verify_drafts_args* a) {
-    constexpr uint32_t piece = ST_THREADS * 32;
+    const uint32_t piece = ST_BYTES / (a->dtype == DFL_F32 ? 4 : 2);
     Split s;
-    s.piece = piece;
     s.n_pieces = (uint32_t)((a->vocab + piece - 1) / piece);
     const uint64_t rows = (uint64_t)a->batch * (a->n_drafts + 1);
-    // Rows behind a draft that falls are spared where they start late enough to know: with more pieces than run at once.  The counters have to be
-    // cleared, a launch of 2 us.
-    s.tickets = a->n_drafts > 0 && rows * s.n_pieces > 2000;
+    // Sparing rows pays with more pieces than the rings hold at once.  The counters have to be cleared, a launch of 2 us.
+    s.tickets = a->n_drafts > 0 && rows * s.n_pieces > 2 * 148 * ST_SLOTS;
     s.piece_bytes = (rows * s.n_pieces * sizeof(Piece) + 255) / 256 * 256;
     s.ticket_bytes = s.tickets ? (rows + a->batch) * sizeof(uint32_t) : 0;
     return s;
@@ -437,9 +599,30 @@ dfl_status check(const dfl_verify_drafts_args* a, bool pointers) {
 
 template <typename T>
 cudaError_t launch(const VerifyParams& p, cudaStream_t st) {
-    const cudaError_t e = launch_k(verify_pieces_kernel<T>, dim3(p.n_pieces * p.rows * p.batch), dim3(ST_THREADS), 0, st, p);
+    const uint64_t items = (uint64_t)p.n_pieces * p.batch * p.rows, most = (uint64_t)sm_count();
+    cudaError_t e = cudaFuncSetAttribute(verify_pieces_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, ST_SLOTS * ST_BYTES);
     if (e != cudaSuccess) return e;
-    return launch_k(verify_draw_kernel<T>, dim3(p.batch * DRAW_CLUSTER), dim3(DRAW_THREADS), 0, st, p);
+    e = launch_k(verify_pieces_kernel<T>, dim3((unsigned)(items < most ? items : most)), dim3(ST_THREADS), ST_SLOTS * ST_BYTES, st, p);
+    if (e != cudaSuccess) return e;
+    // As many CTAs a request as leave a single wave: they share the exponentials, but each decides for itself.  151 936 tokens: 14 us with sixteen for one
+    // request, 42 us with one each for 128 (with eight each 83 us).
+    uint32_t cluster = DRAW_CLUSTER;
+    while (cluster > 1 && (uint64_t)cluster * p.batch > (uint64_t)sm_count()) cluster /= 2;
+    const cudaError_t f = cudaFuncSetAttribute(verify_draw_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (f != cudaSuccess) return f;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.batch * cluster);
+    cfg.blockDim = dim3(DRAW_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, verify_draw_kernel<T>, p);
 }
 
 }  // namespace
@@ -472,7 +655,7 @@ extern "C" dfl_status dfl_verify_drafts(int32_t device, const dfl_verify_drafts_
     p.x_b = a->batch > 1 ? a->logits_batch_stride : 0, p.x_r = a->n_drafts ? a->logits_row_stride : 0;
     p.q_b = a->batch > 1 ? a->probs_batch_stride : 0, p.q_r = a->n_drafts > 1 ? a->probs_row_stride : 0;
     const Split s = split_of(a);
-    p.batch = a->batch, p.rows = a->n_drafts + 1, p.vocab = (uint32_t)a->vocab, p.piece = s.piece, p.n_pieces = s.n_pieces;
+    p.batch = a->batch, p.rows = a->n_drafts + 1, p.vocab = (uint32_t)a->vocab, p.n_pieces = s.n_pieces;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (s.tickets) {
         p.tickets = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a->workspace) + s.piece_bytes);
