@@ -13,10 +13,13 @@
 // runs are split until the items fill the machine, so a few rows over a long prefix use every SM.
 //
 // One persistent CTA an SM; S = Q K^T and O += P V on the tensor cores (tcgen05, both accumulators and P in tensor memory), K and V tiles by
-// TMA into a ring.  Two warpgroups of softmax threads (thread = row), one MMA issuer, one producer.  Up to a head width of 128 the
-// warpgroups have a row tile each (or, when the item has at most 128 rows, every other key tile of the same rows), so one's products run
-// under the other's exponentials; at 256 the output takes half of tensor memory, and one warpgroup works on two score buffers in turn.
-// Step t uses score buffer t & 1 throughout: S(t) is issued behind PV(t - 2), which read that buffer's P.
+// TMA into a ring.  Two warpgroups of softmax threads (thread = row), one MMA issuer, one producer.  A step is a key tile.
+//   * head widths 64 and 128: two streams, each with its warpgroup, score buffer and accumulator, half a step apart, so that one's products run under the
+//     other's exponentials; a row tile each or, when the item has at most 128 rows, every other key tile of the same rows (two parts of a row
+//     then).  P goes out in two halves, the first half's product runs under the second half's exponentials.  (Two buffers of 64 keys a stream
+//     instead were slower: the product of a 64-key tile reads Q from shared memory as often as that of a 128-key tile, 192 bytes a clock.)
+//   * 256: the output takes half of tensor memory, there is one stream with two score buffers; the warpgroups take a half of each key tile's columns,
+//     agree on the maximum through shared memory and scale and write a half of the output's columns each.
 #include <cuda.h>
 
 #include <cmath>
@@ -31,7 +34,7 @@ using namespace ts;
 
 constexpr int BA_KEYS = 128;             // keys of a tile
 constexpr int BA_ROWS = 128;             // rows of a tile
-constexpr int BA_THREADS = 384;          // 2 x 4 softmax warps, MMA issue, producer, two idle warps that make a warpgroup of the last four
+constexpr int BA_THREADS = 384;          // 2 x 4 softmax warps, MMA issue, producer, two idle warps that fill the warpgroup
 // A softmax thread holds a row of 128 scores: of the 168 registers a thread of the launch the last warpgroup gives most away (2 x 216 + 72 = 3 x 168).
 constexpr int BA_REGS_SOFTMAX = 216, BA_REGS_REST = 72;
 constexpr int BA_BOX = BA_KEYS * 128;    // one TMA box: 128 keys x 64 dimensions of 16 bits, 128-byte swizzle
@@ -39,16 +42,22 @@ constexpr float BA_RESCALE = 8.f;        // a row's reference maximum moves when
 
 template <int D>
 struct BaCfg {
-    static constexpr int UNIT = D < 128 ? D : 128;                // dimensions of a ring slot
+    static constexpr bool SPLIT = D > 128;                        // the warpgroups share the rows, each has half the columns
+    static constexpr int UNIT = D == 128 ? 128 : 64;              // dimensions of a ring slot
     static constexpr int UNITS = D / UNIT;                        // slots of a K or V tile
     static constexpr int SLOT = BA_KEYS * UNIT * 2;
-    static constexpr int SLOTS = D == 64 ? 8 : 5;
-    static constexpr int TILES = D <= 128 ? 2 : 1;                // row tiles of a CTA
+    static constexpr int SLOTS = 4 * 32768 / SLOT;
+    static constexpr int TILES = SPLIT ? 1 : 2;                   // row tiles of a CTA
     static constexpr int Q_BYTES = BA_ROWS * D * 2;
     static constexpr int OFF_RING = TILES * Q_BYTES;
-    static constexpr int OFF_BAR = OFF_RING + SLOTS * SLOT;
-    static constexpr int SMEM = OFF_BAR + 256 + 1024;             // barriers, alignment of the base
+    static constexpr int OFF_STAGE = OFF_RING + SLOTS * SLOT;     // 4 KB a softmax warp on its way out
+    static constexpr int OFF_EXCH = OFF_STAGE + 8 * 4096;         // SPLIT: [2][2][128] maxima
+    static constexpr int OFF_BAR = OFF_EXCH + (SPLIT ? 2048 : 0);
+    static constexpr int SMEM = OFF_BAR + 320;                    // barriers, two words
     static constexpr uint32_t TM_S = 0, TM_O = 256;               // columns: two score buffers, the accumulators
+    static constexpr int BUFS = SPLIT ? 2 : 1;                    // score buffers of a stream
+    static constexpr int S_COLS = SPLIT ? 64 : 128;               // columns of a score buffer that are a thread's
+    static constexpr int O_COLS = SPLIT ? D / 2 : D;              // of the output, that a warpgroup scales and writes
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -121,10 +130,6 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
                  : "memory");
 }
 
-// Barriers of a step: by its warpgroup, 0 and 1 when both work; one that works alone has 0 for its even and 2 for its odd steps.  A parity wait only
-// tells a phase from the one before to a party that has seen every phase: none has a barrier that another warpgroup's steps go by.
-__device__ __forceinline__ int bar_of(bool two, int t) { return (t & 1) == 0 ? 0 : two ? 1 : 2; }
-
 // What every role works out alike from an item's number.
 struct Item {
     uint32_t h, row0, row_end;   // rows row0.. of the KV head's, below row_end
@@ -132,10 +137,13 @@ struct Item {
     int p0, p1, o0, o1;          // tiles of the prefix, of the own keys
     uint32_t part;               // where its rows' parts go
     int own, q_len;              // lengths of the request (own items)
-    bool pair;                   // the warpgroups share the rows
-    bool two;                    // both warpgroups work
-    int tiles, steps;
+    bool pair;                   // the warpgroups take the key tiles of the same rows in turn
+    bool two;                    // there are two streams
+    int tiles;
 };
+// steps of a stream: all tiles, or every other one
+__device__ __forceinline__ int steps_of(const Item& it, int stream) { return it.pair ? (it.tiles + 1 - stream) / 2 : stream == 0 || it.two ? it.tiles : 0; }
+
 template <int D>
 __device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx) {
     constexpr uint32_t BLOCK = BaCfg<D>::TILES * BA_ROWS;
@@ -165,9 +173,9 @@ __device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx) 
         it.q_len = q_len_of(p, it.b);
         const uint32_t there = (uint32_t)it.q_len * p.group;
         it.row_end = it.b * per + (first < there ? min(there, per) : first);
-        // keys that the block's last row sees
         const uint32_t last = min(first + (it.pair ? BA_ROWS : BLOCK), there);
-        const int seen = last > first ? min(it.own, max(0, it.own - it.q_len + (int)((last - 1) / p.group) + 1)) : 0;
+        const int seen = last > first ?   // own keys that the block's last row sees
+             min(it.own, max(0, it.own - it.q_len + (int)((last - 1) / p.group) + 1)) : 0;
         const int pre = p.fused ? (int)p.prefix_tiles : 0, all = pre + (seen + BA_KEYS - 1) / BA_KEYS;
         const int t0 = (int)(split * p.o_run), t1 = min(all, t0 + (int)p.o_run);
         it.p0 = min(t0, pre), it.p1 = min(max(t1, it.p0), pre);
@@ -176,8 +184,37 @@ __device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx) 
     }
     it.two = BaCfg<D>::TILES == 2 && (it.pair || it.row_end > it.row0 + BA_ROWS);
     it.tiles = it.row_end > it.row0 ? (it.p1 - it.p0) + (it.o1 - it.o0) : 0;
-    it.steps = it.two && !it.pair ? 2 * it.tiles : it.tiles;
     return it;
+}
+
+// A softmax thread's row.
+struct RowRef {
+    uint32_t r;          // of the KV head's rows
+    bool there;          // the item has it
+    uint32_t b, tok, head;
+    int sees;            // own keys
+};
+__device__ __forceinline__ RowRef row_ref(const BatchAttnParams& p, const Item& it, uint32_t tile, uint32_t row) {
+    RowRef x;
+    x.r = it.row0 + tile * BA_ROWS + row;
+    x.there = x.r < it.row_end;
+    const uint32_t per = p.n * p.group, rem = x.r % per;
+    x.b = x.r / per;
+    x.tok = rem / p.group;
+    x.head = it.h * p.group + rem - x.tok * p.group;
+    x.sees = min(it.own, max(0, it.own - it.q_len + (int)x.tok + 1));
+    return x;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// what was loaded from tensor memory is there: nothing that uses it moves ahead of the wait
+__device__ __forceinline__ void pin(float* v) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]));
 }
 
 template <typename T, int D>
@@ -185,18 +222,18 @@ __global__ void __launch_bounds__(BA_THREADS, 1)
 batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_constant__ CUtensorMap map_pk, const __grid_constant__ CUtensorMap map_pv,
                      const __grid_constant__ CUtensorMap map_ok, const __grid_constant__ CUtensorMap map_ov) {
     using C = BaCfg<D>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* ring = smem + C::OFF_RING;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t* empty = full + C::SLOTS;
-    uint64_t* q_full = empty + C::SLOTS;
-    uint64_t* s_full = q_full + 2;
-    uint64_t* p_full = s_full + 3;
-    uint64_t* pv_done = p_full + 3;
-    uint64_t* tail = pv_done + 3;
-    __shared__ uint32_t tmem_slot;
-    __shared__ int err;   // a wait has run out: what is left is filled with NaN
+    uint64_t* q_full = empty + C::SLOTS;   // [stream]
+    uint64_t* s_full = q_full + 2;         // [stream], or the one stream's [buffer]
+    uint64_t* p_full = s_full + 4;         // [stream][half], or [buffer]
+    uint64_t* pv_done = p_full + 4;        // [stream] once an item, or [buffer]
+    uint64_t* exch = pv_done + 4;          // [warp of a warpgroup]
+    uint64_t* tail = exch + 4;
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(tail + 1);
+    int& err = *reinterpret_cast<int*>(tail + 2);   // a wait has run out: what is left is filled with NaN
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -204,14 +241,15 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 4);
-        for (int i = 0; i < 3; ++i) {
+        for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], C::SPLIT ? 8 : 4);
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[i], C::SPLIT ? 8 : 4);
             mbar_init(&pv_done[i], 1);
+            mbar_init(&exch[i], 2);
         }
         mbar_init(tail, 1);
-        err = 0;
+        err = smem_u32(smem) % 1024;   // the swizzle goes by address: nothing would be right
         mbar_fence_init();
     }
     if (warp == 8) tmem_alloc(&tmem_slot, 512);
@@ -220,137 +258,187 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
     pdl_prologue();
-
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BA_REGS_SOFTMAX));
         // ================= softmax: thread = row =================
-        const int wg = warp >> 2, row = 32 * (warp & 3) + lane;
-        const uint32_t tm_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const uint32_t tm_o = tm_lane + C::TM_O + (C::TILES == 2 ? (uint32_t)(wg * D) : 0u);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BA_REGS_SOFTMAX));
+        const int wg = warp >> 2, wq = warp & 3, row = 32 * wq + lane, stream = C::SPLIT ? 0 : wg;
+        const uint32_t tm_lane = tmem + ((uint32_t)(32 * wq) << 16);
+        const uint32_t tm_o = tm_lane + C::TM_O + (uint32_t)(wg * C::O_COLS);
         const float c = p.scale * 1.4426950408889634f;
-        uint8_t* q_rows = smem + wg * C::Q_BYTES + (warp & 3) * 32 * 128;   // this warp's rows of each block of 64 dimensions
-        uint32_t even = 0, odd = 0, alone = 0;   // uses of the barriers so far
-        for (uint32_t idx = blockIdx.x; idx < p.items; idx += gridDim.x) {
-            const Item it = item_of<D>(p, idx);
-            if (wg > 0 && !it.two) continue;
-            const uint32_t base0 = even, base1 = it.two ? odd : alone;
-            even += (uint32_t)(it.steps + 1) / 2;
-            (it.two ? odd : alone) += (uint32_t)it.steps / 2;
-            auto parity = [&](int t) { return ((t & 1 ? base1 : base0) + (uint32_t)(t >> 1)) & 1u; };
-            const uint32_t r = it.row0 + (it.two && !it.pair ? wg * BA_ROWS : 0) + row;
-            const bool there = r < it.row_end;
-            const uint32_t per = p.n * p.group, b = r / per, rem = r - b * per, tok = rem / p.group, g = rem - tok * p.group, head = it.h * p.group + g;
-            const int sees = min(it.own, max(0, it.own - it.q_len + (int)tok + 1));   // own items
-            const int first = it.two ? wg : 0, stride = it.two ? 2 : 1;
+        uint8_t* q_tile = smem + stream * C::Q_BYTES;
+        uint8_t* stage = smem + C::OFF_STAGE + warp * 4096;
+        uint32_t uses[2] = {0, 0}, swaps = 0, done = 0;   // of the stream's buffers, of the exchange; items with steps
+        // The rows of Q into the operand layout (row r, 16-byte chunk k at chunk k ^ (r & 7)), asynchronously: a warp its 32 rows, or the warps of both
+        // warpgroups 16 each of the same 32.
+        auto fetch_q = [&](const Item& it, const RowRef& rr) {
+            constexpr int CH = D / 8, ROWS = C::SPLIT ? 16 : 32;   // chunks of a row, rows of a warp
+            const int64_t off = rr.there ? rr.b * p.q_b + rr.tok * p.q_t + rr.head * p.q_h : 0;
+            const int r0 = C::SPLIT ? 16 * wg : 0;
+#pragma unroll 8
+            for (int i = lane; i < ROWS * CH; i += 32) {
+                const int r = r0 + i / CH, k = i % CH;
+                const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                const bool v = __shfl_sync(0xffffffffu, (int)rr.there, r) != 0;
+                uint8_t* dst = q_tile + (k >> 3) * BA_BOX + (32 * wq + r) * 128 + (((k & 7) ^ (r & 7)) << 4);
+                if (v) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(static_cast<const T*>(p.q) + o + k * 8) : "memory");
+                else *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+            }
+        };
+        uint32_t idx = blockIdx.x;
+        Item it = item_of<D>(p, idx);
+        RowRef rr = row_ref(p, it, it.pair ? 0 : stream, row);
+        if (steps_of(it, stream) > 0) fetch_q(it, rr);
+        while (true) {
+            const int steps = steps_of(it, stream), n_p = it.p1 - it.p0;
+            const uint32_t base0 = uses[0], base1 = uses[1];
+            uses[0] += (uint32_t)(C::SPLIT ? (steps + 1) / 2 : steps);
+            uses[1] += (uint32_t)(C::SPLIT ? steps / 2 : 0);
+            auto parity = [&](int u) { return (C::SPLIT ? (u & 1 ? base1 : base0) + (uint32_t)(u >> 1) : base0 + (uint32_t)u) & 1u; };
+            auto buf = [&](int u) { return C::SPLIT ? u & 1 : stream; };
             bool ok = *reinterpret_cast<volatile int*>(&err) == 0;
-            const bool active = __any_sync(0xffffffffu, there);
-            const bool stored = there && (!p.direct || (int)tok < q_len_of(p, b));
+            const bool active = __any_sync(0xffffffffu, rr.there);
             float m = -INFINITY, l = 0.f;
-            if (first < it.steps && ok) {
-                // the rows of Q into the operand layout: row r, 16-byte chunk k at chunk k ^ (r & 7)
-                const int64_t off = there ? b * p.q_b + tok * p.q_t + head * p.q_h : 0;
-                constexpr int CH = D / 8;   // chunks of a row
-#pragma unroll 4
-                for (int i = lane; i < 32 * CH; i += 32) {
-                    const int rr = i / CH, k = i % CH;
-                    const int64_t o = __shfl_sync(0xffffffffu, off, rr);
-                    const bool v = __shfl_sync(0xffffffffu, (int)there, rr) != 0;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (v) x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + o + k * 8);
-                    *reinterpret_cast<uint4*>(q_rows + (k >> 3) * BA_BOX + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) = x;
-                }
+            const int sees_all = __reduce_min_sync(0xffffffffu, rr.there ? rr.sees : 0x7fffffff);   // of own keys, every row of the warp
+            if (steps > 0) {
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[wg]);
+                if (lane == 0) mbar_arrive(&q_full[stream]);
             }
-            for (int t = first; t < it.steps && ok; t += stride) {
-                const int x = t & 1, tile = it.two && !it.pair ? t >> 1 : t;
-                ok = mbar_wait_warp_inline(&s_full[bar_of(it.two, t)], parity(t), &err, DEV_ERR_WAIT_FULL);
+            const uint32_t idx_next = idx + gridDim.x;
+            for (int u = 0; u < steps && ok; ++u) {
+                ok = mbar_wait_warp_inline(&s_full[buf(u)], parity(u), &err, DEV_ERR_WAIT_FULL);
                 if (!ok) break;
                 fence_after_sync();
+                if (u == steps - 1 && idx_next < p.items) {   // nothing reads Q any more: the next item's is on its way from here on
+                    const Item next = item_of<D>(p, idx_next);
+                    if (steps_of(next, stream) > 0) fetch_q(next, row_ref(p, next, next.pair ? 0 : stream, row));
+                }
+                constexpr int N = C::S_COLS;
+                const uint32_t tm_s = tm_lane + C::TM_S + 128u * buf(u) + (C::SPLIT ? 64u * wg : 0u);
+                auto hand_over = [&](int half) {   // of P, to the issuer
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[C::SPLIT ? buf(u) : 2 * stream + half]);
+                };
                 if (active) {
-                    const uint32_t tm_s = tm_lane + C::TM_S + 128u * (uint32_t)x;
-                    float s[128];
-                    tmem_ld32(tm_s, *reinterpret_cast<float(*)[32]>(s));
-                    tmem_ld32(tm_s + 32, *reinterpret_cast<float(*)[32]>(s + 32));
-                    tmem_ld32(tm_s + 64, *reinterpret_cast<float(*)[32]>(s + 64));
-                    tmem_ld32(tm_s + 96, *reinterpret_cast<float(*)[32]>(s + 96));
+                    float s[N];
+#pragma unroll
+                    for (int j = 0; j < N; j += 32) tmem_ld32(tm_s + j, *reinterpret_cast<float(*)[32]>(s + j));
                     wait_ld();
-                    const int n_p = it.p1 - it.p0;
-                    const int limit = tile < n_p ? p.prefix - (it.p0 + tile) * BA_KEYS : sees - (it.o0 + tile - n_p) * BA_KEYS;
-                    if (__any_sync(0xffffffffu, limit < BA_KEYS)) {
 #pragma unroll
-                        for (int j = 0; j < 128; ++j) s[j] = j < limit ? s[j] : -INFINITY;
+                    for (int j = 0; j < N; j += 32) pin(s + j);
+                    const int tile = it.pair ? 2 * u + stream : u, first = C::SPLIT ? 64 * wg : 0;
+                    const bool pre = tile < n_p;
+                    const int key0 = (pre ? it.p0 + tile : it.o0 + tile - n_p) * BA_KEYS + first;
+                    if (key0 + N > (pre ? p.prefix : sees_all)) {   // some row of the warp does not see all keys
+                        const int limit = (pre ? p.prefix : rr.sees) - key0;
+#pragma unroll
+                        for (int j = 0; j < N; ++j) s[j] = j < limit ? s[j] : -INFINITY;
                     }
-                    float top[4] = {s[0], s[1], s[2], s[3]};
+                    // The first half's weights are made against the maximum so far, beside the search for the new one: it moves seldom, and then they are
+                    // made again.  (Otherwise the exponentials wait 500 of 2400 clocks a step for it.)
+                    uint32_t w[32];
+                    uint64_t sum2[2] = {0, 0}, mc2 = 0;
+                    const uint64_t c2 = pack2(c, c);
+                    auto weight = [&](int j, int k) {
+                        float a, e;
+                        unpack2(fma2(pack2(s[j + 2 * k], s[j + 2 * k + 1]), c2, mc2), a, e);
+                        a = ex2(a), e = ex2(e);
+                        sum2[k & 1] = add2(sum2[k & 1], pack2(a, e));
+                        w[k] = Pair16<T>::pack(a, e);
+                    };
+                    auto refer = [&]() {   // weights go against m
+                        const float mc = m == -INFINITY ? 0.f : m * c - Pair16<T>::BIAS;
+                        mc2 = pack2(-mc, -mc);
+                        sum2[0] = sum2[1] = 0;
+                    };
+                    refer();
+                    float t4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int j = 4; j < 128; j += 4) {
+                    for (int k = 0; k < 32; ++k) {
+                        weight(0, k);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], s[j + k]);
+                        for (int j = 0; j < N / 64; ++j) t4[(N / 64 * k + j) & 3] = max3(t4[(N / 64 * k + j) & 3], s[(N / 64 * k + j) * 2], s[(N / 64 * k + j) * 2 + 1]);
                     }
-                    const float t4 = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                    const bool moves = m == -INFINITY ? t4 > -INFINITY : (t4 - m) * c > BA_RESCALE;
+                    float top = max3(fmaxf(t4[0], t4[1]), t4[2], t4[3]);
+                    if constexpr (C::SPLIT) {   // both warps of the rows agree on the maximum
+                        float* e = reinterpret_cast<float*>(smem + C::OFF_EXCH) + (swaps & 1) * 256;
+                        e[wg * 128 + row] = top;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&exch[wq]);
+                        ok = mbar_wait_warp_inline(&exch[wq], swaps & 1u, &err, DEV_ERR_WAIT_FULL);
+                        ++swaps;
+                        if (!ok) break;
+                        top = fmaxf(top, e[(wg ^ 1) * 128 + row]);
+                    }
+                    const bool moves = m == -INFINITY ? top > -INFINITY : (top - m) * c > BA_RESCALE;
                     if (__any_sync(0xffffffffu, moves)) {
-                        const float f = moves ? (m == -INFINITY ? 0.f : ex2((m - t4) * c)) : 1.f;
-                        if (t >= first + stride) {   // the accumulator holds earlier tiles: their products have to be done
-                            ok = mbar_wait_warp_inline(&pv_done[bar_of(it.two, t - stride)], parity(t - stride), &err, DEV_ERR_WAIT_DRAIN);
-                            if (!ok) break;
-                            fence_after_sync();
-#pragma unroll
-                            for (int j = 0; j < D; j += 16) {
+                        const float f = moves ? (m == -INFINITY ? 0.f : ex2((m - top) * c)) : 1.f;
+                        if (u > 0) {   // the accumulator holds earlier steps: their products have to be done
+                            if (C::SPLIT) {   // (with one score buffer they are, ahead of this step's scores)
+                                ok = mbar_wait_warp_inline(&pv_done[buf(u - 1)], parity(u - 1), &err, DEV_ERR_WAIT_DRAIN);
+                                if (!ok) break;
+                                fence_after_sync();
+                            }
+#pragma unroll 1
+                            for (int j = 0; j < C::O_COLS; j += 16) {
                                 float o[16];
-                                uint32_t u[16];
+                                uint32_t x[16];
                                 tmem_ld16(tm_o + j, o);
                                 wait_ld();
 #pragma unroll
-                                for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(o[k] * f);
-                                tmem_st16(tm_o + j, u);
+                                for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(o[k] * f);
+                                tmem_st16(tm_o + j, x);
                             }
                         }
                         l *= f;
-                        if (moves) m = t4;
+                        if (moves) m = top;
+                        refer();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) weight(0, k);
                     }
-                    const float mc = m == -INFINITY ? 0.f : m * c - Pair16<T>::BIAS;
-                    const uint64_t c2 = pack2(c, c), mc2 = pack2(-mc, -mc);
-                    uint64_t sum2[2] = {0, 0};
+                    tmem_st32(tm_s, w);
+                    wait_st();
+                    hand_over(0);
+                    if constexpr (N > 64) {
 #pragma unroll
-                    for (int j = 0; j < 64; j += 32) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            float a, e;
-                            unpack2(fma2(pack2(s[2 * (j + k)], s[2 * (j + k) + 1]), c2, mc2), a, e);
-                            a = ex2(a), e = ex2(e);
-                            sum2[k & 1] = add2(sum2[k & 1], pack2(a, e));
-                            w[k] = Pair16<T>::pack(a, e);
-                        }
-                        tmem_st32(tm_s + j, w);
+                        for (int k = 0; k < 32; ++k) weight(64, k);
+                        tmem_st32(tm_s + 32, w);
+                        wait_st();
+                        hand_over(1);
                     }
                     float a, e;
                     unpack2(add2(sum2[0], sum2[1]), a, e);
                     l += a + e;
-                    wait_st();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; j += 64) hand_over(j / 64);
                 }
-                fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[bar_of(it.two, t)]);
             }
-            // the last products of this warpgroup's accumulator
-            const int last = it.steps > first ? first + (it.steps - 1 - first) / stride * stride : -1;
-            if (last >= 0 && ok) {
-                ok = mbar_wait_warp_inline(&pv_done[bar_of(it.two, last)], parity(last), &err, DEV_ERR_WAIT_DRAIN);
+            // the last products of the accumulator
+            if (steps > 0 && ok) {
+                ok = mbar_wait_warp_inline(&pv_done[buf(steps - 1)], C::SPLIT ? parity(steps - 1) : done++ & 1u, &err, DEV_ERR_WAIT_DRAIN);
                 fence_after_sync();
             }
+            if (C::SPLIT && active && ok) {   // the warpgroups' sums
+                float* e = reinterpret_cast<float*>(smem + C::OFF_EXCH) + (swaps & 1) * 256;
+                e[wg * 128 + row] = l;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&exch[wq]);
+                ok = mbar_wait_warp_inline(&exch[wq], swaps & 1u, &err, DEV_ERR_WAIT_FULL);
+                ++swaps;
+                l = wg == 0 ? l + e[128 + row] : e[row] + l;
+            }
             if (!ok) l = __int_as_float(0x7fffffff);
-            const bool holds = last >= 0 && ok;   // the accumulator has something
-            if (!active) continue;
-            const uint32_t row_w = r - lane;      // the warp's first row
-            __syncwarp();
-            if (p.direct) {
+            const bool holds = steps > 0 && ok;   // the accumulator has something
+            const bool mine = active && (C::SPLIT || stream == 0 || it.two);
+            if (mine && p.direct) {
+                const bool stored = rr.there && (int)rr.tok < q_len_of(p, rr.b);
                 const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-                const int64_t off = there ? b * p.o_b + tok * p.o_t + head * p.o_h : 0;
+                const int64_t off = rr.there ? rr.b * p.o_b + rr.tok * p.o_t + rr.head * p.o_h + wg * (C::SPLIT ? C::O_COLS : 0) : 0;
 #pragma unroll 1
-                for (int k = 0; k < D / 64; ++k) {
+                for (int k = 0; k < C::O_COLS / 64; ++k) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         float o[32];
@@ -366,121 +454,148 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                                 const int at = 8 * i + 2 * e;
                                 w[e] = Pair16<T>::pack(holds && l != 0.f ? o[at] * inv : inv, holds && l != 0.f ? o[at + 1] * inv : inv);
                             }
-                            *reinterpret_cast<uint4*>(q_rows + lane * 128 + (((4 * j + i) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * j + i) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     }
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const int rr = 4 * i + (lane >> 3), ch = lane & 7;
-                        const int64_t o = __shfl_sync(0xffffffffu, off, rr);
-                        const uint4 w = *reinterpret_cast<const uint4*>(q_rows + rr * 128 + ((ch ^ (rr & 7)) << 4));
-                        if (__shfl_sync(0xffffffffu, (int)stored, rr)) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + o + 64 * k + 8 * ch) = w;
+                        const int r = 4 * i + (lane >> 3), ch = lane & 7;
+                        const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                        const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+                        if (__shfl_sync(0xffffffffu, (int)stored, r)) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + o + 64 * k + 8 * ch) = w;
                     }
                     __syncwarp();
                 }
-            } else {
+            } else if (mine) {
                 const uint64_t base = ((uint64_t)(it.part + (it.pair ? wg : 0)) * p.n_kv + it.h) * p.rows;
-                if (there) p.part_ml[base + r] = make_float2(m, l);
-                if (!holds) continue;   // a part without mass is not read
-                float* dst = p.part_o + (base + row_w) * D;
+                const uint32_t row_w = rr.r - lane;   // the warp's first row
+                if (rr.there && (!C::SPLIT || wg == 0)) p.part_ml[base + rr.r] = make_float2(m, l);
+                if (holds) {   // a part without mass is not read
+                    float* dst = p.part_o + (base + row_w) * D + wg * (C::SPLIT ? C::O_COLS : 0);
 #pragma unroll 1
-                for (int k = 0; k < D / 32; ++k) {
-                    float o[32];
-                    tmem_ld32(tm_o + 32 * k, o);
-                    wait_ld();
+                    for (int k = 0; k < C::O_COLS / 32; ++k) {
+                        float o[32];
+                        tmem_ld32(tm_o + 32 * k, o);
+                        wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<float4*>(q_rows + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                    __syncwarp();
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int rr = 4 * i + (lane >> 3), ch = lane & 7;
-                        const float4 w = *reinterpret_cast<const float4*>(q_rows + rr * 128 + ((ch ^ (rr & 7)) << 4));
-                        if (row_w + rr < it.row_end) *reinterpret_cast<float4*>(dst + (uint64_t)rr * D + 32 * k + 4 * ch) = w;
+                        for (int i = 0; i < 8; ++i) {
+                            const int r = 4 * i + (lane >> 3), ch = lane & 7;
+                            const float4 w = *reinterpret_cast<const float4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+                            if (row_w + r < it.row_end) *reinterpret_cast<float4*>(dst + (uint64_t)r * D + 32 * k + 4 * ch) = w;
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             }
+            if (idx_next >= p.items) break;
+            idx = idx_next;
+            it = item_of<D>(p, idx);
+            rr = row_ref(p, it, it.pair ? 0 : stream, row);
+            if (steps == 0 && steps_of(it, stream) > 0) fetch_q(it, rr);   // it was not fetched on the way
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BA_REGS_REST));
     }
     if (warp == 8) {
         // ================= MMA issue =================
+        // One warp for both streams: PV and S of a stream one behind the other, then the other's.  (With a warp each the streams' products went through the
+        // pipe interleaved, their scores came at the same time and so did their exponentials: 4650 clocks a tile of 2 x 128 rows.)
         constexpr uint32_t FMT = (Pair16<T>::FMT << 7) | (Pair16<T>::FMT << 10);
-        constexpr uint32_t ID_S = instr_desc(128) | FMT, ID_O = instr_desc(C::UNIT) | FMT | (1u << 16);   // V lies key by key: N-major
-        const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(smem);
-        uint32_t even = 0, odd = 0, alone = 0, q_uses[2] = {0, 0}, seq = 0;
-        bool ok = true;
-        for (uint32_t idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
-            const Item it = item_of<D>(p, idx);
-            const bool in_step = it.two && !it.pair;   // both warpgroups use a key tile
-            auto k_seq = [&](int tile) { return seq + C::UNITS * (uint32_t)(in_step ? 2 * tile : tile == 0 ? 0 : 2 * tile - 1); };
-            auto v_seq = [&](int tile) { return seq + C::UNITS * (uint32_t)(in_step ? 2 * tile + 1 : tile == it.tiles - 1 ? 2 * tile + 1 : 2 * tile + 2); };
-            for (int t = 0; t < it.steps + 2 && ok; ++t) {
-                const int x = t & 1;
-                if (t >= 2) {   // O += P V of step t - 2
-                    const int tp = t - 2, tile = in_step ? tp >> 1 : tp;
-                    ok = mbar_wait_warp(&p_full[bar_of(it.two, tp)], ((x ? (it.two ? odd : alone) : even) + (uint32_t)(tp >> 1)) & 1u, &err, DEV_ERR_WAIT_FULL);
-                    const uint32_t acc = it.two ? (uint32_t)x : 0u;
-                    const bool fresh = tp < (it.two ? 2 : 1), frees = !in_step || x == 1;
-                    for (int u = 0; u < C::UNITS && ok; ++u) {
-                        const uint32_t q = v_seq(tile) + u, slot = q % C::SLOTS;
-                        ok = mbar_wait_warp(&full[slot], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_FULL);
-                        if (!ok) break;
-                        fence_after_sync();
-                        if (elect_one()) {
-                            const uint32_t v_a = ring_a + slot * C::SLOT;
+        constexpr uint32_t ID_S = instr_desc(BA_KEYS) | FMT, ID_O = instr_desc(C::UNIT) | FMT | (1u << 16);   // V lies key by key: N-major
+        constexpr int LAG = C::BUFS;
+        // One thread does it all, and it waits for keys and values ahead of the weights: what stands between a warpgroup's last weights and its next scores
+        // is one wait and the issue of the two products.  (A warp with a vote in each of five waits a step and stream took 900 clocks more than the products.)
+        if (elect_one()) {
+            const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(smem);
+            uint32_t uses[2] = {0, 0}, q_uses[2] = {0, 0}, seq = 0;   // of the score buffers, of the row tiles, of the ring
+            bool ok = true;
+            for (uint32_t idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
+                const Item it = item_of<D>(p, idx);
+                const int steps[2] = {steps_of(it, 0), C::SPLIT ? 0 : steps_of(it, 1)};
+                const bool shared = it.two && !it.pair;   // both streams use a key tile
+                // places of a tile's slots in the ring's sequence, in the order of use
+                auto k_seq = [&](int tile) {
+                    if (C::SPLIT) return seq + C::UNITS * (uint32_t)(tile == 0 ? 0 : 2 * tile - 1);   // K0 K1 V0 K2 V1 ...
+                    return seq + (uint32_t)(it.pair ? 2 * tile - (tile & 1) : 2 * tile);              // K0 K1 V0 V1 K2 K3 ... a tile a stream, K0 V0 K1 V1 ... otherwise
+                };
+                auto v_seq = [&](int tile) {
+                    if (C::SPLIT) return seq + C::UNITS * (uint32_t)(tile == it.tiles - 1 ? 2 * tile + 1 : 2 * tile + 2);
+                    return seq + (uint32_t)(it.pair ? 2 * tile + 1 + ((tile & 1) == 0 && tile < it.tiles - 1 ? 1 : 0) : 2 * tile + 1);
+                };
+                auto landed = [&](uint32_t q) { ok = ok && mbar_wait_one(&full[q % C::SLOTS], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_FULL); };
+                for (int u = 0; u < steps[0] + LAG && ok; ++u) {   // (the second stream never has more steps)
 #pragma unroll
-                            for (int j = 0; j < BA_KEYS / 16; ++j)
-                                mma_ts_rt(tmem + C::TM_O + acc * D + u * C::UNIT, tmem + C::TM_S + 128u * (uint32_t)x + 8u * j, swizzled_desc(v_a + 2048u * j, BA_BOX), ID_O,
-                                          fresh && j == 0 ? 0u : 1u);
-                            if (frees) mma_commit(&empty[slot]);
-                            if (u == C::UNITS - 1) mma_commit(&pv_done[bar_of(it.two, t)]);
+                    for (int x = 0; x < C::TILES; ++x) {
+                        const bool has_pv = u >= LAG && u - LAG < steps[x], has_s = u < steps[x];
+                        const int v = u - LAG, v_tile = it.pair ? 2 * v + x : v, v_buf = C::SPLIT ? v & 1 : x, s_tile = it.pair ? 2 * u + x : u, s_buf = C::SPLIT ? u & 1 : x;
+                        const uint32_t vq = has_pv ? v_seq(v_tile) : 0, kq = has_s ? k_seq(s_tile) : 0;
+                        const bool frees = !shared || x == 1;
+                        if (!C::SPLIT) {   // (units of a wide tile arrive one by one)
+                            if (has_pv) landed(vq);
+                            if (has_s) landed(kq);
                         }
-                        __syncwarp();
-                    }
-                    if (!ok) break;
-                }
-                if (t < it.steps) {   // S = Q K^T
-                    const int tile = in_step ? t >> 1 : t, rt = it.two ? x : 0;
-                    if (t < (it.two ? 2 : 1)) {
-                        ok = mbar_wait_warp(&q_full[rt], q_uses[rt] & 1u, &err, DEV_ERR_WAIT_FULL);
-                        ++q_uses[rt];
-                        if (!ok) break;
-                    }
-                    const bool frees = !in_step || x == 1;
-                    for (int u = 0; u < C::UNITS && ok; ++u) {
-                        const uint32_t q = k_seq(tile) + u, slot = q % C::SLOTS;
-                        ok = mbar_wait_warp(&full[slot], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_FULL);
-                        if (!ok) break;
-                        fence_after_sync();
-                        if (elect_one()) {
-                            const uint32_t k_a = ring_a + slot * C::SLOT, a = q_a + rt * C::Q_BYTES + u * (C::UNIT / 64) * BA_BOX;
+                        if (has_s && u == 0) ok = ok && mbar_wait_one(&q_full[x], q_uses[x]++ & 1u, &err, DEV_ERR_WAIT_FULL);
+                        if (has_pv) {   // O += P V of step u - LAG
+                            const uint32_t use = C::SPLIT ? uses[v & 1] + (uint32_t)(v >> 1) : uses[x] + (uint32_t)v;
+                            const uint32_t p_a = tmem + C::TM_S + 128u * v_buf, tm_o = tmem + C::TM_O + x * D;
 #pragma unroll
-                            for (int j = 0; j < C::UNIT / 16; ++j) {
-                                const uint32_t at = (uint32_t)(j >> 2) * BA_BOX + (uint32_t)(j & 3) * 32u;
-                                mma_ss(tmem + C::TM_S + 128u * (uint32_t)x, swizzled_desc(a + at, 16), swizzled_desc(k_a + at, 16), ID_S, u > 0 || j > 0 ? 1u : 0u);
+                            for (int half = 0; half < (C::SPLIT ? 1 : 2); ++half) {   // of the keys
+                                ok = ok && mbar_wait_one(&p_full[C::SPLIT ? v_buf : 2 * x + half], use & 1u, &err, DEV_ERR_WAIT_FULL);
+#pragma unroll
+                                for (int w = 0; w < C::UNITS; ++w) {
+                                    const uint32_t slot = (vq + w) % C::SLOTS;
+                                    if (C::SPLIT) landed(vq + w);
+                                    if (!ok) break;
+                                    fence_after_sync();
+                                    const uint64_t v_d = swizzled_desc(ring_a + slot * C::SLOT, BA_BOX);
+#pragma unroll
+                                    for (int i = 0; i < (C::SPLIT ? 8 : 4); ++i) {   // 16 keys each: 8 columns of P; (SPLIT) the second warpgroup's 64 columns on
+                                        const int j = half * 4 + i;
+                                        mma_ts_rt(tm_o + w * C::UNIT, p_a + (C::SPLIT ? (j >> 2) * 64u + (j & 3) * 8u : j * 8u), v_d + 128u * j, ID_O, v == 0 && j == 0 ? 0u : 1u);
+                                    }
+                                    if (C::SPLIT || half == 1) {
+                                        if (frees) mma_commit(&empty[slot]);
+                                        if (w == C::UNITS - 1 && (C::SPLIT || v == steps[x] - 1)) mma_commit(&pv_done[v_buf]);
+                                    }
+                                }
                             }
-                            if (frees) mma_commit(&empty[slot]);
-                            if (u == C::UNITS - 1) mma_commit(&s_full[bar_of(it.two, t)]);
                         }
-                        __syncwarp();
+                        if (has_s) {   // S = Q K^T
+#pragma unroll
+                            for (int w = 0; w < C::UNITS; ++w) {
+                                const uint32_t slot = (kq + w) % C::SLOTS;
+                                if (C::SPLIT) landed(kq + w);
+                                if (!ok) break;
+                                if (C::SPLIT || !has_pv) fence_after_sync();
+                                const uint64_t k_d = swizzled_desc(ring_a + slot * C::SLOT, 16), a_d = swizzled_desc(q_a + x * C::Q_BYTES + w * (C::UNIT / 64) * BA_BOX, 16);
+#pragma unroll
+                                for (int j = 0; j < C::UNIT / 16; ++j) {
+                                    const uint64_t at = (uint32_t)((j >> 2) * BA_BOX + (j & 3) * 32) >> 4;
+                                    mma_ss(tmem + C::TM_S + 128u * s_buf, a_d + at, k_d + at, ID_S, w > 0 || j > 0 ? 1u : 0u);
+                                }
+                                if (w == C::UNITS - 1) mma_commit(&s_full[s_buf]);
+                                if (frees) mma_commit(&empty[slot]);
+                            }
+                        }
                     }
                 }
+                uses[0] += (uint32_t)(C::SPLIT ? (steps[0] + 1) / 2 : steps[0]);
+                uses[1] += (uint32_t)(C::SPLIT ? steps[0] / 2 : steps[1]);
+                seq += 2u * C::UNITS * (uint32_t)it.tiles;
             }
-            even += (uint32_t)(it.steps + 1) / 2;
-            (it.two ? odd : alone) += (uint32_t)it.steps / 2;
-            seq += 2u * C::UNITS * (uint32_t)it.tiles;
         }
+        __syncwarp();
     } else if (warp == 9) {
         // ================= producer =================
         uint32_t seq = 0, tails = 0;
         bool ok = true;
         for (uint32_t idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
             const Item it = item_of<D>(p, idx);
-            const bool in_step = it.two && !it.pair;
             const int n_p = it.p1 - it.p0;
             auto load = [&](int tile, bool is_v) {
                 const bool pre = tile < n_p;
@@ -517,16 +632,18 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                     }
                 }
             };
-            if (in_step) {
-                for (int i = 0; i < it.tiles && ok; ++i) {
+            const int ahead = C::SPLIT ? 1 : 0;   // how many tiles the keys are ahead of the values
+            if (it.pair) {
+                for (int i = 0; i < it.tiles && ok; i += 2) {
                     load(i, false);
-                    load(i, true);
-                }
-            } else if (it.tiles > 0) {
-                load(0, false);
-                for (int i = 0; i < it.tiles && ok; ++i) {
                     if (i + 1 < it.tiles) load(i + 1, false);
                     load(i, true);
+                    if (i + 1 < it.tiles) load(i + 1, true);
+                }
+            } else {
+                for (int i = 0; i < it.tiles + ahead && ok; ++i) {
+                    if (i < it.tiles) load(i, false);
+                    if (i >= ahead) load(i - ahead, true);
                 }
             }
         }
@@ -534,6 +651,7 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         for (uint32_t q = seq > (uint32_t)C::SLOTS ? seq - C::SLOTS : 0; q < seq; ++q)
             mbar_wait_warp(&full[q % C::SLOTS], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_DRAIN);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     fence_before_sync();
     __syncthreads();
     if (warp == 8) {
