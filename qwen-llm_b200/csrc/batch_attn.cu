@@ -115,10 +115,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// 128-byte swizzle, 8-row groups 1024 bytes apart.  K-major: `lbo` unused.  MN-major: `lbo` bytes between blocks of 64 along MN.
-__device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr, uint32_t lbo) {
-    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
                  "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
@@ -310,10 +306,6 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                 ok = mbar_wait_warp_inline(&s_full[buf(u)], parity(u), &err, DEV_ERR_WAIT_FULL);
                 if (!ok) break;
                 fence_after_sync();
-                if (u == steps - 1 && idx_next < p.items) {   // nothing reads Q any more: the next item's is on its way from here on
-                    const Item next = item_of<D>(p, idx_next);
-                    if (steps_of(next, stream) > 0) fetch_q(next, row_ref(p, next, next.pair ? 0 : stream, row));
-                }
                 constexpr int N = C::S_COLS;
                 const uint32_t tm_s = tm_lane + C::TM_S + 128u * buf(u) + (C::SPLIT ? 64u * wg : 0u);
                 auto hand_over = [&](int half) {   // of P, to the issuer
@@ -416,7 +408,14 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                     for (int j = 0; j < N; j += 64) hand_over(j / 64);
                 }
             }
-            // the last products of the accumulator
+            // nothing reads Q any more: the next item's is on its way while the last products are waited for
+            Item it_next;
+            RowRef rr_next;
+            if (idx_next < p.items) {
+                it_next = item_of<D>(p, idx_next);
+                rr_next = row_ref(p, it_next, it_next.pair ? 0 : stream, row);
+                if (ok && steps_of(it_next, stream) > 0) fetch_q(it_next, rr_next);
+            }
             if (steps > 0 && ok) {
                 ok = mbar_wait_warp_inline(&pv_done[buf(steps - 1)], C::SPLIT ? parity(steps - 1) : done++ & 1u, &err, DEV_ERR_WAIT_DRAIN);
                 fence_after_sync();
@@ -494,9 +493,8 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
             }
             if (idx_next >= p.items) break;
             idx = idx_next;
-            it = item_of<D>(p, idx);
-            rr = row_ref(p, it, it.pair ? 0 : stream, row);
-            if (steps == 0 && steps_of(it, stream) > 0) fetch_q(it, rr);   // it was not fetched on the way
+            it = it_next;
+            rr = rr_next;
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BA_REGS_REST));
@@ -512,34 +510,40 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         // is one wait and the issue of the two products.  (A warp with a vote in each of five waits a step and stream took 900 clocks more than the products.)
         if (elect_one()) {
             const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(smem);
+            constexpr uint64_t SW = (1ull << 46) | (2ull << 61) | ((uint64_t)(1024 >> 4) << 32);   // 128-byte swizzle, 8-row groups 1024 bytes apart
+            constexpr uint64_t K_DESC = SW | 1ull << 16, V_DESC = SW | (uint64_t)(BA_BOX >> 4) << 16;   // K-major; N-major, 64 dimensions a box
             uint32_t uses[2] = {0, 0}, q_uses[2] = {0, 0}, seq = 0;   // of the score buffers, of the row tiles, of the ring
             bool ok = true;
             for (uint32_t idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
                 const Item it = item_of<D>(p, idx);
                 const int steps[2] = {steps_of(it, 0), C::SPLIT ? 0 : steps_of(it, 1)};
                 const bool shared = it.two && !it.pair;   // both streams use a key tile
-                // places of a tile's slots in the ring's sequence, in the order of use
-                auto k_seq = [&](int tile) {
-                    if (C::SPLIT) return seq + C::UNITS * (uint32_t)(tile == 0 ? 0 : 2 * tile - 1);   // K0 K1 V0 K2 V1 ...
-                    return seq + (uint32_t)(it.pair ? 2 * tile - (tile & 1) : 2 * tile);              // K0 K1 V0 V1 K2 K3 ... a tile a stream, K0 V0 K1 V1 ... otherwise
-                };
-                auto v_seq = [&](int tile) {
-                    if (C::SPLIT) return seq + C::UNITS * (uint32_t)(tile == it.tiles - 1 ? 2 * tile + 1 : 2 * tile + 2);
-                    return seq + (uint32_t)(it.pair ? 2 * tile + 1 + ((tile & 1) == 0 && tile < it.tiles - 1 ? 1 : 0) : 2 * tile + 1);
-                };
+                // Places of K and V in the ring's sequence, in the order of use: K0 V0 K1 V1 ...; with a tile a stream K0 K1 V0 V1 K2 K3 V2 V3 ... and K V of one that
+                // is left; with two buffers K0 K1 V0 K2 V1 ....
+                uint32_t kq[2], vq[2];
+                const uint32_t hop = it.pair ? 4u : 2u * C::UNITS;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    kq[x] = seq + (it.pair ? x : 0);
+                    vq[x] = C::SPLIT ? seq + 2 * C::UNITS : it.pair ? seq + 2 + x : seq + 1;
+                }
                 auto landed = [&](uint32_t q) { ok = ok && mbar_wait_one(&full[q % C::SLOTS], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_FULL); };
                 for (int u = 0; u < steps[0] + LAG && ok; ++u) {   // (the second stream never has more steps)
 #pragma unroll
                     for (int x = 0; x < C::TILES; ++x) {
-                        const bool has_pv = u >= LAG && u - LAG < steps[x], has_s = u < steps[x];
-                        const int v = u - LAG, v_tile = it.pair ? 2 * v + x : v, v_buf = C::SPLIT ? v & 1 : x, s_tile = it.pair ? 2 * u + x : u, s_buf = C::SPLIT ? u & 1 : x;
-                        const uint32_t vq = has_pv ? v_seq(v_tile) : 0, kq = has_s ? k_seq(s_tile) : 0;
+                        const int v = u - LAG;
+                        const bool has_pv = v >= 0 && v < steps[x], has_s = u < steps[x];
+                        const uint32_t v_buf = C::SPLIT ? v & 1 : x, s_buf = C::SPLIT ? u & 1 : x;
                         const bool frees = !shared || x == 1;
+                        const uint32_t k_at = kq[x];
+                        uint32_t v_at = vq[x];
+                        // the last tile's V comes right behind its K where it has no successor or partner
+                        if (C::SPLIT ? v == steps[0] - 1 : it.pair && x == 0 && v == steps[0] - 1 && (it.tiles & 1)) v_at -= C::UNITS;
                         if (!C::SPLIT) {   // (units of a wide tile arrive one by one)
-                            if (has_pv) landed(vq);
-                            if (has_s) landed(kq);
+                            if (has_pv) landed(v_at);
+                            if (has_s) landed(k_at);
                         }
-                        if (has_s && u == 0) ok = ok && mbar_wait_one(&q_full[x], q_uses[x]++ & 1u, &err, DEV_ERR_WAIT_FULL);
+                        if (u == 0 && has_s) ok = ok && mbar_wait_one(&q_full[x], q_uses[x]++ & 1u, &err, DEV_ERR_WAIT_FULL);
                         if (has_pv) {   // O += P V of step u - LAG
                             const uint32_t use = C::SPLIT ? uses[v & 1] + (uint32_t)(v >> 1) : uses[x] + (uint32_t)v;
                             const uint32_t p_a = tmem + C::TM_S + 128u * v_buf, tm_o = tmem + C::TM_O + x * D;
@@ -548,15 +552,15 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                                 ok = ok && mbar_wait_one(&p_full[C::SPLIT ? v_buf : 2 * x + half], use & 1u, &err, DEV_ERR_WAIT_FULL);
 #pragma unroll
                                 for (int w = 0; w < C::UNITS; ++w) {
-                                    const uint32_t slot = (vq + w) % C::SLOTS;
-                                    if (C::SPLIT) landed(vq + w);
+                                    const uint32_t slot = (v_at + w) % C::SLOTS;
+                                    if (C::SPLIT) landed(v_at + w);
                                     if (!ok) break;
                                     fence_after_sync();
-                                    const uint64_t v_d = swizzled_desc(ring_a + slot * C::SLOT, BA_BOX);
+                                    const uint32_t v_lo = (ring_a + slot * C::SLOT) >> 4;
 #pragma unroll
                                     for (int i = 0; i < (C::SPLIT ? 8 : 4); ++i) {   // 16 keys each: 8 columns of P; (SPLIT) the second warpgroup's 64 columns on
-                                        const int j = half * 4 + i;
-                                        mma_ts_rt(tm_o + w * C::UNIT, p_a + (C::SPLIT ? (j >> 2) * 64u + (j & 3) * 8u : j * 8u), v_d + 128u * j, ID_O, v == 0 && j == 0 ? 0u : 1u);
+                                        const uint32_t j = half * 4 + i;
+                                        mma_ts_rt(tm_o + w * C::UNIT, p_a + (C::SPLIT ? (j >> 2) * 64u + (j & 3) * 8u : j * 8u), V_DESC | (v_lo + 128u * j), ID_O, v == 0 && j == 0 ? 0u : 1u);
                                     }
                                     if (C::SPLIT || half == 1) {
                                         if (frees) mma_commit(&empty[slot]);
@@ -564,23 +568,25 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                                     }
                                 }
                             }
+                            vq[x] += hop;
                         }
                         if (has_s) {   // S = Q K^T
 #pragma unroll
                             for (int w = 0; w < C::UNITS; ++w) {
-                                const uint32_t slot = (kq + w) % C::SLOTS;
-                                if (C::SPLIT) landed(kq + w);
+                                const uint32_t slot = (k_at + w) % C::SLOTS;
+                                if (C::SPLIT) landed(k_at + w);
                                 if (!ok) break;
                                 if (C::SPLIT || !has_pv) fence_after_sync();
-                                const uint64_t k_d = swizzled_desc(ring_a + slot * C::SLOT, 16), a_d = swizzled_desc(q_a + x * C::Q_BYTES + w * (C::UNIT / 64) * BA_BOX, 16);
+                                const uint32_t k_lo = (ring_a + slot * C::SLOT) >> 4, a_lo = (q_a + x * C::Q_BYTES + w * (C::UNIT / 64) * BA_BOX) >> 4;
 #pragma unroll
                                 for (int j = 0; j < C::UNIT / 16; ++j) {
-                                    const uint64_t at = (uint32_t)((j >> 2) * BA_BOX + (j & 3) * 32) >> 4;
-                                    mma_ss(tmem + C::TM_S + 128u * s_buf, a_d + at, k_d + at, ID_S, w > 0 || j > 0 ? 1u : 0u);
+                                    const uint32_t at = (uint32_t)((j >> 2) * BA_BOX + (j & 3) * 32) >> 4;
+                                    mma_ss(tmem + C::TM_S + 128u * s_buf, K_DESC | (a_lo + at), K_DESC | (k_lo + at), ID_S, w > 0 || j > 0 ? 1u : 0u);
                                 }
                                 if (w == C::UNITS - 1) mma_commit(&s_full[s_buf]);
                                 if (frees) mma_commit(&empty[slot]);
                             }
+                            kq[x] += C::SPLIT && u == 0 ? C::UNITS : hop;
                         }
                     }
                 }
@@ -685,24 +691,47 @@ __global__ void __launch_bounds__(256) batch_attn_join_kernel(const __grid_const
     float top = -INFINITY;
     for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[i * step + at].x);
     top = warp_max(top);
+    // a lane's E columns of every part, four parts' loads at a time: the parts with mass first, so that the others cost nothing
     float l = 0.f, o[E] = {};
     for (uint32_t i0 = 0; i0 < n; i0 += 32) {
         float w = 0.f, li = 0.f;
         if (i0 + lane < n) {
             const float2 ml = p.part_ml[(i0 + lane) * step + at];
-            w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : ex2((ml.x - top) * c);   // a NaN sum without a maximum: the item gave up
-            li = w * ml.y;
-            if (ml.x == -INFINITY) li = ml.y;
+            w = ml.x == -INFINITY ? 0.f : ex2((ml.x - top) * c);
+            li = ml.x == -INFINITY ? ml.y : w * ml.y;   // a NaN sum without a maximum: the item gave up
         }
         l += warp_sum(li);
-        const unsigned some = __ballot_sync(0xffffffffu, w != 0.f);
-        for (unsigned left = some; left; left &= left - 1) {
-            const int i = __ffs(left) - 1;
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            if (!(wi == wi)) continue;
-            const float* src = p.part_o + ((i0 + i) * step + at) * D + lane * E;
+        unsigned left = __ballot_sync(0xffffffffu, w > 0.f);
+        while (left) {
+            float f[4];
+            float4 x[4][E / 4 ? E / 4 : 1];
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] += wi * src[e];
+            for (int k = 0; k < 4; ++k) {
+                const int i = left ? __ffs(left) - 1 : 0;
+                f[k] = left ? __shfl_sync(0xffffffffu, w, i) : 0.f;
+                if (left) {
+                    const float* src = p.part_o + ((i0 + i) * step + at) * D + lane * E;
+                    if (E >= 4) {
+#pragma unroll
+                        for (int e = 0; e < E / 4; ++e) x[k][e] = __ldcs(reinterpret_cast<const float4*>(src) + e);
+                    } else {
+                        const float2 y = __ldcs(reinterpret_cast<const float2*>(src));
+                        x[k][0] = make_float4(y.x, y.y, 0.f, 0.f);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < (E / 4 ? E / 4 : 1); ++e) x[k][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                left &= left - 1;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float4 y = x[k][e / 4];
+                    o[e] += f[k] * (e % 4 == 0 ? y.x : e % 4 == 1 ? y.y : e % 4 == 2 ? y.z : y.w);
+                }
+            }
         }
     }
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
@@ -751,8 +780,8 @@ dfl_status check(const dfl_prefix_attention_args* a, BatchAttnParams* p) {
     return DFL_OK;
 }
 
-// How the work is cut.  Times in microseconds, measured on B200: a key tile against two row tiles 1.2, against one 0.6 (head width 128), an item's
-// start and end 4, a byte of a part written and read again 1 / 4e6.
+// How the work is cut.  Times in microseconds, measured on B200: a key tile against two row tiles 1.9, against one 0.95 (head width 128), an item's
+// start and end 5, a byte of a part written and read again 1 / 4e6.
 uint32_t ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 void plan(const dfl_prefix_attention_args* a, BatchAttnParams* p, int sms) {
@@ -760,7 +789,7 @@ void plan(const dfl_prefix_attention_args* a, BatchAttnParams* p, int sms) {
     p->rows = p->batch * per;
     p->prefix_tiles = ceil_div((uint64_t)p->prefix, BA_KEYS);
     const uint32_t own_tiles = ceil_div((uint64_t)p->cap, BA_KEYS);
-    const double tile1 = 0.6 * D / 128.0, start = 4.0, part_us = 8.0 * D / 4e6;
+    const double tile1 = 0.95 * D / 128.0, start = 5.0, part_us = 8.0 * D / 4e6;
     // requests that fill their row blocks to four fifths take prefix and own keys in one go
     const uint32_t o_block = D <= 128 && per <= BA_ROWS ? BA_ROWS : block;
     const uint32_t o_blocks = ceil_div(per, o_block);
