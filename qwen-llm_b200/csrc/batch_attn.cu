@@ -254,6 +254,8 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
     pdl_prologue();
+    // The roles are the arms of one chain and each sets its registers itself.  (With the issue and the producer in a second chain behind the softmax arm, width
+    // 256 took 74 us where it takes 64: 30 requests of 8 tokens, 16 heads over 2 KV heads, prefix of 12 001 keys.)
     if (warp < 8) {
         // ================= softmax: thread = row =================
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BA_REGS_SOFTMAX));
@@ -496,10 +498,8 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
             it = it_next;
             rr = rr_next;
         }
-    } else {
+    } else if (warp == 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BA_REGS_REST));
-    }
-    if (warp == 8) {
         // ================= MMA issue =================
         // One warp for both streams: PV and S of a stream one behind the other, then the other's.  (With a warp each the streams' products went through the
         // pipe interleaved, their scores came at the same time and so did their exponentials: 4650 clocks a tile of 2 x 128 rows.)
@@ -597,6 +597,7 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         }
         __syncwarp();
     } else if (warp == 9) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BA_REGS_REST));
         // ================= producer =================
         uint32_t seq = 0, tails = 0;
         bool ok = true;
@@ -656,6 +657,8 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         // nothing may still be in flight into this CTA's shared memory when it leaves
         for (uint32_t q = seq > (uint32_t)C::SLOTS ? seq - C::SLOTS : 0; q < seq; ++q)
             mbar_wait_warp(&full[q % C::SLOTS], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_DRAIN);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BA_REGS_REST));
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     fence_before_sync();
