@@ -339,8 +339,10 @@ cudaError_t launch_quads(const RopeParams& p, dim3 grid, cudaStream_t st) {
 template <typename S, typename D>
 cudaError_t launch_typed(RopeParams& p, cudaStream_t st) {
     const bool quads = in_quads<S, D>(p);
-    // a token's heads are shared out over warps until the machine has eight warps an SM, but a warp keeps a load for each of its lane groups
-    const uint64_t wanted = (uint64_t)sm_count() * 8, parts = (wanted + p.n_tokens - 1) / p.n_tokens;
+    // A token's heads are shared out over as many warps as are resident at once (24 an SM), but a warp keeps a load for each of its lane groups.  One
+    // share more would leave a second round for a few: 100, 300, 768, 1500 tokens of 32 + 8 + 8 heads of 128 take 4.3, 5.8, 8.0, 10.5 us, with the
+    // shares rounded up 4.3, 7.7, 10.2, 14.6, and with eight warps an SM 4.9, 7.0, 10.1, 14.2.
+    const uint64_t parts = (uint64_t)sm_count() * 24 / p.n_tokens > 1 ? (uint64_t)sm_count() * 24 / p.n_tokens : 1;
     const uint32_t groups = quads ? 256 / p.dim : 1, most_parts = (p.n_q + groups - 1) / groups + (p.n_heads - p.n_q + groups - 1) / groups;
     p.parts = (uint32_t)(parts < most_parts ? parts : most_parts);
     const uint64_t items = (uint64_t)p.n_tokens * p.parts, blocks = (items + ROPE_WARPS - 1) / ROPE_WARPS, most = (uint64_t)sm_count() * 3;
