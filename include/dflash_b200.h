@@ -211,10 +211,11 @@ dfl_status dfl_argmax_top2_static(int32_t device, const float* logits_dev, int32
  * buffers.  All three work like dfl_argmax_top2_static: they make `device` the calling thread's current device
  * and leave it so, check their arguments, enqueue on `stream` (a cudaStream_t, NULL = the default stream) and
  * return without waiting; they allocate nothing, keep nothing between calls and may be captured into a graph.
- * Strides are in elements and not negative; the innermost dimension is contiguous; a stride of a dimension with
- * one entry (or none) is not read.  A workspace belongs to the call from its enqueueing until the stream has
- * passed it: calls that can overlap, and graphs that can be replayed at once, need one each.  Inputs of a call
- * do not overlap its outputs except where that is said. */
+ * Strides are in elements and not negative (an output's elements lie apart); the innermost dimension is
+ * contiguous; a stride of a dimension with one entry (or none) is not read; addresses are aligned to their type
+ * at least.  A workspace belongs to the call from its enqueueing until the stream has passed it: calls that can
+ * overlap, and graphs that can be replayed at once, need one each.  Inputs of a call do not overlap its outputs
+ * except where that is said. */
 
 /* Per-head RMS norm of queries and keys, rotation by position, and the store of K and V rows, in one pass:
  *   y = x * rsqrt(mean(x^2) + eps) * weight            (weight f32 [head_dim]; NULL = ones)
@@ -267,7 +268,8 @@ dfl_status dfl_qk_norm_rope(int32_t device, const dfl_qk_norm_rope_args* args, v
  * dtype: DFL_F16 or DFL_BF16 for all tensors; head_dim 64, 128 or 256; n_q_heads a multiple of n_kv_heads, at
  * most 64 query heads a KV head; prefix_len and own_capacity below 2^30; addresses and strides multiples of 16
  * bytes.  own_len may be NULL when own_capacity is 0.  Scores, softmax and sums in f32; the weights of a tile
- * are rounded to dtype for the product with V, as is the result.  batch, n_tokens 0: enqueues nothing. */
+ * are rounded to dtype for the product with V, as is the result.  Every wait on the device is bounded; should one
+ * run out, the output rows it concerns are NaN.  batch, n_tokens 0: enqueues nothing. */
 typedef struct dfl_prefix_attention_args {
     int32_t dtype;
     uint32_t batch, n_tokens, n_q_heads, n_kv_heads, head_dim;
@@ -302,8 +304,8 @@ dfl_status dfl_prefix_attention(int32_t device, const dfl_prefix_attention_args*
  * is drawn: from the residual max(p - q, 0) of the first refused draft (from p itself should that be empty),
  * or from p of the last row when all stand - the lowest token whose cumulated mass exceeds u_sample[b] times
  * the whole.  n_accepted_out[b] = drafts that stand; tokens_out[b] = those drafts, the drawn token, then -1.
- * Where a row that the decision reads is no distribution (a NaN or +inf logit, all -inf, a negative or NaN
- * temperature), n_accepted_out[b] = -1 - row and every token is -1.  A draft outside [0, vocab) does not stand.
+ * Where a row that the decision reads is no distribution (a NaN or +inf logit, all -inf, a negative, infinite or
+ * NaN temperature), n_accepted_out[b] = -1 - row and every token is -1.  A draft outside [0, vocab) does not stand.
  * u in [0, 1); draft_probs finite and not negative.  The sums that draw a token are in 64 bits, so the token is
  * the one that the definition gives.  n_drafts 0..DFL_MAX_VERIFY_DRAFTS, 1 <= vocab < 2^31; dtype of the logits: DFL_F32,
  * DFL_F16 or DFL_BF16. */

@@ -102,6 +102,19 @@ def _dense(x, name, shape, like, dtype):
     return x.data_ptr()
 
 
+def _output(x, name, shape, like, dtype=None):
+    _need(x, name, shape, like, dtype)
+    if any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
+        raise ValueError(f"{name}: an expanded dimension cannot be written")
+    return x
+
+
+def _no_grad(torch, *tensors):
+    """The operators have no backward pass: a result that autograd would take for a constant is refused."""
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
+        raise RuntimeError("no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
 @contextlib.contextmanager
 def _elsewhere(torch, x, stream):
     with torch.cuda.device(x.device):
@@ -151,12 +164,13 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
             raise ValueError("k_rows: needs k_out (and v_out)")
     if v is not None:
         _need(v, "v", (T, hk, D), q, q.dtype)
+    _no_grad(torch, q, k, v, q_weight, k_weight)
     with _on(torch, q, stream) as handle:
-        q_out = torch.empty((T, hq, D), dtype=q.dtype, device=q.device) if q_out is None else _need(q_out, "q_out", (T, hq, D), q)
-        k_out = torch.empty((T, hk, D), dtype=q_out.dtype, device=q.device) if k_out is None else _need(k_out, "k_out", (None, hk, D), q, q_out.dtype)
+        q_out = torch.empty((T, hq, D), dtype=q.dtype, device=q.device) if q_out is None else _output(q_out, "q_out", (T, hq, D), q)
+        k_out = torch.empty((T, hk, D), dtype=q_out.dtype, device=q.device) if k_out is None else _output(k_out, "k_out", (None, hk, D), q, q_out.dtype)
         v_in, v_s, vo, vo_s = 0, (0, 0), 0, (0, 0)
         if v is not None:
-            v_out = torch.empty((T, hk, D), dtype=q_out.dtype, device=q.device) if v_out is None else _need(v_out, "v_out", (k_out.shape[0], hk, D), q, q_out.dtype)
+            v_out = torch.empty((T, hk, D), dtype=q_out.dtype, device=q.device) if v_out is None else _output(v_out, "v_out", (k_out.shape[0], hk, D), q, q_out.dtype)
             v_in, v_s, vo, vo_s = v.data_ptr(), v.stride(), v_out.data_ptr(), v_out.stride()
         q_s, k_s, qo_s, ko_s = q.stride(), k.stride(), q_out.stride(), k_out.stride()
         a = _ROPE.pack(_dtype(dtypes, q, "q"), _dtype(dtypes, q_out, "q_out"), T, hq, hk, D, rotary_dim, axes, *sections, *(0,) * (MAX_ROPE_AXES - axes),
@@ -189,10 +203,11 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
         lens = _dense(own_len, "own_len", (B,), q, torch.int32)
         ok, ok_s, ov, ov_s = own_k.data_ptr(), own_k.stride(), own_v.data_ptr(), own_v.stride()
     q_lens = 0 if q_len is None else _dense(q_len, "q_len", (B,), q, torch.int32)
+    _no_grad(torch, q, prefix_k, prefix_v, own_k, own_v)
     with _on(torch, q, stream) as handle:
         if out is None:
             out = (torch.empty if q_len is None else torch.zeros)((B, n, hq, D), dtype=q.dtype, device=q.device)
-        _need(out, "out", (B, n, hq, D), q, q.dtype)
+        _output(out, "out", (B, n, hq, D), q, q.dtype)
         q_s, pk_s, pv_s, o_s = q.stride(), prefix_k.stride(), prefix_v.stride(), out.stride()
         fields = (_dtype(dtypes, q, "q"), B, n, hq, hk, D, D ** -0.5 if scale is None else scale, 0, P, cap, q.data_ptr(), q_s[0], q_s[1], q_s[2],
                   prefix_k.data_ptr(), prefix_v.data_ptr(), pk_s[0], pk_s[1], pv_s[0], pv_s[1], ok, ov, ok_s[0], ok_s[1], ok_s[2], ov_s[0], ov_s[1], ov_s[2],
@@ -226,6 +241,7 @@ def verify_drafts(logits, drafts, u_accept, u_sample, *, draft_probs=None, n_dra
         probs, p_s = draft_probs.data_ptr(), draft_probs.stride()
     nd = 0 if n_draft is None else _dense(n_draft, "n_draft", (B,), logits, torch.int32)
     temp = 0 if temperature is None else _dense(temperature, "temperature", (B,), logits, torch.float32)
+    _no_grad(torch, logits, draft_probs)
     with _on(torch, logits, stream) as handle:
         n_accepted = torch.empty(B, dtype=torch.int32, device=logits.device)
         tokens = torch.empty((B, R), dtype=torch.int32, device=logits.device)

@@ -771,6 +771,8 @@ dfl_status check(const dfl_prefix_attention_args* a, BatchAttnParams* p) {
     }
     for (const void* x : {a->q, (const void*)a->out, pre ? a->prefix_k : nullptr, pre ? a->prefix_v : nullptr, own ? a->own_k : nullptr, own ? a->own_v : nullptr})
         if (reinterpret_cast<uintptr_t>(x) % 16) return fail(DFL_ERR_BAD_ARG, "prefix_attention: addresses must be multiples of 16 bytes");
+    for (const void* x : {(const void*)a->own_len, (const void*)a->q_len})
+        if (reinterpret_cast<uintptr_t>(x) % 4) return fail(DFL_ERR_BAD_ARG, "prefix_attention: own_len and q_len must be aligned to their type");
     p->q = a->q, p->pk = a->prefix_k, p->pv = a->prefix_v, p->ok = a->own_k, p->ov = a->own_v, p->out = a->out;
     p->own_len = a->own_len, p->q_len = a->q_len;
     p->batch = a->batch, p->n = a->n_tokens, p->n_q = a->n_q_heads, p->n_kv = a->n_kv_heads, p->group = a->n_q_heads / a->n_kv_heads;
@@ -780,6 +782,7 @@ dfl_status check(const dfl_prefix_attention_args* a, BatchAttnParams* p) {
     if ((a->prefix_len > 1 && (!p->pk_r || !p->pv_r)) || (pre && heads && (!p->pk_h || !p->pv_h)) || (a->own_capacity > 1 && (!p->ok_r || !p->ov_r)) ||
         (own && heads && (!p->ok_h || !p->ov_h)) || (own && a->batch > 1 && (!p->ok_b || !p->ov_b)))
         return fail(DFL_ERR_BAD_SHAPE, "prefix_attention: a stride of K or V is zero");
+    if (work && ((a->batch > 1 && !p->o_b) || (a->n_tokens > 1 && !p->o_t) || (a->n_q_heads > 1 && !p->o_h))) return fail(DFL_ERR_BAD_SHAPE, "prefix_attention: a stride of out is zero");
     return DFL_OK;
 }
 

@@ -391,6 +391,11 @@ extern "C" dfl_status dfl_qk_norm_rope(int32_t device, const dfl_qk_norm_rope_ar
         if (half && !a->positions) return fail(DFL_ERR_BAD_ARG, "qk_norm_rope: positions are needed");
         if (a->n_kv_heads && !a->kv_rows && a->n_kv_out_rows < a->n_tokens) return fail(DFL_ERR_BAD_SHAPE, "qk_norm_rope: fewer output rows than tokens");
     }
+    const uintptr_t src = a->src_dtype == DFL_F32 ? 4 : 2, dst = a->dst_dtype == DFL_F32 ? 4 : 2;
+    auto off = [](const void* x, uintptr_t word) { return reinterpret_cast<uintptr_t>(x) % word != 0; };
+    if (off(a->q, src) || off(a->k, src) || off(a->v, src) || off(a->q_out, dst) || off(a->k_out, dst) || off(a->v_out, dst) || off(a->q_weight, 4) ||
+        off(a->k_weight, 4) || off(a->positions, 4) || off(a->kv_rows, 8))
+        return fail(DFL_ERR_BAD_ARG, "qk_norm_rope: an address is not aligned to its type");
     DFL_CHECK(use_device(device));
     RopeParams p = {};
     p.q = a->q, p.k = a->k, p.v = has_v ? a->v : nullptr, p.q_out = a->q_out, p.k_out = a->k_out, p.v_out = a->v_out;

@@ -380,10 +380,10 @@ template <typename T>
 __device__ __forceinline__ void load4(const T* row, uint32_t at, uint32_t end, bool vec, float* x) {
     if (vec && at + 4 <= end) {
         if (sizeof(T) == 4) {
-            const float4 w = __ldg(reinterpret_cast<const float4*>(row + at));
+            const float4 w = *reinterpret_cast<const float4*>(row + at);
             x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
         } else {
-            const uint2 w = __ldg(reinterpret_cast<const uint2*>(row + at));
+            const uint2 w = *reinterpret_cast<const uint2*>(row + at);
             float y[8];
             unpack_logits<T>(make_uint4(w.x, w.y, 0, 0), true, y);
             x[0] = y[0], x[1] = y[1], x[2] = y[2], x[3] = y[3];
@@ -512,7 +512,11 @@ __global__ void __launch_bounds__(DRAW_THREADS, 1) verify_draw_kernel(const __gr
             sum_up(R{}, 1);
             rest = whole > 0.0;            // nothing may be left of p beside q: then from p
         }
-        if (!rest) sum_up(W{}, 2);
+        for (int slot = 2; !rest; slot = 1) {
+            sum_up(W{}, slot);
+            if (whole > 0.0 || d < 0) break;
+            d = -1;                        // the refused draft had all the mass (u was not below one): from p too
+        }
         // inside [0, whole) even if u is not inside [0, 1)
         double target = fmax((double)u_sample * whole, 0.0);
         if (!(target < whole)) target = __longlong_as_double(__double_as_longlong(whole) - 1);
@@ -590,6 +594,11 @@ dfl_status check(const dfl_verify_drafts_args* a, bool pointers) {
     if (!pointers || a->batch == 0) return DFL_OK;
     if (!a->logits || !a->u_sample || !a->n_accepted_out || !a->tokens_out) return fail(DFL_ERR_BAD_ARG, "verify_drafts: null pointer");
     if (a->n_drafts && (!a->drafts || !a->u_accept)) return fail(DFL_ERR_BAD_ARG, "verify_drafts: drafts and u_accept are needed");
+    const uintptr_t word = a->dtype == DFL_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(a->logits) % word) return fail(DFL_ERR_BAD_ARG, "verify_drafts: the logits are not aligned to their type");
+    for (const void* x : {(const void*)a->draft_probs, (const void*)a->drafts, (const void*)a->n_draft, (const void*)a->temperature, (const void*)a->u_accept,
+                          (const void*)a->u_sample, (const void*)a->n_accepted_out, (const void*)a->tokens_out})
+        if (reinterpret_cast<uintptr_t>(x) % 4) return fail(DFL_ERR_BAD_ARG, "verify_drafts: an address is not aligned to its type");
     const bool many = a->batch > 1;
     if ((many && a->logits_batch_stride < 0) || (a->n_drafts && a->logits_row_stride < 0)) return fail(DFL_ERR_BAD_SHAPE, "verify_drafts: negative stride");
     if (a->draft_probs && ((many && a->probs_batch_stride < 0) || (a->n_drafts > 1 && a->probs_row_stride < 0)))

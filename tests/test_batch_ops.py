@@ -146,3 +146,28 @@ def test_wrappers_refuse_what_they_can_see():
         pkg.prefix_attention(q, q, q)
     with pytest.raises(ValueError, match="logits: shape"):
         pkg.verify_drafts(q[0], None, None, None)
+
+
+# addresses that their type does not allow, and K or V rows that lie one upon another
+MORE_REFUSED = [
+    (rope_args, "dfl_qk_norm_rope", dict(q=PTR + 2), "BAD_ARG"),
+    (rope_args, "dfl_qk_norm_rope", dict(k_out=PTR + 1), "BAD_ARG"),
+    (rope_args, "dfl_qk_norm_rope", dict(q_weight=PTR + 2), "BAD_ARG"),
+    (rope_args, "dfl_qk_norm_rope", dict(positions=PTR + 2), "BAD_ARG"),
+    (rope_args, "dfl_qk_norm_rope", dict(kv_rows=PTR + 4), "BAD_ARG"),
+    (attn_args, "dfl_prefix_attention", dict(own_len=PTR + 2), "BAD_ARG"),
+    (attn_args, "dfl_prefix_attention", dict(q_len=PTR + 1), "BAD_ARG"),
+    (attn_args, "dfl_prefix_attention", dict(own_k_batch_stride=0), "BAD_SHAPE"),
+    (attn_args, "dfl_prefix_attention", dict(prefix_v_head_stride=0), "BAD_SHAPE"),
+    (attn_args, "dfl_prefix_attention", dict(prefix_k_row_stride=0), "BAD_SHAPE"),
+    (attn_args, "dfl_prefix_attention", dict(out_token_stride=0), "BAD_SHAPE"),
+    (verify_args, "dfl_verify_drafts", dict(logits=PTR + 2), "BAD_ARG"),
+    (verify_args, "dfl_verify_drafts", dict(draft_probs=PTR + 2), "BAD_ARG"),
+    (verify_args, "dfl_verify_drafts", dict(tokens_out=PTR + 2), "BAD_ARG"),
+    (verify_args, "dfl_verify_drafts", dict(workspace=None), "BAD_ARG"),
+]
+
+
+@pytest.mark.parametrize("make,entry,change,status", MORE_REFUSED, ids=["%s-%s" % (e[4:], "-".join(c)) for _, e, c, _ in MORE_REFUSED])
+def test_refused_addresses_and_strides(make, entry, change, status):
+    test_refused_before_anything_runs(make, entry, change, status)

@@ -530,3 +530,124 @@ def test_two_calls_at_once_on_two_streams():
     for w, runs in zip(want, got):
         for r in runs:
             assert all(torch.equal(a, b) for a, b in zip(r, w))
+
+
+# ---- what is refused only where there is a device ------------------------------------------------------------------
+def test_workspaces_that_are_too_small_or_lie_askew():
+    import ctypes as C
+    import importlib
+    ops = importlib.import_module("qwen-llm_b200.batch_ops")
+    q, pk, pv, ok, ov = attn_case(3, 1, 8, 2, 128, 5000, 64, "bf16")
+    own_len = torch.tensor([1, 64, 9], device="cuda", dtype=torch.int32)
+    out = torch.full_like(q, 7)
+    a = ops.PrefixAttentionArgs(dtype=ops.BF16, batch=3, n_tokens=1, n_q_heads=8, n_kv_heads=2, head_dim=128, scale=0.1, prefix_len=5000, own_capacity=64)
+    for name, x in (("q", q), ("prefix_k", pk), ("prefix_v", pv), ("own_k", ok), ("own_v", ov), ("own_len", own_len), ("out", out)):
+        setattr(a, name, x.data_ptr())
+    for name, x in (("q", q), ("out", out)):
+        for i, n in enumerate(("batch", "token", "head")):
+            setattr(a, f"{name}_{n}_stride", x.stride(i))
+    for name, x in (("prefix_k", pk), ("prefix_v", pv)):
+        for i, n in enumerate(("row", "head")):
+            setattr(a, f"{name}_{n}_stride", x.stride(i))
+    for name, x in (("own_k", ok), ("own_v", ov)):
+        for i, n in enumerate(("batch", "row", "head")):
+            setattr(a, f"{name}_{n}_stride", x.stride(i))
+    L = pkg.lib()
+    I, V = C.c_int32, C.c_void_p
+    query, call = C.CFUNCTYPE(I, I, V, V)(("dfl_prefix_attention_workspace", L)), C.CFUNCTYPE(I, I, V, V)(("dfl_prefix_attention", L))
+    need = C.c_uint64()
+    pkg.check(query(0, C.byref(a), C.byref(need)))
+    assert need.value > 0
+    work = torch.empty(need.value + 512, device="cuda", dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = work.data_ptr(), need.value - 1
+    for change, name in ((dict(), "BAD_SHAPE"), (dict(workspace=work.data_ptr() + 128, workspace_bytes=need.value), "BAD_ARG"), (dict(workspace=None), "BAD_ARG")):
+        for k, v in change.items():
+            setattr(a, k, v)
+        with pytest.raises(pkg.DflError) as e:
+            pkg.check(call(0, C.byref(a), None))
+        assert e.value.name == name
+    torch.cuda.synchronize()
+    assert (out == 7).all()
+    a.workspace = work.data_ptr()
+    pkg.check(call(0, C.byref(a), None))
+    torch.cuda.synchronize()
+    attn_check(out, q, pk, pv, ok, ov, own_len, scale=a.scale)
+
+
+def test_wrappers_refuse_gradients_and_outputs_that_overlap_themselves():
+    q, pk, pv, ok, ov = attn_case(2, 3, 4, 2, 64, 100, 8, "f16")
+    pos = torch.arange(6, device="cuda", dtype=torch.int32)
+    flat, keys = q.reshape(6, 4, 64), pk[:6]
+    for x in (q.clone().requires_grad_(), q):
+        if x.requires_grad:
+            with pytest.raises(RuntimeError, match="no backward pass"):
+                pkg.prefix_attention(x, pk, pv)
+            with pytest.raises(RuntimeError, match="no backward pass"):
+                pkg.qk_norm_rope(x.reshape(6, 4, 64), keys, pos, theta=1e4)
+            with torch.no_grad():
+                a = pkg.prefix_attention(x, pk, pv)
+        else:
+            assert torch.equal(pkg.prefix_attention(x, pk, pv), a)
+    logits = torch.zeros(2, 2, 10, device="cuda", requires_grad=True)
+    u = torch.zeros(2, 1, device="cuda")
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        pkg.verify_drafts(logits, u.to(torch.int32), u, u[:, 0].contiguous())
+    with pytest.raises(ValueError, match="out: an expanded dimension"):
+        pkg.prefix_attention(q, pk, pv, out=torch.empty(1, 3, 4, 64, device="cuda", dtype=torch.half).expand(2, 3, 4, 64))
+    with pytest.raises(ValueError, match="k_out: an expanded dimension"):
+        pkg.qk_norm_rope(flat, keys, pos, theta=1e4, k_out=torch.empty(6, 1, 64, device="cuda", dtype=torch.half).expand(6, 2, 64))
+    with pytest.raises(pkg.DflError, match="a stride of K or V is zero"):
+        pkg.prefix_attention(q, pk[:, :1].expand(100, 2, 64), pv)
+
+
+# ---- sizes that spread otherwise -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("tokens,hq,hk,dim", [(300, 32, 8, 128), (40, 5, 3, 64), (1500, 2, 2, 256)])
+def test_rope_heads_shared_out_over_warps(tokens, hq, hk, dim):
+    q, k, v, pos, sections, w = rope_case(tokens, hq, hk, dim, dim // 2, 1, False, "bf16")
+    rows = torch.randperm(2 * tokens, device="cuda", generator=rng(1))[:tokens]
+    rows[::5] = -1
+    cache = [torch.full((2 * tokens, hk, dim), 3.0, device="cuda", dtype=torch.bfloat16) for _ in "kv"]
+    qo, ko, vo = pkg.qk_norm_rope(q, k, pos, theta=1e4, rotary_dim=dim // 2, sections=sections, q_weight=w[0], k_weight=w[1], v=v, k_out=cache[0], v_out=cache[1], k_rows=rows)
+    rope_close(qo, *rope_ref(q, w[0], pos, 1e4, dim // 2, sections, False), dim)
+    kept = rows >= 0
+    want, size = rope_ref(k, w[1], pos, 1e4, dim // 2, sections, False)
+    rope_close(ko[rows[kept]], want[kept], size[kept], dim)
+    assert torch.equal(vo[rows[kept]], v[kept])
+    left = torch.ones(2 * tokens, device="cuda", dtype=torch.bool)
+    left[rows[kept]] = False
+    assert (ko[left] == 3).all() and (vo[left] == 3).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_more_pieces_than_are_under_way_at_once(probs, dt):
+    B, K, V = 70, 15, 20001      # some rows are never needed, and which becomes known on the way
+    x, d, ua, us, q = verify_case(B, K, V, dt, probs, 7)
+    g = rng(5)
+    n = torch.randint(0, K + 1, (B,), device="cuda", generator=g).to(torch.int32)
+    t = torch.rand(B, device="cuda", generator=g) * 1.5
+    t[::4] = 0
+    a, _ = verify_check(x, d, ua, us, q)
+    b, _ = verify_check(x, d, ua, us, q, n, t)
+    assert (a < K).any() and (a > 0).any() and not torch.equal(a, b)
+    x[3, 2, 5] = math.nan
+    verify_check(x, d, ua, us, q, n, t)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = pkg.verify_drafts(x, d, ua, us, draft_probs=q, n_draft=n, temperature=t)
+    for seed in (8, 9):
+        new = verify_case(B, K, V, dt, probs, seed)
+        for old, y in zip((x, d, ua, us) + ((q,) if probs else ()), new):
+            old.copy_(y)
+        graph.replay()
+        want = pkg.verify_drafts(x, d, ua, us, draft_probs=q, n_draft=n, temperature=t)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_verify_a_refused_draft_with_all_the_mass():
+    # u = 1 lies outside [0, 1): such a draft falls, nothing is left beside it, and it is drawn from the target itself
+    x = torch.full((2, 2, 300), -math.inf, device="cuda")
+    x[:, :, 17] = 2.0
+    d = torch.full((2, 1), 17, device="cuda", dtype=torch.int32)
+    n, tok = pkg.verify_drafts(x, d, torch.ones(2, 1, device="cuda"), torch.tensor([0.0, 0.9], device="cuda"))
+    assert n.tolist() == [0, 0] and tok.tolist() == [[17, -1]] * 2
