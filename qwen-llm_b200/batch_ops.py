@@ -58,7 +58,7 @@ _FNS = None
 
 
 def _fns():
-    """The library's entry points with their argument types, and torch."""
+    """The library's entry points with their argument types, torch, the status check, dtype codes, and the handle of a device's current stream."""
     global _FNS
     if _FNS is None:
         import torch
@@ -71,7 +71,9 @@ def _fns():
             f = getattr(L, "dfl_" + name)
             f.argtypes, f.restype = [C.c_int32, C.c_char_p, C.POINTER(C.c_uint64)], C.c_int32
         dtypes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-        _FNS = (L, torch, check, dtypes)
+        # the handle without a Stream object around it, where torch has that: 0.1 us instead of 2.3
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+        _FNS = (L, torch, check, dtypes, raw)
     return _FNS
 
 
@@ -82,54 +84,68 @@ def _dtype(dtypes, x, name):
     return d
 
 
-def _need(x, name, shape, like, dtype=None):
-    """x has this shape (None: any extent) and dtype, lies on like's device, with a contiguous last dimension."""
-    if x.shape != shape and (x.dim() != len(shape) or any(want is not None and got != want for got, want in zip(x.shape, shape))):
-        raise ValueError(f"{name}: shape {tuple(x.shape)}, expected {tuple('any' if s is None else s for s in shape)}")
-    if x.device != like.device or not x.is_cuda:
-        raise ValueError(f"{name}: on {x.device}, expected {like.device} (a CUDA device)" if like.is_cuda else f"{name}: on {x.device}, expected a CUDA device")
-    if dtype is not None and x.dtype != dtype:
-        raise TypeError(f"{name}: dtype {x.dtype}, expected {dtype}")
-    if shape and shape[-1] != 1 and x.stride(-1) != 1 and x.shape[-1] > 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous")
-    return x
+def _device(x, name, dims, what):
+    """The device number of the tensor that the others are measured by."""
+    if x.dim() != dims:
+        raise ValueError(f"{name}: shape {tuple(x.shape)}, expected {what}")
+    if not x.is_cuda:
+        raise ValueError(f"{name}: on {x.device}, expected a CUDA device")
+    return x.get_device()
 
 
-def _dense(x, name, shape, like, dtype):
-    _need(x, name, shape, like, dtype)
+def _extents(x, name, dims, what):
+    if x.dim() != dims:
+        raise ValueError(f"{name}: shape {tuple(x.shape)}, expected {what}")
+    return x.shape
+
+
+# Calls of a few microseconds on the device are bounded by the checks here, so a tensor is asked for each of its properties once and looked at closely
+# only when it is out of line: norm and rotation of one token take the host 12 us a call, 9 of them here.
+def _take(x, name, shape, dtype, dev):
+    """(address, strides) of a tensor that has this shape and dtype, lies on device number `dev` and is contiguous in its last dimension."""
+    s = x.stride()
+    if x.shape != shape or x.dtype is not dtype or x.get_device() != dev or s[-1] != 1:
+        if x.shape != shape:
+            raise ValueError(f"{name}: shape {tuple(x.shape)}, expected {tuple(shape)}")
+        if x.get_device() != dev:
+            raise ValueError(f"{name}: on {x.device}, expected cuda:{dev}")
+        if x.dtype is not dtype:
+            raise TypeError(f"{name}: dtype {x.dtype}, expected {dtype}")
+        if x.shape[-1] > 1:
+            raise ValueError(f"{name}: the last dimension must be contiguous")
+    return x.data_ptr(), s
+
+
+def _take_out(x, name, shape, dtype, dev):
+    p, s = _take(x, name, shape, dtype, dev)
+    if 0 in s and any(i == 0 and n > 1 for i, n in zip(s, x.shape)):
+        raise ValueError(f"{name}: an expanded dimension cannot be written")
+    return p, s
+
+
+def _dense(x, name, shape, dtype, dev):
+    p, _ = _take(x, name, shape, dtype, dev)
     if not x.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
-    return x.data_ptr()
-
-
-def _output(x, name, shape, like, dtype=None):
-    _need(x, name, shape, like, dtype)
-    if any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
-        raise ValueError(f"{name}: an expanded dimension cannot be written")
-    return x
+    return p
 
 
 def _no_grad(torch, *tensors):
     """The operators have no backward pass: a result that autograd would take for a constant is refused."""
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
-        raise RuntimeError("no backward pass: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                raise RuntimeError("no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 @contextlib.contextmanager
-def _elsewhere(torch, x, stream):
-    with torch.cuda.device(x.device):
-        s = torch.cuda.current_stream(x.device) if stream is None else stream
-        if s.device != x.device:
-            raise ValueError(f"stream on {s.device}, tensors on {x.device}")
-        with torch.cuda.stream(s):
-            yield s.cuda_stream
-
-
-def _on(torch, x, stream):
-    """The call's device and stream as torch's current ones (what is allocated inside belongs to that stream), and the stream's handle."""
-    if stream is None and torch.cuda.current_device() == x.device.index:
-        return contextlib.nullcontext(torch.cuda.current_stream(x.device).cuda_stream)
-    return _elsewhere(torch, x, stream)
+def _current(torch, dev, stream):
+    """The device, and the stream where one is given, as torch's current ones: what is allocated inside belongs to that stream."""
+    with torch.cuda.device(dev):
+        if stream is not None and stream.device.index != dev:
+            raise ValueError(f"stream on {stream.device}, tensors on cuda:{dev}")
+        with torch.cuda.stream(stream):
+            yield
 
 
 def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, interleaved=False, q_weight=None, k_weight=None, eps=1e-6,
@@ -138,46 +154,57 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
     an axis), and the store of the K (and V) rows: at row t, or at k_rows[t] (int64) of k_out / v_out [rows, Hkv, D], rows outside of which
     are dropped.  Weights are f32 [D].  Outputs that are not given are new tensors of q's dtype.  Returns (q_out, k_out) or, with v, (q_out,
     k_out, v_out)."""
-    L, torch, check, dtypes = _fns()
-    if q.dim() != 3:
-        raise ValueError(f"q: shape {tuple(q.shape)}, expected [tokens, heads, dim]")
-    T, hq, D = q.shape
-    _need(q, "q", (T, hq, D), q)
-    hk = k.shape[1] if k.dim() == 3 else 0
-    _need(k, "k", (T, hk, D), q, q.dtype)
+    L, torch, check, dtypes, raw = _fns()
+    dev = _device(q, "q", 3, "[tokens, heads, dim]")
+    if stream is not None or torch.cuda.current_device() != dev:
+        with _current(torch, dev, stream):
+            return qk_norm_rope(q, k, positions, theta=theta, rotary_dim=rotary_dim, sections=sections, interleaved=interleaved, q_weight=q_weight,
+                                k_weight=k_weight, eps=eps, q_out=q_out, k_out=k_out, k_rows=k_rows, v=v, v_out=v_out)
+    shape, dt, f32 = q.shape, q.dtype, torch.float32
+    T, hq, D = shape
+    hk = _extents(k, "k", 3, "[tokens, heads, dim]")[1]
+    kv_shape = (T, hk, D)
+    q_p, q_s = _take(q, "q", shape, dt, dev)
+    k_p, k_s = _take(k, "k", kv_shape, dt, dev)
     if positions.dim() == 1:
-        positions = positions[None]
-    axes = positions.shape[0]
-    _need(positions, "positions", (axes, T), q, torch.int32)
+        axes, axis_stride = 1, 0
+        pos_p, _ = _take(positions, "positions", (T,), torch.int32, dev)
+    else:
+        axes = _extents(positions, "positions", 2, "[tokens] or [axes, tokens]")[0]
+        pos_p, pos_s = _take(positions, "positions", (axes, T), torch.int32, dev)
+        axis_stride = pos_s[0]
     if not 1 <= axes <= MAX_ROPE_AXES:
         raise ValueError("positions: one to three axes")
     rotary_dim = D if rotary_dim is None else rotary_dim
     sections = [rotary_dim // 2] if sections is None and axes == 1 else sections
     if sections is None or len(sections) != axes:
         raise ValueError("sections: one number of frequencies for each axis")
-    wq = 0 if q_weight is None else _dense(q_weight, "q_weight", (D,), q, torch.float32)
-    wk = 0 if k_weight is None else _dense(k_weight, "k_weight", (D,), q, torch.float32)
+    wq = 0 if q_weight is None else _take(q_weight, "q_weight", (D,), f32, dev)[0]
+    wk = 0 if k_weight is None else _take(k_weight, "k_weight", (D,), f32, dev)[0]
     rows = 0
     if k_rows is not None:
-        rows = _dense(k_rows, "k_rows", (T,), q, torch.int64)
+        rows, _ = _take(k_rows, "k_rows", (T,), torch.int64, dev)
         if k_out is None or (v is not None and v_out is None):
             raise ValueError("k_rows: needs k_out (and v_out)")
-    if v is not None:
-        _need(v, "v", (T, hk, D), q, q.dtype)
     _no_grad(torch, q, k, v, q_weight, k_weight)
-    with _on(torch, q, stream) as handle:
-        q_out = torch.empty((T, hq, D), dtype=q.dtype, device=q.device) if q_out is None else _output(q_out, "q_out", (T, hq, D), q)
-        k_out = torch.empty((T, hk, D), dtype=q_out.dtype, device=q.device) if k_out is None else _output(k_out, "k_out", (None, hk, D), q, q_out.dtype)
-        v_in, v_s, vo, vo_s = 0, (0, 0), 0, (0, 0)
-        if v is not None:
-            v_out = torch.empty((T, hk, D), dtype=q_out.dtype, device=q.device) if v_out is None else _output(v_out, "v_out", (k_out.shape[0], hk, D), q, q_out.dtype)
-            v_in, v_s, vo, vo_s = v.data_ptr(), v.stride(), v_out.data_ptr(), v_out.stride()
-        q_s, k_s, qo_s, ko_s = q.stride(), k.stride(), q_out.stride(), k_out.stride()
-        a = _ROPE.pack(_dtype(dtypes, q, "q"), _dtype(dtypes, q_out, "q_out"), T, hq, hk, D, rotary_dim, axes, *sections, *(0,) * (MAX_ROPE_AXES - axes),
-                       1 if interleaved else 0, theta, eps, 0, q.data_ptr(), k.data_ptr(), v_in, q_s[0], q_s[1], k_s[0], k_s[1], v_s[0], v_s[1], wq, wk,
-                       positions.data_ptr(), positions.stride(0), rows, k_out.shape[0], q_out.data_ptr(), k_out.data_ptr(), vo,
-                       qo_s[0], qo_s[1], ko_s[0], ko_s[1], vo_s[0], vo_s[1])
-        check(L.dfl_qk_norm_rope(q.device.index, a, handle))
+    if q_out is None:
+        q_out = torch.empty(shape, dtype=dt, device=q.device)
+    out_dt = q_out.dtype
+    qo_p, qo_s = _take_out(q_out, "q_out", shape, out_dt, dev)
+    if k_out is None:
+        k_out = torch.empty(kv_shape, dtype=out_dt, device=q.device)
+    n_rows = _extents(k_out, "k_out", 3, "[rows, heads, dim]")[0]
+    ko_p, ko_s = _take_out(k_out, "k_out", (n_rows, hk, D), out_dt, dev)
+    v_p, v_s, vo_p, vo_s = 0, (0, 0), 0, (0, 0)
+    if v is not None:
+        v_p, v_s = _take(v, "v", kv_shape, dt, dev)
+        if v_out is None:
+            v_out = torch.empty(kv_shape, dtype=out_dt, device=q.device)
+        vo_p, vo_s = _take_out(v_out, "v_out", (n_rows, hk, D), out_dt, dev)
+    a = _ROPE.pack(_dtype(dtypes, q, "q"), _dtype(dtypes, q_out, "q_out"), T, hq, hk, D, rotary_dim, axes, *sections, *(0,) * (MAX_ROPE_AXES - axes),
+                   1 if interleaved else 0, theta, eps, 0, q_p, k_p, v_p, q_s[0], q_s[1], k_s[0], k_s[1], v_s[0], v_s[1], wq, wk, pos_p, axis_stride, rows,
+                   n_rows, qo_p, ko_p, vo_p, qo_s[0], qo_s[1], ko_s[0], ko_s[1], vo_s[0], vo_s[1])
+    check(L.dfl_qk_norm_rope(dev, a, raw(dev)))
     return (q_out, k_out) if v is None else (q_out, k_out, v_out)
 
 
@@ -185,37 +212,37 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
     """Attention of a batch over one shared prefix and each request's own rows: q [B, n, Hq, D], prefix_k / prefix_v [P, Hkv, D], own_k / own_v
     [B, cap, Hkv, D] of which own_len[b] (int32) are in use, the block's own rows the last of them.  q_len (int32 [B]): how many of a request's n
     queries exist (all when None); output rows behind them are left as they were (zero in a new tensor).  scale: 1 / sqrt(D) when None."""
-    L, torch, check, dtypes = _fns()
-    if q.dim() != 4:
-        raise ValueError(f"q: shape {tuple(q.shape)}, expected [batch, tokens, heads, dim]")
-    B, n, hq, D = q.shape
-    _need(q, "q", (B, n, hq, D), q)
-    _need(prefix_k, "prefix_k", (None, None, D), q, q.dtype)
-    P, hk = prefix_k.shape[:2]
-    _need(prefix_v, "prefix_v", (P, hk, D), q, q.dtype)
-    cap, ok, ok_s, ov, ov_s, lens = 0, 0, (0, 0, 0), 0, (0, 0, 0), 0
+    L, torch, check, dtypes, raw = _fns()
+    dev = _device(q, "q", 4, "[batch, tokens, heads, dim]")
+    if stream is not None or torch.cuda.current_device() != dev:
+        with _current(torch, dev, stream):
+            return prefix_attention(q, prefix_k, prefix_v, own_k, own_v, own_len, q_len=q_len, scale=scale, out=out)
+    shape, dt = q.shape, q.dtype
+    B, n, hq, D = shape
+    q_p, q_s = _take(q, "q", shape, dt, dev)
+    P, hk, _ = _extents(prefix_k, "prefix_k", 3, "[keys, heads, dim]")
+    pk_p, pk_s = _take(prefix_k, "prefix_k", (P, hk, D), dt, dev)
+    pv_p, pv_s = _take(prefix_v, "prefix_v", (P, hk, D), dt, dev)
+    cap, ok_p, ok_s, ov_p, ov_s, lens = 0, 0, (0, 0, 0), 0, (0, 0, 0), 0
     if own_k is not None:
         if own_v is None or own_len is None:
             raise ValueError("own_k: needs own_v and own_len")
-        _need(own_k, "own_k", (B, None, hk, D), q, q.dtype)
-        cap = own_k.shape[1]
-        _need(own_v, "own_v", (B, cap, hk, D), q, q.dtype)
-        lens = _dense(own_len, "own_len", (B,), q, torch.int32)
-        ok, ok_s, ov, ov_s = own_k.data_ptr(), own_k.stride(), own_v.data_ptr(), own_v.stride()
-    q_lens = 0 if q_len is None else _dense(q_len, "q_len", (B,), q, torch.int32)
+        cap = _extents(own_k, "own_k", 4, "[batch, rows, heads, dim]")[1]
+        ok_p, ok_s = _take(own_k, "own_k", (B, cap, hk, D), dt, dev)
+        ov_p, ov_s = _take(own_v, "own_v", (B, cap, hk, D), dt, dev)
+        lens, _ = _take(own_len, "own_len", (B,), torch.int32, dev)
+    q_lens = 0 if q_len is None else _take(q_len, "q_len", (B,), torch.int32, dev)[0]
     _no_grad(torch, q, prefix_k, prefix_v, own_k, own_v)
-    with _on(torch, q, stream) as handle:
-        if out is None:
-            out = (torch.empty if q_len is None else torch.zeros)((B, n, hq, D), dtype=q.dtype, device=q.device)
-        _output(out, "out", (B, n, hq, D), q, q.dtype)
-        q_s, pk_s, pv_s, o_s = q.stride(), prefix_k.stride(), prefix_v.stride(), out.stride()
-        fields = (_dtype(dtypes, q, "q"), B, n, hq, hk, D, D ** -0.5 if scale is None else scale, 0, P, cap, q.data_ptr(), q_s[0], q_s[1], q_s[2],
-                  prefix_k.data_ptr(), prefix_v.data_ptr(), pk_s[0], pk_s[1], pv_s[0], pv_s[1], ok, ov, ok_s[0], ok_s[1], ok_s[2], ov_s[0], ov_s[1], ov_s[2],
-                  lens, q_lens, out.data_ptr(), o_s[0], o_s[1], o_s[2])
-        dev, need = q.device.index, C.c_uint64()
-        check(L.dfl_prefix_attention_workspace(dev, _ATTN.pack(*fields, 0, 0), need))
-        work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-        check(L.dfl_prefix_attention(dev, _ATTN.pack(*fields, work.data_ptr() if need.value else 0, need.value), handle))
+    if out is None:
+        out = (torch.empty if q_len is None else torch.zeros)(shape, dtype=dt, device=q.device)
+    o_p, o_s = _take_out(out, "out", shape, dt, dev)
+    fields = (_dtype(dtypes, q, "q"), B, n, hq, hk, D, D ** -0.5 if scale is None else scale, 0, P, cap, q_p, q_s[0], q_s[1], q_s[2], pk_p, pv_p, pk_s[0], pk_s[1],
+              pv_s[0], pv_s[1], ok_p, ov_p, ok_s[0], ok_s[1], ok_s[2], ov_s[0], ov_s[1], ov_s[2], lens, q_lens, o_p, o_s[0], o_s[1], o_s[2])
+    need = C.c_uint64()
+    check(L.dfl_prefix_attention_workspace(dev, _ATTN.pack(*fields, 0, 0), need))
+    size = need.value
+    work = q.new_empty(size // 2) if size else None   # of 16-bit elements
+    check(L.dfl_prefix_attention(dev, _ATTN.pack(*fields, work.data_ptr() if size else 0, size), raw(dev)))
     return out
 
 
@@ -224,31 +251,29 @@ def verify_drafts(logits, drafts, u_accept, u_sample, *, draft_probs=None, n_dra
     (n_accepted int32 [B], tokens int32 [B, K + 1], -1 behind the drawn token).  u_accept [B, K] and u_sample [B] are f32 in [0, 1).
     draft_probs f32 [B, K, V]: the distributions the drafts were drawn from (None: each draft had all the mass); n_draft int32 [B]: drafts that
     exist; temperature f32 [B]: 0 is greedy.  n_accepted[b] = -1 - row where that row is no distribution."""
-    L, torch, check, dtypes = _fns()
-    if logits.dim() != 3:
-        raise ValueError(f"logits: shape {tuple(logits.shape)}, expected [batch, drafts + 1, vocab]")
-    B, R, V = logits.shape
+    L, torch, check, dtypes, raw = _fns()
+    dev = _device(logits, "logits", 3, "[batch, drafts + 1, vocab]")
+    if stream is not None or torch.cuda.current_device() != dev:
+        with _current(torch, dev, stream):
+            return verify_drafts(logits, drafts, u_accept, u_sample, draft_probs=draft_probs, n_draft=n_draft, temperature=temperature)
+    shape, f32, i32 = logits.shape, torch.float32, torch.int32
+    B, R, V = shape
     K = R - 1
     if K < 0:
         raise ValueError("logits: one row at least")
-    _need(logits, "logits", (B, R, V), logits)
-    d = _dense(drafts, "drafts", (B, K), logits, torch.int32)
-    ua = _dense(u_accept, "u_accept", (B, K), logits, torch.float32)
-    us = _dense(u_sample, "u_sample", (B,), logits, torch.float32)
-    probs, p_s = 0, (0, 0)
-    if draft_probs is not None:
-        _need(draft_probs, "draft_probs", (B, K, V), logits, torch.float32)
-        probs, p_s = draft_probs.data_ptr(), draft_probs.stride()
-    nd = 0 if n_draft is None else _dense(n_draft, "n_draft", (B,), logits, torch.int32)
-    temp = 0 if temperature is None else _dense(temperature, "temperature", (B,), logits, torch.float32)
+    x_p, x_s = _take(logits, "logits", shape, logits.dtype, dev)
+    d = _dense(drafts, "drafts", (B, K), i32, dev)
+    ua = _dense(u_accept, "u_accept", (B, K), f32, dev)
+    us, _ = _take(u_sample, "u_sample", (B,), f32, dev)
+    probs, p_s = (0, (0, 0)) if draft_probs is None else _take(draft_probs, "draft_probs", (B, K, V), f32, dev)
+    nd = 0 if n_draft is None else _take(n_draft, "n_draft", (B,), i32, dev)[0]
+    temp = 0 if temperature is None else _take(temperature, "temperature", (B,), f32, dev)[0]
     _no_grad(torch, logits, draft_probs)
-    with _on(torch, logits, stream) as handle:
-        n_accepted = torch.empty(B, dtype=torch.int32, device=logits.device)
-        tokens = torch.empty((B, R), dtype=torch.int32, device=logits.device)
-        fields = (_dtype(dtypes, logits, "logits"), B, K, 0, V, logits.data_ptr(), logits.stride(0), logits.stride(1), probs, p_s[0], p_s[1], d, nd, temp, ua, us,
-                  n_accepted.data_ptr(), tokens.data_ptr())
-        dev, need = logits.device.index, C.c_uint64()
-        check(L.dfl_verify_drafts_workspace(dev, _VERIFY.pack(*fields, 0, 0), need))
-        work = torch.empty(need.value, dtype=torch.uint8, device=logits.device) if need.value else None
-        check(L.dfl_verify_drafts(dev, _VERIFY.pack(*fields, work.data_ptr() if need.value else 0, need.value), handle))
+    n_accepted, tokens = drafts.new_empty(B), drafts.new_empty((B, R))
+    fields = (_dtype(dtypes, logits, "logits"), B, K, 0, V, x_p, x_s[0], x_s[1], probs, p_s[0], p_s[1], d, nd, temp, ua, us, n_accepted.data_ptr(), tokens.data_ptr())
+    need = C.c_uint64()
+    check(L.dfl_verify_drafts_workspace(dev, _VERIFY.pack(*fields, 0, 0), need))
+    size = need.value
+    work = drafts.new_empty(size // 4) if size else None   # of 32-bit elements
+    check(L.dfl_verify_drafts(dev, _VERIFY.pack(*fields, work.data_ptr() if size else 0, size), raw(dev)))
     return n_accepted, tokens
