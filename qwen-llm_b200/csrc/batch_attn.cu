@@ -76,6 +76,7 @@ struct BatchAttnParams {
     uint32_t o_blocks, o_splits, o_run;  // of one request
     uint32_t prefix_tiles;
     int32_t fused, direct, p_pair, o_pair;   // p_pair / o_pair: the warpgroups share a row tile and take the key tiles in turn
+    bool gaps;                           // requests may lack whole row blocks
     uint32_t p_parts, parts;             // parts a row may have in the workspace, the prefix's first
     float2* part_ml;                     // [parts][n_kv][rows] reference maximum, sum
     float* part_o;                       // [parts][n_kv][rows][D]
@@ -183,6 +184,30 @@ __device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx) 
     return it;
 }
 
+// The items of a CTA, `first` and then those behind `idx`: every gridDim.x-th.  Where requests may lack whole row blocks (GAPS; the host does not know their
+// lengths) every gridDim.x-th of the items that have rows: a warp looks 32 of them over at a time.  By number alone some CTAs get seven items and others
+// five: 4 prompts of 1024 to 2048 tokens over 8192 keys took 951 us instead of 828.  The other kernels go without: the search alone costs them 3 %.
+template <int D, bool GAPS>
+__device__ __forceinline__ uint32_t item_behind(const BatchAttnParams& p, bool first, uint32_t idx) {
+    if (!GAPS) return first ? blockIdx.x : idx + gridDim.x;
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t base = first ? 0 : idx + 1, skip = first ? blockIdx.x : gridDim.x - 1;
+    for (; base < p.items; base += 32) {
+        const uint32_t i = base + lane;
+        bool has = i < p.p_items;
+        if (!has && i < p.items) {
+            const uint32_t bh = (i - p.p_items) % (p.batch * p.n_kv), rest = (i - p.p_items) / (p.batch * p.n_kv);
+            const uint32_t block = p.o_blocks - 1 - rest / p.o_splits;
+            has = block * (p.o_pair ? BA_ROWS : BaCfg<D>::TILES * BA_ROWS) < (uint32_t)q_len_of(p, bh / p.n_kv) * p.group;
+        }
+        const unsigned there = __ballot_sync(0xffffffffu, has);
+        const uint32_t n = __popc(there);
+        if (skip < n) return base + __ffs(__ballot_sync(0xffffffffu, has && __popc(there & ((1u << lane) - 1)) == skip)) - 1;
+        skip -= n;
+    }
+    return p.items;
+}
+
 // A softmax thread's row.
 struct RowRef {
     uint32_t r;          // of the KV head's rows
@@ -213,7 +238,7 @@ __device__ __forceinline__ void pin(float* v) {
         asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]));
 }
 
-template <typename T, int D>
+template <typename T, int D, bool GAPS>
 __global__ void __launch_bounds__(BA_THREADS, 1)
 batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_constant__ CUtensorMap map_pk, const __grid_constant__ CUtensorMap map_pv,
                      const __grid_constant__ CUtensorMap map_ok, const __grid_constant__ CUtensorMap map_ov) {
@@ -282,11 +307,15 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                 else *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
             }
         };
-        uint32_t idx = blockIdx.x;
-        Item it = item_of<D>(p, idx);
-        RowRef rr = row_ref(p, it, it.pair ? 0 : stream, row);
-        if (steps_of(it, stream) > 0) fetch_q(it, rr);
-        while (true) {
+        uint32_t idx = item_behind<D, GAPS>(p, true, 0);
+        Item it;
+        RowRef rr;
+        if (idx < p.items) {
+            it = item_of<D>(p, idx);
+            rr = row_ref(p, it, it.pair ? 0 : stream, row);
+            if (steps_of(it, stream) > 0) fetch_q(it, rr);
+        }
+        while (idx < p.items) {
             const int steps = steps_of(it, stream), n_p = it.p1 - it.p0;
             const uint32_t base0 = uses[0], base1 = uses[1];
             uses[0] += (uint32_t)(C::SPLIT ? (steps + 1) / 2 : steps);
@@ -303,7 +332,6 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[stream]);
             }
-            const uint32_t idx_next = idx + gridDim.x;
             for (int u = 0; u < steps && ok; ++u) {
                 ok = mbar_wait_warp_inline(&s_full[buf(u)], parity(u), &err, DEV_ERR_WAIT_FULL);
                 if (!ok) break;
@@ -411,6 +439,7 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                 }
             }
             // nothing reads Q any more: the next item's is on its way while the last products are waited for
+            const uint32_t idx_next = item_behind<D, GAPS>(p, false, idx);
             Item it_next;
             RowRef rr_next;
             if (idx_next < p.items) {
@@ -493,7 +522,6 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                     }
                 }
             }
-            if (idx_next >= p.items) break;
             idx = idx_next;
             it = it_next;
             rr = rr_next;
@@ -508,92 +536,92 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         constexpr int LAG = C::BUFS;
         // One thread does it all, and it waits for keys and values ahead of the weights: what stands between a warpgroup's last weights and its next scores
         // is one wait and the issue of the two products.  (A warp with a vote in each of five waits a step and stream took 900 clocks more than the products.)
-        if (elect_one()) {
-            const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(smem);
-            constexpr uint64_t SW = (1ull << 46) | (2ull << 61) | ((uint64_t)(1024 >> 4) << 32);   // 128-byte swizzle, 8-row groups 1024 bytes apart
-            constexpr uint64_t K_DESC = SW | 1ull << 16, V_DESC = SW | (uint64_t)(BA_BOX >> 4) << 16;   // K-major; N-major, 64 dimensions a box
-            uint32_t uses[2] = {0, 0}, q_uses[2] = {0, 0}, seq = 0;   // of the score buffers, of the row tiles, of the ring
-            bool ok = true;
-            for (uint32_t idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
-                const Item it = item_of<D>(p, idx);
-                const int steps[2] = {steps_of(it, 0), C::SPLIT ? 0 : steps_of(it, 1)};
-                const bool shared = it.two && !it.pair;   // both streams use a key tile
-                // Places of K and V in the ring's sequence, in the order of use: K0 V0 K1 V1 ...; with a tile a stream K0 K1 V0 V1 K2 K3 V2 V3 ... and K V of one that
-                // is left; with two buffers K0 K1 V0 K2 V1 ....
-                uint32_t kq[2], vq[2];
-                const uint32_t hop = it.pair ? 4u : 2u * C::UNITS;
+        const bool lead = elect_one();
+        const uint32_t ring_a = smem_u32(ring), q_a = smem_u32(smem);
+        constexpr uint64_t SW = (1ull << 46) | (2ull << 61) | ((uint64_t)(1024 >> 4) << 32);   // 128-byte swizzle, 8-row groups 1024 bytes apart
+        constexpr uint64_t K_DESC = SW | 1ull << 16, V_DESC = SW | (uint64_t)(BA_BOX >> 4) << 16;   // K-major; N-major, 64 dimensions a box
+        uint32_t uses[2] = {0, 0}, q_uses[2] = {0, 0}, seq = 0;   // of the score buffers, of the row tiles, of the ring
+        bool ok = true;
+        for (uint32_t idx = item_behind<D, GAPS>(p, true, 0); idx < p.items; idx = item_behind<D, GAPS>(p, false, idx)) {
+            if (!lead || !ok) continue;
+            const Item it = item_of<D>(p, idx);
+            const int steps[2] = {steps_of(it, 0), C::SPLIT ? 0 : steps_of(it, 1)};
+            const bool shared = it.two && !it.pair;   // both streams use a key tile
+            // Places of K and V in the ring's sequence, in the order of use: K0 V0 K1 V1 ...; with a tile a stream K0 K1 V0 V1 K2 K3 V2 V3 ... and K V of one that
+            // is left; with two buffers K0 K1 V0 K2 V1 ....
+            uint32_t kq[2], vq[2];
+            const uint32_t hop = it.pair ? 4u : 2u * C::UNITS;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    kq[x] = seq + (it.pair ? x : 0);
-                    vq[x] = C::SPLIT ? seq + 2 * C::UNITS : it.pair ? seq + 2 + x : seq + 1;
-                }
-                auto landed = [&](uint32_t q) { ok = ok && mbar_wait_one(&full[q % C::SLOTS], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_FULL); };
-                for (int u = 0; u < steps[0] + LAG && ok; ++u) {   // (the second stream never has more steps)
+            for (int x = 0; x < 2; ++x) {
+                kq[x] = seq + (it.pair ? x : 0);
+                vq[x] = C::SPLIT ? seq + 2 * C::UNITS : it.pair ? seq + 2 + x : seq + 1;
+            }
+            auto landed = [&](uint32_t q) { ok = ok && mbar_wait_one(&full[q % C::SLOTS], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_FULL); };
+            for (int u = 0; u < steps[0] + LAG && ok; ++u) {   // (the second stream never has more steps)
 #pragma unroll
-                    for (int x = 0; x < C::TILES; ++x) {
-                        const int v = u - LAG;
-                        const bool has_pv = v >= 0 && v < steps[x], has_s = u < steps[x];
-                        const uint32_t v_buf = C::SPLIT ? v & 1 : x, s_buf = C::SPLIT ? u & 1 : x;
-                        const bool frees = !shared || x == 1;
-                        const uint32_t k_at = kq[x];
-                        uint32_t v_at = vq[x];
-                        // the last tile's V comes right behind its K where it has no successor or partner
-                        if (C::SPLIT ? v == steps[0] - 1 : it.pair && x == 0 && v == steps[0] - 1 && (it.tiles & 1)) v_at -= C::UNITS;
-                        if (!C::SPLIT) {   // (units of a wide tile arrive one by one)
-                            if (has_pv) landed(v_at);
-                            if (has_s) landed(k_at);
-                        }
-                        if (u == 0 && has_s) ok = ok && mbar_wait_one(&q_full[x], q_uses[x]++ & 1u, &err, DEV_ERR_WAIT_FULL);
-                        if (has_pv) {   // O += P V of step u - LAG
-                            const uint32_t use = C::SPLIT ? uses[v & 1] + (uint32_t)(v >> 1) : uses[x] + (uint32_t)v;
-                            const uint32_t p_a = tmem + C::TM_S + 128u * v_buf, tm_o = tmem + C::TM_O + x * D;
+                for (int x = 0; x < C::TILES; ++x) {
+                    const int v = u - LAG;
+                    const bool has_pv = v >= 0 && v < steps[x], has_s = u < steps[x];
+                    const uint32_t v_buf = C::SPLIT ? v & 1 : x, s_buf = C::SPLIT ? u & 1 : x;
+                    const bool frees = !shared || x == 1;
+                    const uint32_t k_at = kq[x];
+                    uint32_t v_at = vq[x];
+                    // the last tile's V comes right behind its K where it has no successor or partner
+                    if (C::SPLIT ? v == steps[0] - 1 : it.pair && x == 0 && v == steps[0] - 1 && (it.tiles & 1)) v_at -= C::UNITS;
+                    if (!C::SPLIT) {   // (units of a wide tile arrive one by one)
+                        if (has_pv) landed(v_at);
+                        if (has_s) landed(k_at);
+                    }
+                    if (u == 0 && has_s) ok = ok && mbar_wait_one(&q_full[x], q_uses[x]++ & 1u, &err, DEV_ERR_WAIT_FULL);
+                    if (has_pv) {   // O += P V of step u - LAG
+                        const uint32_t use = C::SPLIT ? uses[v & 1] + (uint32_t)(v >> 1) : uses[x] + (uint32_t)v;
+                        const uint32_t p_a = tmem + C::TM_S + 128u * v_buf, tm_o = tmem + C::TM_O + x * D;
 #pragma unroll
-                            for (int half = 0; half < (C::SPLIT ? 1 : 2); ++half) {   // of the keys
-                                ok = ok && mbar_wait_one(&p_full[C::SPLIT ? v_buf : 2 * x + half], use & 1u, &err, DEV_ERR_WAIT_FULL);
-#pragma unroll
-                                for (int w = 0; w < C::UNITS; ++w) {
-                                    const uint32_t slot = (v_at + w) % C::SLOTS;
-                                    if (C::SPLIT) landed(v_at + w);
-                                    if (!ok) break;
-                                    fence_after_sync();
-                                    const uint32_t v_lo = (ring_a + slot * C::SLOT) >> 4;
-#pragma unroll
-                                    for (int i = 0; i < (C::SPLIT ? 8 : 4); ++i) {   // 16 keys each: 8 columns of P; (SPLIT) the second warpgroup's 64 columns on
-                                        const uint32_t j = half * 4 + i;
-                                        mma_ts_rt(tm_o + w * C::UNIT, p_a + (C::SPLIT ? (j >> 2) * 64u + (j & 3) * 8u : j * 8u), V_DESC | (v_lo + 128u * j), ID_O, v == 0 && j == 0 ? 0u : 1u);
-                                    }
-                                    if (C::SPLIT || half == 1) {
-                                        if (frees) mma_commit(&empty[slot]);
-                                        if (w == C::UNITS - 1 && (C::SPLIT || v == steps[x] - 1)) mma_commit(&pv_done[v_buf]);
-                                    }
-                                }
-                            }
-                            vq[x] += hop;
-                        }
-                        if (has_s) {   // S = Q K^T
+                        for (int half = 0; half < (C::SPLIT ? 1 : 2); ++half) {   // of the keys
+                            ok = ok && mbar_wait_one(&p_full[C::SPLIT ? v_buf : 2 * x + half], use & 1u, &err, DEV_ERR_WAIT_FULL);
 #pragma unroll
                             for (int w = 0; w < C::UNITS; ++w) {
-                                const uint32_t slot = (k_at + w) % C::SLOTS;
-                                if (C::SPLIT) landed(k_at + w);
+                                const uint32_t slot = (v_at + w) % C::SLOTS;
+                                if (C::SPLIT) landed(v_at + w);
                                 if (!ok) break;
-                                if (C::SPLIT || !has_pv) fence_after_sync();
-                                const uint32_t k_lo = (ring_a + slot * C::SLOT) >> 4, a_lo = (q_a + x * C::Q_BYTES + w * (C::UNIT / 64) * BA_BOX) >> 4;
+                                fence_after_sync();
+                                const uint32_t v_lo = (ring_a + slot * C::SLOT) >> 4;
 #pragma unroll
-                                for (int j = 0; j < C::UNIT / 16; ++j) {
-                                    const uint32_t at = (uint32_t)((j >> 2) * BA_BOX + (j & 3) * 32) >> 4;
-                                    mma_ss(tmem + C::TM_S + 128u * s_buf, K_DESC | (a_lo + at), K_DESC | (k_lo + at), ID_S, w > 0 || j > 0 ? 1u : 0u);
+                                for (int i = 0; i < (C::SPLIT ? 8 : 4); ++i) {   // 16 keys each: 8 columns of P; (SPLIT) the second warpgroup's 64 columns on
+                                    const uint32_t j = half * 4 + i;
+                                    mma_ts_rt(tm_o + w * C::UNIT, p_a + (C::SPLIT ? (j >> 2) * 64u + (j & 3) * 8u : j * 8u), V_DESC | (v_lo + 128u * j), ID_O, v == 0 && j == 0 ? 0u : 1u);
                                 }
-                                if (w == C::UNITS - 1) mma_commit(&s_full[s_buf]);
-                                if (frees) mma_commit(&empty[slot]);
+                                if (C::SPLIT || half == 1) {
+                                    if (frees) mma_commit(&empty[slot]);
+                                    if (w == C::UNITS - 1 && (C::SPLIT || v == steps[x] - 1)) mma_commit(&pv_done[v_buf]);
+                                }
                             }
-                            kq[x] += C::SPLIT && u == 0 ? C::UNITS : hop;
                         }
+                        vq[x] += hop;
+                    }
+                    if (has_s) {   // S = Q K^T
+#pragma unroll
+                        for (int w = 0; w < C::UNITS; ++w) {
+                            const uint32_t slot = (k_at + w) % C::SLOTS;
+                            if (C::SPLIT) landed(k_at + w);
+                            if (!ok) break;
+                            if (C::SPLIT || !has_pv) fence_after_sync();
+                            const uint32_t k_lo = (ring_a + slot * C::SLOT) >> 4, a_lo = (q_a + x * C::Q_BYTES + w * (C::UNIT / 64) * BA_BOX) >> 4;
+#pragma unroll
+                            for (int j = 0; j < C::UNIT / 16; ++j) {
+                                const uint32_t at = (uint32_t)((j >> 2) * BA_BOX + (j & 3) * 32) >> 4;
+                                mma_ss(tmem + C::TM_S + 128u * s_buf, K_DESC | (a_lo + at), K_DESC | (k_lo + at), ID_S, w > 0 || j > 0 ? 1u : 0u);
+                            }
+                            if (w == C::UNITS - 1) mma_commit(&s_full[s_buf]);
+                            if (frees) mma_commit(&empty[slot]);
+                        }
+                        kq[x] += C::SPLIT && u == 0 ? C::UNITS : hop;
                     }
                 }
-                uses[0] += (uint32_t)(C::SPLIT ? (steps[0] + 1) / 2 : steps[0]);
-                uses[1] += (uint32_t)(C::SPLIT ? steps[0] / 2 : steps[1]);
-                seq += 2u * C::UNITS * (uint32_t)it.tiles;
             }
+            uses[0] += (uint32_t)(C::SPLIT ? (steps[0] + 1) / 2 : steps[0]);
+            uses[1] += (uint32_t)(C::SPLIT ? steps[0] / 2 : steps[1]);
+            seq += 2u * C::UNITS * (uint32_t)it.tiles;
         }
         __syncwarp();
     } else if (warp == 9) {
@@ -601,7 +629,7 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         // ================= producer =================
         uint32_t seq = 0, tails = 0;
         bool ok = true;
-        for (uint32_t idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
+        for (uint32_t idx = item_behind<D, GAPS>(p, true, 0); idx < p.items && ok; idx = item_behind<D, GAPS>(p, false, idx)) {
             const Item it = item_of<D>(p, idx);
             const int n_p = it.p1 - it.p0;
             auto load = [&](int tile, bool is_v) {
@@ -839,6 +867,7 @@ void plan(const dfl_prefix_attention_args* a, BatchAttnParams* p, int sms) {
     p->items = p->p_items + (uint32_t)o_items;
     p->parts = p->p_parts + p->o_splits * (p->o_pair ? 2 : 1);
     p->direct = p->parts == 1;
+    p->gaps = p->q_len != nullptr && p->o_blocks > 1;   // (of one block a request the items come round evenly by themselves)
 }
 
 uint64_t ml_bytes(const BatchAttnParams& p) { return ((uint64_t)p.parts * p.n_kv * p.rows * sizeof(float2) + 255) / 256 * 256; }
@@ -875,9 +904,10 @@ dfl_status make_map(CUtensorMap* map, const void* base, int32_t dtype, uint32_t 
 
 template <typename T, int D>
 dfl_status launch(const BatchAttnParams& p, const CUtensorMap (&m)[4], int sms, cudaStream_t st) {
-    DFL_CUDA(cudaFuncSetAttribute(batch_attn_t5_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, BaCfg<D>::SMEM));
+    const auto kernel = p.gaps ? batch_attn_t5_kernel<T, D, true> : batch_attn_t5_kernel<T, D, false>;
+    DFL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BaCfg<D>::SMEM));
     const uint32_t grid = p.items < (uint32_t)sms ? p.items : (uint32_t)sms;
-    DFL_CUDA(launch_k(batch_attn_t5_kernel<T, D>, dim3(grid), dim3(BA_THREADS), BaCfg<D>::SMEM, st, p, m[0], m[1], m[2], m[3]));
+    DFL_CUDA(launch_k(kernel, dim3(grid), dim3(BA_THREADS), BaCfg<D>::SMEM, st, p, m[0], m[1], m[2], m[3]));
     count_launch();
     if (!p.direct) {
         DFL_CUDA(launch_k(batch_attn_join_kernel<T, D>, dim3(ceil_div((uint64_t)p.rows * p.n_kv, 8)), dim3(256), 0, st, p));
