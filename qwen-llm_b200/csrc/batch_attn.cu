@@ -76,6 +76,7 @@ struct BatchAttnParams {
     uint32_t o_blocks, o_splits, o_run;  // of one request
     uint32_t prefix_tiles;
     int32_t fused, direct, p_pair, o_pair;   // p_pair / o_pair: the warpgroups share a row tile and take the key tiles in turn
+    bool o_twin;                         // two of the own items, a warpgroup each
     bool gaps;                           // requests may lack whole row blocks
     uint32_t p_parts, parts;             // parts a row may have in the workspace, the prefix's first
     float2* part_ml;                     // [parts][n_kv][rows] reference maximum, sum
@@ -135,6 +136,7 @@ struct Item {
     uint32_t part;               // where its rows' parts go
     int own, q_len;              // lengths of the request (own items)
     bool pair;                   // the warpgroups take the key tiles of the same rows in turn
+    bool twin;                   // or each has an item of its own: this is one of them
     bool two;                    // there are two streams
     int tiles;
 };
@@ -142,9 +144,10 @@ struct Item {
 __device__ __forceinline__ int steps_of(const Item& it, int stream) { return it.pair ? (it.tiles + 1 - stream) / 2 : stream == 0 || it.two ? it.tiles : 0; }
 
 template <int D>
-__device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx) {
+__device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx, uint32_t stream) {
     constexpr uint32_t BLOCK = BaCfg<D>::TILES * BA_ROWS;
     Item it;
+    it.twin = false;
     it.o0 = it.o1 = it.p0 = it.p1 = 0;
     it.own = it.q_len = 0;
     it.b = 0;
@@ -159,18 +162,21 @@ __device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx) 
         it.part = split * (it.pair ? 2u : 1u);
     } else {                 // the later rows of a request see more keys: they go first
         idx -= p.p_items;
+        it.twin = BaCfg<D>::TILES == 2 && p.o_twin;
+        if (it.twin) idx = 2 * idx + stream;
         const uint32_t bh = idx % (p.batch * p.n_kv), rest = idx / (p.batch * p.n_kv), split = rest % p.o_splits;
-        const uint32_t block = p.o_blocks - 1 - rest / p.o_splits, per = p.n * p.group;
+        const bool none = it.twin && rest >= p.o_splits;   // the partner of an odd one
+        const uint32_t block = none ? 0 : p.o_blocks - 1 - rest / p.o_splits, per = p.n * p.group;
         it.h = bh % p.n_kv;
         it.b = bh / p.n_kv;
-        it.pair = p.o_pair != 0;
-        const uint32_t first = block * (it.pair ? BA_ROWS : BLOCK);
+        it.pair = p.o_pair && !it.twin;
+        const uint32_t first = block * (p.o_pair ? BA_ROWS : BLOCK);
         it.row0 = it.b * per + first;
         it.own = own_len_of(p, it.b);
         it.q_len = q_len_of(p, it.b);
-        const uint32_t there = (uint32_t)it.q_len * p.group;
+        const uint32_t there = none ? 0 : (uint32_t)it.q_len * p.group;
         it.row_end = it.b * per + (first < there ? min(there, per) : first);
-        const uint32_t last = min(first + (it.pair ? BA_ROWS : BLOCK), there);
+        const uint32_t last = min(first + (p.o_pair ? BA_ROWS : BLOCK), there);
         const int seen = last > first ?   // own keys that the block's last row sees
              min(it.own, max(0, it.own - it.q_len + (int)((last - 1) / p.group) + 1)) : 0;
         const int pre = p.fused ? (int)p.prefix_tiles : 0, all = pre + (seen + BA_KEYS - 1) / BA_KEYS;
@@ -179,7 +185,7 @@ __device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx) 
         it.o0 = max(t0 - pre, 0), it.o1 = max(t1 - pre, it.o0);
         it.part = p.p_parts + split * (it.pair ? 2u : 1u);
     }
-    it.two = BaCfg<D>::TILES == 2 && (it.pair || it.row_end > it.row0 + BA_ROWS);
+    it.two = BaCfg<D>::TILES == 2 && (it.pair || it.twin || it.row_end > it.row0 + BA_ROWS);
     it.tiles = it.row_end > it.row0 ? (it.p1 - it.p0) + (it.o1 - it.o0) : 0;
     return it;
 }
@@ -311,8 +317,8 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         Item it;
         RowRef rr;
         if (idx < p.items) {
-            it = item_of<D>(p, idx);
-            rr = row_ref(p, it, it.pair ? 0 : stream, row);
+            it = item_of<D>(p, idx, stream);
+            rr = row_ref(p, it, it.pair || it.twin ? 0 : stream, row);
             if (steps_of(it, stream) > 0) fetch_q(it, rr);
         }
         while (idx < p.items) {
@@ -443,8 +449,8 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
             Item it_next;
             RowRef rr_next;
             if (idx_next < p.items) {
-                it_next = item_of<D>(p, idx_next);
-                rr_next = row_ref(p, it_next, it_next.pair ? 0 : stream, row);
+                it_next = item_of<D>(p, idx_next, stream);
+                rr_next = row_ref(p, it_next, it_next.pair || it_next.twin ? 0 : stream, row);
                 if (ok && steps_of(it_next, stream) > 0) fetch_q(it_next, rr_next);
             }
             if (steps > 0 && ok) {
@@ -544,30 +550,30 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         bool ok = true;
         for (uint32_t idx = item_behind<D, GAPS>(p, true, 0); idx < p.items; idx = item_behind<D, GAPS>(p, false, idx)) {
             if (!lead || !ok) continue;
-            const Item it = item_of<D>(p, idx);
-            const int steps[2] = {steps_of(it, 0), C::SPLIT ? 0 : steps_of(it, 1)};
-            const bool shared = it.two && !it.pair;   // both streams use a key tile
-            // Places of K and V in the ring's sequence, in the order of use: K0 V0 K1 V1 ...; with a tile a stream K0 K1 V0 V1 K2 K3 V2 V3 ... and K V of one that
-            // is left; with two buffers K0 K1 V0 K2 V1 ....
-            uint32_t kq[2], vq[2];
-            const uint32_t hop = it.pair ? 4u : 2u * C::UNITS;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                kq[x] = seq + (it.pair ? x : 0);
-                vq[x] = C::SPLIT ? seq + 2 * C::UNITS : it.pair ? seq + 2 + x : seq + 1;
-            }
+            const Item it = item_of<D>(p, idx, 0);
+            const int tiles1 = it.twin ? item_of<D>(p, idx, 1).tiles : 0;
+            const int steps[2] = {steps_of(it, 0), C::SPLIT ? 0 : it.twin ? tiles1 : steps_of(it, 1)};
+            const bool own_tiles = it.pair || it.twin, shared = it.two && !own_tiles;   // each stream has tiles of its own, or both use a tile
+            // Places of K and V in the ring's sequence, in the order of use: K0 V0 K1 V1 ...; with a tile a stream K0 K1 V0 V1 K2 K3 V2 V3 ..., as far as both have
+            // steps; with two buffers K0 K1 V0 K2 V1 ....
+            uint32_t now = seq, before = seq;   // of step u, of the step before
+            auto width = [&](int u) { return own_tiles ? (uint32_t)(u < steps[0]) + (uint32_t)(u < steps[1]) : 1u; };   // tiles of a step
             auto landed = [&](uint32_t q) { ok = ok && mbar_wait_one(&full[q % C::SLOTS], (q / C::SLOTS) & 1u, &err, DEV_ERR_WAIT_FULL); };
-            for (int u = 0; u < steps[0] + LAG && ok; ++u) {   // (the second stream never has more steps)
+            for (int u = 0; u < max(steps[0], steps[1]) + LAG && ok; ++u) {
 #pragma unroll
                 for (int x = 0; x < C::TILES; ++x) {
                     const int v = u - LAG;
                     const bool has_pv = v >= 0 && v < steps[x], has_s = u < steps[x];
                     const uint32_t v_buf = C::SPLIT ? v & 1 : x, s_buf = C::SPLIT ? u & 1 : x;
                     const bool frees = !shared || x == 1;
-                    const uint32_t k_at = kq[x];
-                    uint32_t v_at = vq[x];
-                    // the last tile's V comes right behind its K where it has no successor or partner
-                    if (C::SPLIT ? v == steps[0] - 1 : it.pair && x == 0 && v == steps[0] - 1 && (it.tiles & 1)) v_at -= C::UNITS;
+                    uint32_t k_at, v_at;
+                    if (C::SPLIT) {   // the last tile's V comes right behind its K
+                        k_at = seq + (u == 0 ? 0 : 2 * u - 1) * C::UNITS;
+                        v_at = seq + (2 * v + (v == steps[0] - 1 ? 1 : 2)) * C::UNITS;
+                    } else {
+                        k_at = now + (uint32_t)(own_tiles && x && u < steps[0]);
+                        v_at = before + width(v) + (uint32_t)(own_tiles && x && v < steps[0]);
+                    }
                     if (!C::SPLIT) {   // (units of a wide tile arrive one by one)
                         if (has_pv) landed(v_at);
                         if (has_s) landed(k_at);
@@ -597,7 +603,6 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                                 }
                             }
                         }
-                        vq[x] += hop;
                     }
                     if (has_s) {   // S = Q K^T
 #pragma unroll
@@ -615,13 +620,14 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                             if (w == C::UNITS - 1) mma_commit(&s_full[s_buf]);
                             if (frees) mma_commit(&empty[slot]);
                         }
-                        kq[x] += C::SPLIT && u == 0 ? C::UNITS : hop;
                     }
                 }
+                before = now;
+                now += 2 * width(u);
             }
             uses[0] += (uint32_t)(C::SPLIT ? (steps[0] + 1) / 2 : steps[0]);
             uses[1] += (uint32_t)(C::SPLIT ? steps[0] / 2 : steps[1]);
-            seq += 2u * C::UNITS * (uint32_t)it.tiles;
+            seq += 2u * C::UNITS * (uint32_t)(it.tiles + tiles1);
         }
         __syncwarp();
     } else if (warp == 9) {
@@ -630,9 +636,9 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         uint32_t seq = 0, tails = 0;
         bool ok = true;
         for (uint32_t idx = item_behind<D, GAPS>(p, true, 0); idx < p.items && ok; idx = item_behind<D, GAPS>(p, false, idx)) {
-            const Item it = item_of<D>(p, idx);
-            const int n_p = it.p1 - it.p0;
-            auto load = [&](int tile, bool is_v) {
+            const Item it = item_of<D>(p, idx, 0);
+            auto load = [&](const Item& it, int tile, bool is_v) {
+                const int n_p = it.p1 - it.p0;
                 const bool pre = tile < n_p;
                 const int key = (pre ? it.p0 + tile : it.o0 + tile - n_p) * BA_KEYS;
                 const int valid = pre ? BA_KEYS : it.own - key;   // behind the prefix and the capacity TMA itself fills in zeros
@@ -668,17 +674,20 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                 }
             };
             const int ahead = C::SPLIT ? 1 : 0;   // how many tiles the keys are ahead of the values
-            if (it.pair) {
-                for (int i = 0; i < it.tiles && ok; i += 2) {
-                    load(i, false);
-                    if (i + 1 < it.tiles) load(i + 1, false);
-                    load(i, true);
-                    if (i + 1 < it.tiles) load(i + 1, true);
+            if (it.pair || it.twin) {
+                const Item it1 = it.twin ? item_of<D>(p, idx, 1) : it;
+                const int n0 = steps_of(it, 0), n1 = it.twin ? it1.tiles : steps_of(it, 1), step = it.twin ? 1 : 2, first1 = it.twin ? 0 : 1;
+                for (int i = 0; i < max(n0, n1) && ok; ++i) {
+#pragma unroll 1
+                    for (int is_v = 0; is_v < 2; ++is_v) {
+                        if (i < n0) load(it, step * i, is_v);
+                        if (i < n1) load(it1, step * i + first1, is_v);
+                    }
                 }
             } else {
                 for (int i = 0; i < it.tiles + ahead && ok; ++i) {
-                    if (i < it.tiles) load(i, false);
-                    if (i >= ahead) load(i - ahead, true);
+                    if (i < it.tiles) load(it, i, false);
+                    if (i >= ahead) load(it, i - ahead, true);
                 }
             }
         }
@@ -715,7 +724,7 @@ __global__ void __launch_bounds__(256) batch_attn_join_kernel(const __grid_const
         const uint32_t block = (p.o_pair || D > 128 ? BA_ROWS : 2 * BA_ROWS), first = rem / block * block, last = min(first + block, (uint32_t)q_len * p.group);
         const int seen = min(own, max(0, own - q_len + (int)((last - 1) / p.group) + 1));
         const uint32_t tiles = (p.fused ? p.prefix_tiles : 0u) + (uint32_t)(seen + BA_KEYS - 1) / BA_KEYS;
-        n += (tiles + p.o_run - 1) / p.o_run * (p.o_pair ? 2u : 1u);
+        n += (tiles + p.o_run - 1) / p.o_run * (p.o_pair && !p.o_twin ? 2u : 1u);
     }
     const float c = p.scale * 1.4426950408889634f;
     const uint64_t at = (uint64_t)h * p.rows + r, step = (uint64_t)p.n_kv * p.rows;
@@ -828,11 +837,12 @@ void plan(const dfl_prefix_attention_args* a, BatchAttnParams* p, int sms) {
     const uint32_t o_block = D <= 128 && per <= BA_ROWS ? BA_ROWS : block;
     const uint32_t o_blocks = ceil_div(per, o_block);
     p->fused = 5ull * per >= 4ull * o_blocks * o_block && p->prefix_tiles > 0 && own_tiles > 0;
+    double best_us;   // of the last answer
     auto splits_for = [&](uint64_t items, uint32_t tiles, double tile_us, double part_cost) {
-        if (items > 64ull * sms) return 1u;
         uint32_t best = 1u;
-        double best_us = 1e30;
-        for (uint32_t s = 1; s <= tiles && s <= 64; ++s) {
+        best_us = ceil_div(items, (uint64_t)sms) * (tiles * tile_us + start) + part_cost;
+        if (items > 64ull * sms) return 1u;
+        for (uint32_t s = 2; s <= tiles && s <= 64; ++s) {
             const uint32_t run = ceil_div(tiles, s);
             if (ceil_div(tiles, run) != s) continue;
             const double us = ceil_div(items * s, (uint64_t)sms) * (run * tile_us + start) + s * part_cost;
@@ -842,6 +852,7 @@ void plan(const dfl_prefix_attention_args* a, BatchAttnParams* p, int sms) {
     };
     p->p_items = p->p_blocks = p->p_splits = p->p_run = p->p_parts = 0;
     p->o_blocks = p->o_splits = p->o_run = 0;
+    p->o_twin = false;
     p->p_pair = D <= 128 && p->rows <= BA_ROWS;
     p->o_pair = D <= 128 && per <= BA_ROWS;
     const double part_cost = (double)p->rows * p->n_kv * part_us;
@@ -861,11 +872,18 @@ void plan(const dfl_prefix_attention_args* a, BatchAttnParams* p, int sms) {
         const uint64_t items = (uint64_t)p->batch * p->n_kv * o_blocks;
         const double tile_us = D <= 128 && !p->o_pair ? 2 * tile1 : tile1;
         p->o_splits = tiles > 0 ? splits_for(items, tiles, tile_us, part_cost * (p->o_pair ? 2 : 1)) : 1;
+        if (p->o_pair && tiles > 0 && items > 1) {   // enough of them that two at a time still fill the machine
+            const double pair_us = best_us;
+            const uint32_t s = splits_for((items + 1) / 2, tiles, 2 * tile_us, part_cost);
+            p->o_twin = best_us < pair_us;
+            if (p->o_twin) p->o_splits = s;
+        }
         p->o_run = tiles > 0 ? ceil_div(tiles, p->o_splits) : 1;
         o_items = items * p->o_splits;
+        if (p->o_twin) o_items = (o_items + 1) / 2;
     }
     p->items = p->p_items + (uint32_t)o_items;
-    p->parts = p->p_parts + p->o_splits * (p->o_pair ? 2 : 1);
+    p->parts = p->p_parts + p->o_splits * (p->o_pair && !p->o_twin ? 2 : 1);
     p->direct = p->parts == 1;
     p->gaps = p->q_len != nullptr && p->o_blocks > 1;   // (of one block a request the items come round evenly by themselves)
 }

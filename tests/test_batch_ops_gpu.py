@@ -651,3 +651,9 @@ def test_verify_a_refused_draft_with_all_the_mass():
     d = torch.full((2, 1), 17, device="cuda", dtype=torch.int32)
     n, tok = pkg.verify_drafts(x, d, torch.ones(2, 1, device="cuda"), torch.tensor([0.0, 0.9], device="cuda"))
     assert n.tolist() == [0, 0] and tok.tolist() == [[17, -1]] * 2
+
+
+@pytest.mark.parametrize("case", [(333, 1, 3, 1, 128, 64, 260, "f16", "rows"), (301, 2, 4, 1, 64, 0, 500, "bf16", "rows"), (151, 1, 5, 5, 128, 700, 1030, "bf16", "heads")], ids=str)
+def test_attention_of_many_requests_with_few_rows(case):
+    # an odd number of them, of lengths from nothing to all
+    test_attention_against_the_definition(case)
