@@ -54,6 +54,7 @@ def _packer(cls):
 
 
 _ROPE, _ATTN, _VERIFY = _packer(QkNormRopeArgs), _packer(PrefixAttentionArgs), _packer(VerifyDraftsArgs)
+_WORK = struct.Struct("@PQ")   # the last two fields of the structures with a workspace
 _FNS = None
 
 
@@ -236,13 +237,15 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
     if out is None:
         out = (torch.empty if q_len is None else torch.zeros)(shape, dtype=dt, device=q.device)
     o_p, o_s = _take_out(out, "out", shape, dt, dev)
-    fields = (_dtype(dtypes, q, "q"), B, n, hq, hk, D, D ** -0.5 if scale is None else scale, 0, P, cap, q_p, q_s[0], q_s[1], q_s[2], pk_p, pv_p, pk_s[0], pk_s[1],
-              pv_s[0], pv_s[1], ok_p, ov_p, ok_s[0], ok_s[1], ok_s[2], ov_s[0], ov_s[1], ov_s[2], lens, q_lens, o_p, o_s[0], o_s[1], o_s[2])
+    a = _ATTN.pack(_dtype(dtypes, q, "q"), B, n, hq, hk, D, D ** -0.5 if scale is None else scale, 0, P, cap, q_p, q_s[0], q_s[1], q_s[2], pk_p, pv_p, pk_s[0], pk_s[1],
+                   pv_s[0], pv_s[1], ok_p, ov_p, ok_s[0], ok_s[1], ok_s[2], ov_s[0], ov_s[1], ov_s[2], lens, q_lens, o_p, o_s[0], o_s[1], o_s[2], 0, 0)
     need = C.c_uint64()
-    check(L.dfl_prefix_attention_workspace(dev, _ATTN.pack(*fields, 0, 0), need))
+    check(L.dfl_prefix_attention_workspace(dev, a, need))
     size = need.value
-    work = q.new_empty(size // 2) if size else None   # of 16-bit elements
-    check(L.dfl_prefix_attention(dev, _ATTN.pack(*fields, work.data_ptr() if size else 0, size), raw(dev)))
+    if size:
+        work = q.new_empty(size // 2)   # of 16-bit elements
+        a = a[:-_WORK.size] + _WORK.pack(work.data_ptr(), size)
+    check(L.dfl_prefix_attention(dev, a, raw(dev)))
     return out
 
 
@@ -270,10 +273,13 @@ def verify_drafts(logits, drafts, u_accept, u_sample, *, draft_probs=None, n_dra
     temp = 0 if temperature is None else _take(temperature, "temperature", (B,), f32, dev)[0]
     _no_grad(torch, logits, draft_probs)
     n_accepted, tokens = drafts.new_empty(B), drafts.new_empty((B, R))
-    fields = (_dtype(dtypes, logits, "logits"), B, K, 0, V, x_p, x_s[0], x_s[1], probs, p_s[0], p_s[1], d, nd, temp, ua, us, n_accepted.data_ptr(), tokens.data_ptr())
+    a = _VERIFY.pack(_dtype(dtypes, logits, "logits"), B, K, 0, V, x_p, x_s[0], x_s[1], probs, p_s[0], p_s[1], d, nd, temp, ua, us, n_accepted.data_ptr(),
+                     tokens.data_ptr(), 0, 0)
     need = C.c_uint64()
-    check(L.dfl_verify_drafts_workspace(dev, _VERIFY.pack(*fields, 0, 0), need))
+    check(L.dfl_verify_drafts_workspace(dev, a, need))
     size = need.value
-    work = drafts.new_empty(size // 4) if size else None   # of 32-bit elements
-    check(L.dfl_verify_drafts(dev, _VERIFY.pack(*fields, work.data_ptr() if size else 0, size), raw(dev)))
+    if size:
+        work = drafts.new_empty(size // 4)   # of 32-bit elements
+        a = a[:-_WORK.size] + _WORK.pack(work.data_ptr(), size)
+    check(L.dfl_verify_drafts(dev, a, raw(dev)))
     return n_accepted, tokens
