@@ -313,13 +313,22 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                 else *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
             }
         };
+        auto q_there = [&]() {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[stream]);
+        };
         uint32_t idx = item_behind<D, GAPS>(p, true, 0);
         Item it;
         RowRef rr;
         if (idx < p.items) {
             it = item_of<D>(p, idx, stream);
             rr = row_ref(p, it, it.pair || it.twin ? 0 : stream, row);
-            if (steps_of(it, stream) > 0) fetch_q(it, rr);
+            if (steps_of(it, stream) > 0) {
+                fetch_q(it, rr);
+                q_there();
+            }
         }
         while (idx < p.items) {
             const int steps = steps_of(it, stream), n_p = it.p1 - it.p0;
@@ -332,12 +341,6 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
             const bool active = __any_sync(0xffffffffu, rr.there);
             float m = -INFINITY, l = 0.f;
             const int sees_all = __reduce_min_sync(0xffffffffu, rr.there ? rr.sees : 0x7fffffff);   // of own keys, every row of the warp
-            if (steps > 0) {
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[stream]);
-            }
             for (int u = 0; u < steps && ok; ++u) {
                 ok = mbar_wait_warp_inline(&s_full[buf(u)], parity(u), &err, DEV_ERR_WAIT_FULL);
                 if (!ok) break;
@@ -448,14 +451,22 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
             const uint32_t idx_next = item_behind<D, GAPS>(p, false, idx);
             Item it_next;
             RowRef rr_next;
+            bool q_next = false;
             if (idx_next < p.items) {
                 it_next = item_of<D>(p, idx_next, stream);
                 rr_next = row_ref(p, it_next, it_next.pair || it_next.twin ? 0 : stream, row);
-                if (ok && steps_of(it_next, stream) > 0) fetch_q(it_next, rr_next);
+                q_next = steps_of(it_next, stream) > 0;
+                if (ok && q_next) fetch_q(it_next, rr_next);
             }
             if (steps > 0 && ok) {
                 ok = mbar_wait_warp_inline(&pv_done[buf(steps - 1)], C::SPLIT ? parity(steps - 1) : done++ & 1u, &err, DEV_ERR_WAIT_DRAIN);
                 fence_after_sync();
+            }
+            // The next item's first scores are made while this one's output goes out: their buffer is free, and the accumulator is not written before these
+            // warps hand over weights.
+            if (ok && q_next) {
+                fence_before_sync();
+                q_there();
             }
             if (C::SPLIT && active && ok) {   // the warpgroups' sums
                 float* e = reinterpret_cast<float*>(smem + C::OFF_EXCH) + (swaps & 1) * 256;
