@@ -717,32 +717,44 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
     }
 }
 
-// Joins the parts of a row: a warp a row.
-template <typename T, int D>
+// Joins the parts of a row: W warps a row, each every W-th part.  Bound by the latency of the parts' loads: a warp has four parts under way.
+template <typename T, int D, int W>
 __global__ void __launch_bounds__(256) batch_attn_join_kernel(const __grid_constant__ BatchAttnParams p) {
     pdl_prologue();
     constexpr int E = D / 32;
-    const uint64_t idx = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const uint32_t lane = threadIdx.x & 31;
-    if (idx >= (uint64_t)p.rows * p.n_kv) return;
-    const uint32_t h = (uint32_t)(idx / p.rows), r = (uint32_t)(idx % p.rows), per = p.n * p.group, b = r / per, rem = r - b * per, tok = rem / p.group;
-    const int q_len = q_len_of(p, b);
-    if ((int)tok >= q_len) return;
-    // the parts that were written: all of the prefix's; of the own keys those that begin ahead of the last key the row's block sees
-    uint32_t n = p.p_parts;
-    if (p.o_splits > 0) {
-        const int own = own_len_of(p, b);
-        const uint32_t block = (p.o_pair || D > 128 ? BA_ROWS : 2 * BA_ROWS), first = rem / block * block, last = min(first + block, (uint32_t)q_len * p.group);
-        const int seen = min(own, max(0, own - q_len + (int)((last - 1) / p.group) + 1));
-        const uint32_t tiles = (p.fused ? p.prefix_tiles : 0u) + (uint32_t)(seen + BA_KEYS - 1) / BA_KEYS;
-        n += (tiles + p.o_run - 1) / p.o_run * (p.o_pair && !p.o_twin ? 2u : 1u);
+    __shared__ float sums[8][D];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part0 = warp % W;
+    const uint64_t idx = (uint64_t)blockIdx.x * (8 / W) + warp / W;
+    uint32_t n = 0, h = 0, r = 0, b = 0, tok = 0, rem = 0;
+    if (idx < (uint64_t)p.rows * p.n_kv) {
+        h = (uint32_t)(idx / p.rows), r = (uint32_t)(idx % p.rows);
+        const uint32_t per = p.n * p.group;
+        b = r / per, rem = r - b * per, tok = rem / p.group;
+        const int q_len = q_len_of(p, b);
+        if ((int)tok < q_len) {
+            // the parts that were written: all of the prefix's; of the own keys those that begin ahead of the last key the row's block sees
+            n = p.p_parts;
+            if (p.o_splits > 0) {
+                const int own = own_len_of(p, b);
+                const uint32_t block = (p.o_pair || D > 128 ? BA_ROWS : 2 * BA_ROWS), first = rem / block * block, last = min(first + block, (uint32_t)q_len * p.group);
+                const int seen = min(own, max(0, own - q_len + (int)((last - 1) / p.group) + 1));
+                const uint32_t tiles = (p.fused ? p.prefix_tiles : 0u) + (uint32_t)(seen + BA_KEYS - 1) / BA_KEYS;
+                n += (tiles + p.o_run - 1) / p.o_run * (p.o_pair && !p.o_twin ? 2u : 1u);
+            }
+        } else {
+            n = ~0u;   // the row is not there
+        }
+    } else {
+        n = ~0u;
     }
+    const bool there = n != ~0u;
+    if (!there) n = 0;
     const float c = p.scale * 1.4426950408889634f;
     const uint64_t at = (uint64_t)h * p.rows + r, step = (uint64_t)p.n_kv * p.rows;
     float top = -INFINITY;
     for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, p.part_ml[i * step + at].x);
     top = warp_max(top);
-    // a lane's E columns of every part, four parts' loads at a time: the parts with mass first, so that the others cost nothing
+    // a lane's E columns of every part of the warp's: the parts with mass only, so that the others cost nothing
     float l = 0.f, o[E] = {};
     for (uint32_t i0 = 0; i0 < n; i0 += 32) {
         float w = 0.f, li = 0.f;
@@ -752,7 +764,7 @@ __global__ void __launch_bounds__(256) batch_attn_join_kernel(const __grid_const
             li = ml.x == -INFINITY ? ml.y : w * ml.y;   // a NaN sum without a maximum: the item gave up
         }
         l += warp_sum(li);
-        unsigned left = __ballot_sync(0xffffffffu, w > 0.f);
+        unsigned left = __ballot_sync(0xffffffffu, w > 0.f && lane % W == part0);
         while (left) {
             float f[4];
             float4 x[4][E / 4 ? E / 4 : 1];
@@ -785,6 +797,18 @@ __global__ void __launch_bounds__(256) batch_attn_join_kernel(const __grid_const
             }
         }
     }
+    if (W > 1) {   // the row's warps' sums, in the order of the warps
+#pragma unroll
+        for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = o[e];
+        __syncthreads();
+        if (part0) return;
+#pragma unroll
+        for (int k = 1; k < W; ++k) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += sums[warp + k][lane * E + e];
+        }
+    }
+    if (!there) return;
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
     T* dst = static_cast<T*>(p.out) + b * p.o_b + tok * p.o_t + (h * p.group + rem - tok * p.group) * p.o_h + lane * E;
 #pragma unroll
@@ -939,7 +963,11 @@ dfl_status launch(const BatchAttnParams& p, const CUtensorMap (&m)[4], int sms, 
     DFL_CUDA(launch_k(kernel, dim3(grid), dim3(BA_THREADS), BaCfg<D>::SMEM, st, p, m[0], m[1], m[2], m[3]));
     count_launch();
     if (!p.direct) {
-        DFL_CUDA(launch_k(batch_attn_join_kernel<T, D>, dim3(ceil_div((uint64_t)p.rows * p.n_kv, 8)), dim3(256), 0, st, p));
+        const uint64_t rows = (uint64_t)p.rows * p.n_kv;
+        // Few rows: eight warps a row, as long as their CTAs (eight an SM) are one wave.  One token over 16 000 keys, one KV head: 15 us with them, 32 without; 15
+        // requests of 10 tokens, 14 heads: 52 and 51; 48 of 16 tokens, 32 heads: 306 and 238.
+        if (rows <= 8ull * sms) DFL_CUDA(launch_k(batch_attn_join_kernel<T, D, 8>, dim3((unsigned)rows), dim3(256), 0, st, p));
+        else DFL_CUDA(launch_k(batch_attn_join_kernel<T, D, 1>, dim3(ceil_div(rows, 8)), dim3(256), 0, st, p));
         count_launch();
     }
     return DFL_OK;
