@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) qk_norm_rope_any_kernel(const
     __shared__ uint64_t turn[ROPE_MAX_DIM / 2];
     __shared__ uint8_t axis[ROPE_MAX_DIM / 2];
     __shared__ float y[ROPE_WARPS][ROPE_MAX_DIM];
+    __shared__ float2 table[ROPE_WARPS][ROPE_MAX_DIM / 2];
     for (uint32_t j = threadIdx.x; j < p.half; j += blockDim.x) turn[j] = p.turn[j], axis[j] = p.axis[j];
     pdl_prologue();
     __syncthreads();
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) qk_norm_rope_any_kernel(const
     for (uint64_t item = (uint64_t)blockIdx.x * ROPE_WARPS + warp; item < n_items; item += (uint64_t)gridDim.x * ROPE_WARPS) {
         const uint32_t token = (uint32_t)(item / p.parts), part = (uint32_t)(item % p.parts);
         const int64_t row = row_of(p, token);
+        for (uint32_t j = lane; j < p.half; j += 32) table[warp][j] = turn_of(p.pos[axis[j] * p.pos_axis + token], turn[j]);
         for (uint32_t h = part; h < p.n_heads; h += p.parts) {
             const HeadRef<S, D> r = head_of<S, D>(p, h, token, row);
             float sum = 0.f;
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) qk_norm_rope_any_kernel(const
                     const uint32_t f = j < p.half ? j : j - p.half;
                     float out = y[warp][j] * norm * (r.w ? r.w[j] : 1.f);
                     if (r.normed && j < 2 * p.half) {
-                        const float2 t = turn_of(p.pos[axis[f] * p.pos_axis + token], turn[f]);
+                        const float2 t = table[warp][f];
                         const uint32_t o = j < p.half ? j + p.half : f;
                         const float other = y[warp][o] * norm * (r.w ? r.w[o] : 1.f);
                         out = j < p.half ? out * t.x - other * t.y : out * t.x + other * t.y;
@@ -163,14 +165,16 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) qk_norm_rope_any_kernel(const
 // other; a warp has every `parts`-th unit of its tokens.  What bounds it is how much is in flight: a warp keeps three stages of 2 KB of units on
 // their way into its own piece of shared memory (16-byte asynchronous copies, across the borders of tokens), 24 warps an SM.
 // A lane takes two runs of four elements that turn together (j and j + half), so no value crosses lanes but the sum of squares; weight and angle
-// are one factor, made once a token, and everything runs on pairs of f32.
+// are one factor, made once a token, and everything runs on pairs of f32.  Where runs of four do not meet runs of four (!PAIRED: half is no multiple of
+// four) the runs are any, and an element's partner is read from the staged copy of the head: 32 768 tokens of 8 + 4 + 4 heads of 64, half 30:
+// 81 us (393 with a lane per element).
 constexpr int ROPE_STAGES = 4, ROPE_STAGE_BYTES = 2048;
 
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
-template <typename S, typename D, int L>
+template <typename S, typename D, int L, bool PAIRED>
 __global__ void __launch_bounds__(32 * ROPE_WARPS, 3) qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
     constexpr int MAXH = L * 4, PER = (MAXH + 31) / 32;   // frequencies, of a lane
     constexpr uint32_t G = 32 / L, DIM = 8 * L;
@@ -183,8 +187,17 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 3) qk_norm_rope_kernel(const 
     pdl_prologue();
     __syncthreads();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane / L, i = lane % L;
-    const bool turns = 4 * i < p.half;
-    const uint32_t c0 = turns ? 4 * i : 2 * p.half + 8 * (i - p.half / 4), c1 = turns ? p.half + 4 * i : c0 + 4;
+    const bool turns = PAIRED && 4 * i < p.half;
+    const uint32_t c0 = PAIRED && !turns ? 2 * p.half + 8 * (i - p.half / 4) : 4 * i, c1 = turns ? p.half + 4 * i : PAIRED ? c0 + 4 : DIM / 2 + 4 * i;
+    uint32_t other[4];           // !PAIRED: two partners' places each
+    if (!PAIRED) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const uint32_t x = (e < 4 ? c0 : c1 - 4) + e;
+            const uint32_t a = x < p.half ? x + p.half : x < 2 * p.half ? x - p.half : x, b = x + 1 < p.half ? x + 1 + p.half : x + 1 < 2 * p.half ? x + 1 - p.half : x + 1;
+            other[e / 2] = a | b << 16;
+        }
+    }
     uint8_t* ring = stages + warp * (ROPE_STAGES * ROPE_STAGE_BYTES);
     const uint64_t n_items = (uint64_t)p.n_tokens * p.parts, hop = (uint64_t)gridDim.x * ROPE_WARPS;
     const uint32_t uq = (p.n_q + G - 1) / G, uk = (p.n_kv + G - 1) / G, kinds = p.v ? 3 : p.n_kv ? 2 : 1;
@@ -269,10 +282,24 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 3) qk_norm_rope_kernel(const 
             float4 wa = make_float4(1.f, 1.f, 1.f, 1.f), wb = wa, t0 = make_float4(1.f, 0.f, 1.f, 0.f), t1 = t0;
             if (w) wa = *reinterpret_cast<const float4*>(w + c0), wb = *reinterpret_cast<const float4*>(w + c1);
             if (turns) t0 = *reinterpret_cast<const float4*>(&table[warp][4 * i]), t1 = *reinterpret_cast<const float4*>(&table[warp][4 * i + 2]);
-            f_ac[0] = pack2(wa.x * t0.x, wa.y * t0.z), f_ac[1] = pack2(wa.z * t1.x, wa.w * t1.z);
-            f_bs[0] = pack2(-wb.x * t0.y, -wb.y * t0.w), f_bs[1] = pack2(-wb.z * t1.y, -wb.w * t1.w);
-            f_bc[0] = pack2(wb.x * t0.x, wb.y * t0.z), f_bc[1] = pack2(wb.z * t1.x, wb.w * t1.z);
-            f_as[0] = pack2(wa.x * t0.y, wa.y * t0.w), f_as[1] = pack2(wa.z * t1.y, wa.w * t1.w);
+            if (!PAIRED) {   // own factors in f_ac, f_bc, partners' in f_as, f_bs
+                const float own[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+                float mine[8], its[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t x = (e < 4 ? c0 : c1 - 4) + e, o = other[e / 2] >> (e % 2 * 16) & 0xffff;
+                    const float2 t = x < 2 * p.half ? table[warp][x < p.half ? x : o] : make_float2(1.f, 0.f);
+                    mine[e] = own[e] * t.x;
+                    its[e] = (w ? w[o] : 1.f) * (x < p.half ? -t.y : t.y);
+                }
+                f_ac[0] = pack2(mine[0], mine[1]), f_ac[1] = pack2(mine[2], mine[3]), f_bc[0] = pack2(mine[4], mine[5]), f_bc[1] = pack2(mine[6], mine[7]);
+                f_as[0] = pack2(its[0], its[1]), f_as[1] = pack2(its[2], its[3]), f_bs[0] = pack2(its[4], its[5]), f_bs[1] = pack2(its[6], its[7]);
+            } else {
+                f_ac[0] = pack2(wa.x * t0.x, wa.y * t0.z), f_ac[1] = pack2(wa.z * t1.x, wa.w * t1.z);
+                f_bs[0] = pack2(-wb.x * t0.y, -wb.y * t0.w), f_bs[1] = pack2(-wb.z * t1.y, -wb.w * t1.w);
+                f_bc[0] = pack2(wb.x * t0.x, wb.y * t0.z), f_bc[1] = pack2(wb.z * t1.x, wb.w * t1.z);
+                f_as[0] = pack2(wa.x * t0.y, wa.y * t0.w), f_as[1] = pack2(wa.z * t1.y, wa.w * t1.w);
+            }
         }
         kind_now = at.kind;
         asm volatile("cp.async.wait_group %0;" ::"n"(ROPE_STAGES - 1) : "memory");
@@ -298,11 +325,24 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 3) qk_norm_rope_kernel(const 
                 for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                 const float norm = rsqrtf(sum * (1.f / DIM) + p.eps);
                 const uint64_t n2 = pack2(norm, norm);
+                if (!PAIRED) {
+                    float y[8];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint64_t x = mul2(fma2(a2[e], f_ac[e], mul2(b2[e], f_bs[e])), n2), y = mul2(fma2(b2[e], f_bc[e], mul2(a2[e], f_as[e])), n2);
-                    unpack2(x, a[2 * e], a[2 * e + 1]);
-                    unpack2(y, b[2 * e], b[2 * e + 1]);
+                    for (int e = 0; e < 8; ++e) y[e] = to_f<S>(st[u * 256 + (other[e / 2] >> (e % 2 * 16) & 0xffff)]);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint64_t x = mul2(fma2(a2[e], f_ac[e], mul2(pack2(y[2 * e], y[2 * e + 1]), f_as[e])), n2);
+                        const uint64_t z = mul2(fma2(b2[e], f_bc[e], mul2(pack2(y[4 + 2 * e], y[5 + 2 * e]), f_bs[e])), n2);
+                        unpack2(x, a[2 * e], a[2 * e + 1]);
+                        unpack2(z, b[2 * e], b[2 * e + 1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint64_t x = mul2(fma2(a2[e], f_ac[e], mul2(b2[e], f_bs[e])), n2), y = mul2(fma2(b2[e], f_bc[e], mul2(a2[e], f_as[e])), n2);
+                        unpack2(x, a[2 * e], a[2 * e + 1]);
+                        unpack2(y, b[2 * e], b[2 * e + 1]);
+                    }
                 }
             }
             if (stored && h < at.n) {
@@ -326,26 +366,27 @@ bool in_quads(const RopeParams& p) {
     auto src = [&](const void* x, int64_t a, int64_t b) { return reinterpret_cast<uintptr_t>(x) % 16 == 0 && a % chunk == 0 && b % chunk == 0; };
     auto dst = [&](const void* x, int64_t a, int64_t b) { return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(D)) == 0 && a % 4 == 0 && b % 4 == 0; };
     const bool kv = p.n_kv > 0, v = p.n_heads > p.n_q + p.n_kv;
-    return p.half % 4 == 0 && (p.dim == 64 || p.dim == 128 || p.dim == 256) && (!p.n_q || (src(p.q, p.q_t, p.q_h) && dst(p.q_out, p.qo_t, p.qo_h))) &&
+    return (p.dim == 64 || p.dim == 128 || p.dim == 256) && (!p.n_q || (src(p.q, p.q_t, p.q_h) && dst(p.q_out, p.qo_t, p.qo_h))) &&
            (!kv || (src(p.k, p.k_t, p.k_h) && dst(p.k_out, p.ko_t, p.ko_h))) && (!v || (src(p.v, p.v_t, p.v_h) && dst(p.v_out, p.vo_t, p.vo_h))) &&
            reinterpret_cast<uintptr_t>(p.qw) % 16 == 0 && reinterpret_cast<uintptr_t>(p.kw) % 16 == 0;
 }
 template <typename S, typename D, int L>
 cudaError_t launch_quads(const RopeParams& p, dim3 grid, cudaStream_t st) {
     constexpr int smem = ROPE_WARPS * ROPE_STAGES * ROPE_STAGE_BYTES;
-    const cudaError_t e = cudaFuncSetAttribute(qk_norm_rope_kernel<S, D, L>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    return e != cudaSuccess ? e : launch_k(qk_norm_rope_kernel<S, D, L>, grid, dim3(32 * ROPE_WARPS), smem, st, p);
+    const auto kernel = p.half % 4 == 0 ? qk_norm_rope_kernel<S, D, L, true> : qk_norm_rope_kernel<S, D, L, false>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return e != cudaSuccess ? e : launch_k(kernel, grid, dim3(32 * ROPE_WARPS), smem, st, p);
 }
 template <typename S, typename D>
 cudaError_t launch_typed(RopeParams& p, cudaStream_t st) {
     const bool quads = in_quads<S, D>(p);
-    // A token's heads are shared out over as many warps as are resident at once (24 an SM), but a warp keeps a load for each of its lane groups.  One
-    // share more would leave a second round for a few: 100, 300, 768, 1500 tokens of 32 + 8 + 8 heads of 128 take 4.3, 5.8, 8.0, 10.5 us, with the
-    // shares rounded up 4.3, 7.7, 10.2, 14.6, and with eight warps an SM 4.9, 7.0, 10.1, 14.2.
-    const uint64_t parts = (uint64_t)sm_count() * 24 / p.n_tokens > 1 ? (uint64_t)sm_count() * 24 / p.n_tokens : 1;
+    // A token's heads are shared out over as many warps as are resident at once (24 an SM; 48 with a lane per element), but a warp keeps a load for each of
+    // its lane groups.  One share more would leave a second round for a few: 100, 300, 768, 1500 tokens of 32 + 8 + 8 heads of 128 take 4.3, 5.8, 8.0,
+    // 10.5 us, with the shares rounded up 4.3, 7.7, 10.2, 14.6, and with eight warps an SM 4.9, 7.0, 10.1, 14.2.
+    const uint64_t most = (uint64_t)sm_count() * (quads ? 3 : 6), parts = most * ROPE_WARPS / p.n_tokens > 1 ? most * ROPE_WARPS / p.n_tokens : 1;
     const uint32_t groups = quads ? 256 / p.dim : 1, most_parts = (p.n_q + groups - 1) / groups + (p.n_heads - p.n_q + groups - 1) / groups;
     p.parts = (uint32_t)(parts < most_parts ? parts : most_parts);
-    const uint64_t items = (uint64_t)p.n_tokens * p.parts, blocks = (items + ROPE_WARPS - 1) / ROPE_WARPS, most = (uint64_t)sm_count() * 3;
+    const uint64_t items = (uint64_t)p.n_tokens * p.parts, blocks = (items + ROPE_WARPS - 1) / ROPE_WARPS;
     const dim3 grid((unsigned)(blocks < most ? blocks : most)), block(32 * ROPE_WARPS);
     if (!quads) return launch_k(qk_norm_rope_any_kernel<S, D>, grid, block, 0, st, p);
     if (p.dim == 64) return launch_quads<S, D, 8>(p, grid, st);

@@ -657,3 +657,10 @@ def test_verify_a_refused_draft_with_all_the_mass():
 def test_attention_of_many_requests_with_few_rows(case):
     # an odd number of them, of lengths from nothing to all
     test_attention_against_the_definition(case)
+
+
+@pytest.mark.parametrize("case", [(300, 8, 4, 64, 60, 1, True, "bf16", "f16"), (33, 6, 2, 64, 2, 1, False, "f32", "f32"), (257, 4, 3, 128, 102, 3, True, "bf16", "bf16"),
+                                  (40, 5, 1, 128, 126, 1, False, "f16", "f32"), (65, 3, 2, 256, 250, 2, False, "f32", "bf16"), (7, 1, 1, 256, 6, 3, True, "f16", "f16"),
+                                  (90, 4, 2, 80, 78, 2, True, "bf16", "bf16"), (129, 2, 2, 96, 96, 1, False, "f32", "f16")], ids=str)
+def test_rope_rotary_widths_of_all_kinds(case):
+    test_rope_against_the_definition(case)
