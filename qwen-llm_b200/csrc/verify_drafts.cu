@@ -614,9 +614,13 @@ cudaError_t launch(const VerifyParams& p, cudaStream_t st) {
     e = launch_k(verify_pieces_kernel<T>, dim3((unsigned)(items < most ? items : most)), dim3(ST_THREADS), ST_SLOTS * ST_BYTES, st, p);
     if (e != cudaSuccess) return e;
     // As many CTAs a request as leave a single wave: they share the exponentials, but each decides for itself.  151 936 tokens: 14 us with sixteen for one
-    // request, 42 us with one each for 128 (with eight each 83 us).
+    // request, 42 us with one each for 128 (with eight each 83 us).  Of sixteen CTAs seven clusters find room side by side (8 requests of 153 430 tokens:
+    // 20 us with eight each, 27 with sixteen).  Each CTA has a thousand tokens at least, and four thousand where the clusters take more than half of the
+    // SMs, because large ones then wait for each other's places: 16 requests of 32 000 tokens 16 us with four each, 22 with eight; of 1328 tokens 11 with
+    // one, 19 with eight.
+    const uint64_t sms = (uint64_t)sm_count();
     uint32_t cluster = DRAW_CLUSTER;
-    while (cluster > 1 && (uint64_t)cluster * p.batch > (uint64_t)sm_count()) cluster /= 2;
+    while (cluster > 1 && ((uint64_t)cluster * p.batch > (cluster == DRAW_CLUSTER ? sms * 4 / 5 : sms) || cluster * (2ull * cluster * p.batch > sms ? 4096u : 1024u) > p.vocab)) cluster /= 2;
     const cudaError_t f = cudaFuncSetAttribute(verify_draw_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (f != cudaSuccess) return f;
     cudaLaunchConfig_t cfg = {};
