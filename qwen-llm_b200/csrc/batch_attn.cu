@@ -15,8 +15,9 @@
 // One persistent CTA an SM; S = Q K^T and O += P V on the tensor cores (tcgen05, both accumulators and P in tensor memory), K and V tiles by
 // TMA into a ring.  Two warpgroups of softmax threads (thread = row), one MMA issuer, one producer.  A step is a key tile.
 //   * head widths 64 and 128: two streams, each with its warpgroup, score buffer and accumulator, half a step apart, so that one's products run under the
-//     other's exponentials; a row tile each or, when the item has at most 128 rows, every other key tile of the same rows (two parts of a row
-//     then).  P goes out in two halves, the first half's product runs under the second half's exponentials.  (Two buffers of 64 keys a stream
+//     other's exponentials.  They take a row tile each; of an item with at most 128 rows every other key tile (two parts of a row then: joining them in
+//     the CTA took 119 us where the second kernel takes 113, 64 requests of a token over 32 768 + 1024 keys); or, with enough such items, an item
+//     each, so that their starts and ends coincide (105 us).  P goes out in two halves, the first half's product runs under the second half's exponentials.  (Two buffers of 64 keys a stream
 //     instead were slower: the product of a 64-key tile reads Q from shared memory as often as that of a 128-key tile, 192 bytes a clock.)
 //   * 256: the output takes half of tensor memory, there is one stream with two score buffers; the warpgroups take a half of each key tile's columns,
 //     agree on the maximum through shared memory and scale and write a half of the output's columns each.
@@ -964,9 +965,11 @@ dfl_status launch(const BatchAttnParams& p, const CUtensorMap (&m)[4], int sms, 
     count_launch();
     if (!p.direct) {
         const uint64_t rows = (uint64_t)p.rows * p.n_kv;
-        // Few rows: eight warps a row, as long as their CTAs (eight an SM) are one wave.  One token over 16 000 keys, one KV head: 15 us with them, 32 without; 15
-        // requests of 10 tokens, 14 heads: 52 and 51; 48 of 16 tokens, 32 heads: 306 and 238.
+        // Few rows: eight warps a row, as long as their CTAs (eight an SM) are one wave.  One token over 16 000 keys, one KV head: 15 us with them, 32 without; 48
+        // requests of 16 tokens, 32 heads: 306 and 238.  Two a row up to 16 rows an SM: 64 requests of a token, 32 heads, over 8000 + 256 keys 48.7 us (one: 51.5,
+        // four: 51.2), 100 of them 71.0 (one: 68.5).
         if (rows <= 8ull * sms) DFL_CUDA(launch_k(batch_attn_join_kernel<T, D, 8>, dim3((unsigned)rows), dim3(256), 0, st, p));
+        else if (rows <= 16ull * sms) DFL_CUDA(launch_k(batch_attn_join_kernel<T, D, 2>, dim3(ceil_div(rows, 4)), dim3(256), 0, st, p));
         else DFL_CUDA(launch_k(batch_attn_join_kernel<T, D, 1>, dim3(ceil_div(rows, 8)), dim3(256), 0, st, p));
         count_launch();
     }

@@ -664,3 +664,8 @@ def test_attention_of_many_requests_with_few_rows(case):
                                   (90, 4, 2, 80, 78, 2, True, "bf16", "bf16"), (129, 2, 2, 96, 96, 1, False, "f32", "f16")], ids=str)
 def test_rope_rotary_widths_of_all_kinds(case):
     test_rope_against_the_definition(case)
+
+
+@pytest.mark.parametrize("case", [(100, 1, 16, 4, 64, 3000, 130, "bf16", "rows"), (50, 4, 8, 2, 256, 900, 40, "f16", "rows"), (50, 2, 16, 4, 128, 2500, 140, "f16", "heads")], ids=str)
+def test_attention_of_some_hundred_rows_a_head(case):
+    test_attention_against_the_definition(case)
