@@ -78,7 +78,8 @@ struct BatchAttnParams {
     uint32_t prefix_tiles;
     int32_t fused, direct, p_pair, o_pair;   // p_pair / o_pair: the warpgroups share a row tile and take the key tiles in turn
     bool o_twin;                         // two of the own items, a warpgroup each
-    bool gaps;                           // requests may lack whole row blocks
+    int32_t walk;                        // how a CTA finds its items: Walk
+    uint32_t free_ctas, early;           // the CTAs with a prefix item less than the others, the last of the grid; own items that they take ahead of the rest
     uint32_t p_parts, parts;             // parts a row may have in the workspace, the prefix's first
     float2* part_ml;                     // [parts][n_kv][rows] reference maximum, sum
     float* part_o;                       // [parts][n_kv][rows][D]
@@ -191,12 +192,28 @@ __device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx, 
     return it;
 }
 
-// The items of a CTA, `first` and then those behind `idx`: every gridDim.x-th.  Where requests may lack whole row blocks (GAPS; the host does not know their
-// lengths) every gridDim.x-th of the items that have rows: a warp looks 32 of them over at a time.  By number alone some CTAs get seven items and others
-// five: 4 prompts of 1024 to 2048 tokens over 8192 keys took 951 us instead of 828.  The other kernels go without: the search alone costs them 3 %.
-template <int D, bool GAPS>
+// The items of a CTA, `first` and then those behind `idx`.  The search costs the hot loop some registers, 3 % of the time, so it is three kernels:
+//   * PLAIN: every gridDim.x-th.
+//   * RANKS: where requests may lack whole row blocks (the host does not know their lengths) every gridDim.x-th of the items that have rows: a warp looks 32
+//     of them over at a time.  By number alone some CTAs get seven items and others five: 4 prompts of 1024 to 2048 tokens over 8192 keys took 951 us
+//     instead of 828.
+//   * EARLY: every gridDim.x-th of the prefix's and then of the own ones, of which the CTAs that had a prefix item less than the others take some ahead (see
+//     plan(): 30 requests of 8 tokens, heads of 256, over 12 001 keys 62.7 us without, 57.0 with; 56 of 7 tokens over 2506 keys 84 and 74).
+enum Walk { PLAIN, RANKS, EARLY };
+template <int D, Walk WALK>
 __device__ __forceinline__ uint32_t item_behind(const BatchAttnParams& p, bool first, uint32_t idx) {
-    if (!GAPS) return first ? blockIdx.x : idx + gridDim.x;
+    if (WALK == PLAIN) return first ? blockIdx.x : idx + gridDim.x;
+    if (WALK == EARLY) {
+        const uint32_t next = first ? blockIdx.x : idx + (idx >= p.p_items && idx < p.p_items + p.early ? p.free_ctas : gridDim.x);
+        if (next < p.p_items || (!first && idx >= p.p_items + p.early)) return next;
+        if (!first && idx >= p.p_items) {   // from one early item to the next
+            if (next < p.p_items + p.early) return next;
+        } else if (blockIdx.x >= gridDim.x - p.free_ctas) {
+            const uint32_t own = blockIdx.x - (gridDim.x - p.free_ctas);
+            if (own < p.early) return p.p_items + own;
+        }
+        return p.p_items + p.early + blockIdx.x;
+    }
     const uint32_t lane = threadIdx.x & 31;
     uint32_t base = first ? 0 : idx + 1, skip = first ? blockIdx.x : gridDim.x - 1;
     for (; base < p.items; base += 32) {
@@ -245,7 +262,7 @@ __device__ __forceinline__ void pin(float* v) {
         asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]));
 }
 
-template <typename T, int D, bool GAPS>
+template <typename T, int D, Walk WALK>
 __global__ void __launch_bounds__(BA_THREADS, 1)
 batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_constant__ CUtensorMap map_pk, const __grid_constant__ CUtensorMap map_pv,
                      const __grid_constant__ CUtensorMap map_ok, const __grid_constant__ CUtensorMap map_ov) {
@@ -320,7 +337,7 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[stream]);
         };
-        uint32_t idx = item_behind<D, GAPS>(p, true, 0);
+        uint32_t idx = item_behind<D, WALK>(p, true, 0);
         Item it;
         RowRef rr;
         if (idx < p.items) {
@@ -456,7 +473,7 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                 }
             }
             // nothing reads Q any more: the next item's is on its way while the last products are waited for
-            const uint32_t idx_next = item_behind<D, GAPS>(p, false, idx);
+            const uint32_t idx_next = item_behind<D, WALK>(p, false, idx);
             Item it_next;
             RowRef rr_next;
             bool q_next = false;
@@ -567,7 +584,7 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         constexpr uint64_t K_DESC = SW | 1ull << 16, V_DESC = SW | (uint64_t)(BA_BOX >> 4) << 16;   // K-major; N-major, 64 dimensions a box
         uint32_t uses[2] = {0, 0}, q_uses[2] = {0, 0}, seq = 0;   // of the score buffers, of the row tiles, of the ring
         bool ok = true;
-        for (uint32_t idx = item_behind<D, GAPS>(p, true, 0); idx < p.items; idx = item_behind<D, GAPS>(p, false, idx)) {
+        for (uint32_t idx = item_behind<D, WALK>(p, true, 0); idx < p.items; idx = item_behind<D, WALK>(p, false, idx)) {
             if (!lead || !ok) continue;
             const Item it = item_of<D>(p, idx, 0);
             const int tiles1 = it.twin ? item_of<D>(p, idx, 1).tiles : 0;
@@ -654,7 +671,7 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
         // ================= producer =================
         uint32_t seq = 0, tails = 0;
         bool ok = true;
-        for (uint32_t idx = item_behind<D, GAPS>(p, true, 0); idx < p.items && ok; idx = item_behind<D, GAPS>(p, false, idx)) {
+        for (uint32_t idx = item_behind<D, WALK>(p, true, 0); idx < p.items && ok; idx = item_behind<D, WALK>(p, false, idx)) {
             const Item it = item_of<D>(p, idx, 0);
             auto load = [&](const Item& it, int tile, bool is_v) {
                 const int n_p = it.p1 - it.p0;
@@ -899,10 +916,11 @@ void plan(const dfl_prefix_attention_args* a, BatchAttnParams* p, int sms) {
     p->p_pair = D <= 128 && p->rows <= BA_ROWS;
     p->o_pair = D <= 128 && per <= BA_ROWS;
     const double part_cost = (double)p->rows * p->n_kv * part_us;
+    double prefix_tile_us = 0, own_tile_us = 0;
     if (p->prefix_tiles > 0 && !p->fused) {
         p->p_blocks = ceil_div(p->rows, p->p_pair ? BA_ROWS : block);
         const uint64_t items = (uint64_t)p->p_blocks * p->n_kv;
-        const double tile_us = D <= 128 && !p->p_pair ? 2 * tile1 : tile1;
+        const double tile_us = prefix_tile_us = D <= 128 && !p->p_pair ? 2 * tile1 : tile1;
         p->p_splits = splits_for(items, p->prefix_tiles, tile_us, part_cost * (p->p_pair ? 2 : 1));
         p->p_run = ceil_div(p->prefix_tiles, p->p_splits);
         p->p_items = (uint32_t)(items * p->p_splits);
@@ -922,13 +940,34 @@ void plan(const dfl_prefix_attention_args* a, BatchAttnParams* p, int sms) {
             if (p->o_twin) p->o_splits = s;
         }
         p->o_run = tiles > 0 ? ceil_div(tiles, p->o_splits) : 1;
+        own_tile_us = p->o_twin ? 2 * tile_us : tile_us;
         o_items = items * p->o_splits;
         if (p->o_twin) o_items = (o_items + 1) / 2;
     }
     p->items = p->p_items + (uint32_t)o_items;
     p->parts = p->p_parts + p->o_splits * (p->o_pair && !p->o_twin ? 2 : 1);
     p->direct = p->parts == 1;
-    p->gaps = p->q_len != nullptr && p->o_blocks > 1;   // (of one block a request the items come round evenly by themselves)
+    p->walk = p->q_len != nullptr && p->o_blocks > 1 ? RANKS : PLAIN;   // (of one block a request the items come round evenly by themselves)
+    // Own items ahead for the CTAs that have a prefix item less than the others, where that is worth a twentieth.
+    p->free_ctas = p->early = 0;
+    const uint64_t grid = p->items < (uint32_t)sms ? p->items : sms, short_of = p->p_items % grid, rounds = p->p_items / grid;
+    if (p->walk == PLAIN && short_of && o_items > 0) {
+        const double own_us = own_tile_us * p->o_run + start, prefix_us = prefix_tile_us * p->p_run + start;
+        auto plain_us = [&](uint64_t c) {   // of CTA c
+            const uint64_t prefix = rounds + (c < short_of), all = p->items / grid + (c < p->items % grid);
+            return prefix * prefix_us + (all - prefix) * own_us;
+        };
+        double best = 0;
+        for (uint64_t c : {(uint64_t)0, short_of, p->items % grid, grid - 1}) best = plain_us(c) > best ? plain_us(c) : best;
+        best *= 0.95;
+        p->free_ctas = (uint32_t)(grid - short_of);
+        for (uint64_t e = 1; e <= 64; ++e) {
+            const uint64_t early = e * p->free_ctas < o_items ? e * p->free_ctas : o_items;
+            const double idle = ceil_div(early, p->free_ctas) * own_us, busy = idle > prefix_us ? idle : prefix_us;
+            const double us = rounds * prefix_us + busy + ceil_div(o_items - early, grid) * own_us;
+            if (us < best) best = us, p->early = (uint32_t)early, p->walk = EARLY;
+        }
+    }
 }
 
 uint64_t ml_bytes(const BatchAttnParams& p) { return ((uint64_t)p.parts * p.n_kv * p.rows * sizeof(float2) + 255) / 256 * 256; }
@@ -965,7 +1004,7 @@ dfl_status make_map(CUtensorMap* map, const void* base, int32_t dtype, uint32_t 
 
 template <typename T, int D>
 dfl_status launch(const BatchAttnParams& p, const CUtensorMap (&m)[4], int sms, cudaStream_t st) {
-    const auto kernel = p.gaps ? batch_attn_t5_kernel<T, D, true> : batch_attn_t5_kernel<T, D, false>;
+    const auto kernel = p.walk == RANKS ? batch_attn_t5_kernel<T, D, RANKS> : p.walk == EARLY ? batch_attn_t5_kernel<T, D, EARLY> : batch_attn_t5_kernel<T, D, PLAIN>;
     DFL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BaCfg<D>::SMEM));
     const uint32_t grid = p.items < (uint32_t)sms ? p.items : (uint32_t)sms;
     DFL_CUDA(launch_k(kernel, dim3(grid), dim3(BA_THREADS), BaCfg<D>::SMEM, st, p, m[0], m[1], m[2], m[3]));
