@@ -669,3 +669,9 @@ def test_rope_rotary_widths_of_all_kinds(case):
 @pytest.mark.parametrize("case", [(100, 1, 16, 4, 64, 3000, 130, "bf16", "rows"), (50, 4, 8, 2, 256, 900, 40, "f16", "rows"), (50, 2, 16, 4, 128, 2500, 140, "f16", "heads")], ids=str)
 def test_attention_of_some_hundred_rows_a_head(case):
     test_attention_against_the_definition(case)
+
+
+@pytest.mark.parametrize("case", [(56, 7, 56, 8, 128, 1300, 246, "f16", "rows"), (42, 100, 8, 8, 128, 853, 100, "bf16", "rows"), (30, 8, 16, 2, 256, 6001, 515, "bf16", "heads"),
+                                  (60, 12, 12, 2, 64, 5000, 300, "f16", "rows")], ids=str)
+def test_attention_of_prefix_and_own_items_that_fill_up_each_other(case):
+    test_attention_against_the_definition(case)
