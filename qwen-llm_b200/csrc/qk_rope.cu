@@ -127,9 +127,9 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) qk_norm_rope_any_kernel(const
     pdl_prologue();
     __syncthreads();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint64_t n_items = (uint64_t)p.n_tokens * p.parts;
-    for (uint64_t item = (uint64_t)blockIdx.x * ROPE_WARPS + warp; item < n_items; item += (uint64_t)gridDim.x * ROPE_WARPS) {
-        const uint32_t token = (uint32_t)(item / p.parts), part = (uint32_t)(item % p.parts);
+    const uint32_t n_items = p.n_tokens * p.parts;   // (several shares a token only of few tokens: below 2^31)
+    for (uint32_t item = blockIdx.x * ROPE_WARPS + warp; item < n_items; item += gridDim.x * ROPE_WARPS) {
+        const uint32_t token = item / p.parts, part = item % p.parts;
         const int64_t row = row_of(p, token);
         for (uint32_t j = lane; j < p.half; j += 32) table[warp][j] = turn_of(p.pos[axis[j] * p.pos_axis + token], turn[j]);
         for (uint32_t h = part; h < p.n_heads; h += p.parts) {
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS) qk_norm_rope_any_kernel(const
 // A lane takes two runs of four elements that turn together (j and j + half), so no value crosses lanes but the sum of squares; weight and angle
 // are one factor, made once a token, and everything runs on pairs of f32.  Where runs of four do not meet runs of four (!PAIRED: half is no multiple of
 // four) the runs are any, and an element's partner is read from the staged copy of the head: 32 768 tokens of 8 + 4 + 4 heads of 64, half 30:
-// 81 us (393 with a lane per element).
+// 69 us (390 with a lane per element).
 constexpr int ROPE_STAGES = 4, ROPE_STAGE_BYTES = 2048;
 
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
@@ -199,38 +199,38 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 3) qk_norm_rope_kernel(const 
         }
     }
     uint8_t* ring = stages + warp * (ROPE_STAGES * ROPE_STAGE_BYTES);
-    const uint64_t n_items = (uint64_t)p.n_tokens * p.parts, hop = (uint64_t)gridDim.x * ROPE_WARPS;
+    const uint32_t n_items = p.n_tokens * p.parts, hop = gridDim.x * ROPE_WARPS;   // (several shares a token only of few tokens: below 2^31)
+    const bool whole = p.parts == 1;   // items are tokens: no division (with 64-bit ones 32 768 tokens of 32 + 8 + 8 heads took 142 us instead of 133, of 2 + 2 + 2 53 instead of 41)
     const uint32_t uq = (p.n_q + G - 1) / G, uk = (p.n_kv + G - 1) / G, kinds = p.v ? 3 : p.n_kv ? 2 : 1;
 
     // a walk over the units: item (token and share), kind (q, k, v), first head
     struct Walk {
-        uint64_t item;
-        uint32_t token, kind, h, n;   // n: heads of the kind
+        uint32_t item, token, kind, h, n;   // n: heads of the kind
     };
     const uint32_t step = p.parts * G;
     auto settle = [&](Walk& w) {      // on to a kind and an item that has units
         while (w.h >= w.n) {
             if (++w.kind < kinds) {
-                const uint32_t before = w.kind == 1 ? uq : uq + uk, part = (uint32_t)(w.item - (uint64_t)w.token * p.parts);
+                const uint32_t before = w.kind == 1 ? uq : uq + uk, part = w.item - w.token * p.parts;
                 w.n = p.n_kv;
-                w.h = (part + p.parts - before % p.parts) % p.parts * G;
+                w.h = whole ? 0 : (part + p.parts - before % p.parts) % p.parts * G;
             } else {
                 w.item += hop;
                 if (w.item >= n_items) return;
-                w.token = (uint32_t)(w.item / p.parts);
+                w.token = whole ? w.item : w.item / p.parts;
                 w.kind = 0;
                 w.n = p.n_q;
-                w.h = (uint32_t)(w.item - (uint64_t)w.token * p.parts) * G;
+                w.h = (w.item - w.token * p.parts) * G;
             }
         }
     };
     auto start = [&]() {
         Walk w;
-        w.item = (uint64_t)blockIdx.x * ROPE_WARPS + warp;
+        w.item = blockIdx.x * ROPE_WARPS + warp;
         w.kind = 0, w.n = p.n_q, w.token = 0, w.h = 0;
         if (w.item < n_items) {
-            w.token = (uint32_t)(w.item / p.parts);
-            w.h = (uint32_t)(w.item - (uint64_t)w.token * p.parts) * G;
+            w.token = w.item / p.parts;
+            w.h = (w.item - w.token * p.parts) * G;
             settle(w);
         }
         return w;
@@ -253,15 +253,15 @@ __global__ void __launch_bounds__(32 * ROPE_WARPS, 3) qk_norm_rope_kernel(const 
         slot_in = slot_in + 1 == ROPE_STAGES ? 0 : slot_in + 1;
     };
     int32_t pos[PER];
-    auto fetch = [&](uint64_t item) {
-        const uint32_t token = (uint32_t)(item / p.parts);
+    auto fetch = [&](uint32_t item) {
+        const uint32_t token = whole ? item : item / p.parts;
 #pragma unroll
         for (int k = 0; k < PER; ++k)
             if (lane + 32 * k < p.half) pos[k] = p.pos[axis[lane + 32 * k] * p.pos_axis + token];
     };
     if (at.item < n_items) fetch(at.item);
     for (int s = 0; s < ROPE_STAGES - 1; ++s) issue();
-    uint64_t now = ~0ull;        // the item whose angles are in the registers
+    uint32_t now = ~0u;          // the item whose angles are in the registers
     uint32_t kind_now = 3;       // and the kind whose factors are
     int64_t row = -1;
     uint64_t f_ac[2], f_bs[2], f_bc[2], f_as[2];   // w_a cos, w_b sin, w_b cos, w_a sin
