@@ -672,6 +672,7 @@ def test_attention_of_some_hundred_rows_a_head(case):
 
 
 @pytest.mark.parametrize("case", [(56, 7, 56, 8, 128, 1300, 246, "f16", "rows"), (42, 100, 8, 8, 128, 853, 100, "bf16", "rows"), (30, 8, 16, 2, 256, 6001, 515, "bf16", "heads"),
-                                  (60, 12, 12, 2, 64, 5000, 300, "f16", "rows"), (30, 8, 16, 2, 256, 12001, 515, "f16", "heads")], ids=str)
+                                  (60, 12, 12, 2, 64, 5000, 300, "f16", "rows"), (30, 8, 16, 2, 256, 12001, 515, "f16", "heads"),
+                                  (56, 7, 56, 8, 64, 1300, 246, "bf16", "rows"), (42, 60, 8, 8, 64, 1853, 300, "f16", "heads")], ids=str)
 def test_attention_of_prefix_and_own_items_that_fill_up_each_other(case):
     test_attention_against_the_definition(case)
