@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(DRAW_THREADS, 1) verify_draw_kernel(const __gr
                 for (int i = 0; i < N; ++i) w[i] = (uint32_t)d == at + i / 4 * 128 + i % 4 ? 0.0 : w[i];
             }
         };
-        double whole = 0.0, start = 0.0, end = 0.0;   // of the row, of the warp's run
+        double whole = 0.0;   // of the row
         auto sum_up = [&](auto kind, int slot) {
             // two blocks at a time, the next two on their way; lanes are added up once a segment of an even number of blocks
             double mine = 0.0;
@@ -493,26 +493,23 @@ __global__ void __launch_bounds__(DRAW_THREADS, 1) verify_draw_kernel(const __gr
             __syncthreads();   // warp_sums of an earlier call are read
             if (lane == 0) warp_sums[warp] = mine;
             __syncthreads();
-            // Running sums of the CTA's warps, of the cluster's CTAs.  Every warp makes the same ones, and the end of a run is the same number as
-            // the next one's start, so the runs share [0, whole) out without gap or overlap.
             const double in_cta = warp_scan(lane < DRAW_WARPS ? warp_sums[lane] : 0.0, lane);
             const double in_all = __shfl_sync(0xffffffffu, in_cta, DRAW_WARPS - 1);
             if (warp == 0 && lane < size) cluster.map_shared_rank(slots[slot], lane)[rank] = in_all;
             cluster.sync();
-            const double in_row = warp_scan(lane < size ? slots[slot][lane] : 0.0, lane);
-            whole = __shfl_sync(0xffffffffu, in_row, size - 1);
-            const double before = rank ? __shfl_sync(0xffffffffu, in_row, rank - 1) : 0.0;
-            start = warp ? before + __shfl_sync(0xffffffffu, in_cta, warp - 1) : before;
-            end = warp + 1 < DRAW_WARPS ? before + __shfl_sync(0xffffffffu, in_cta, warp) : __shfl_sync(0xffffffffu, in_row, rank);
+            whole = __shfl_sync(0xffffffffu, warp_scan(lane < size ? slots[slot][lane] : 0.0, lane), size - 1);
         };
         bool rest = refused && p.probs;   // drawn from the residual
+        int slot = 2;
         if (rest) {
             sum_up(W{}, 0);
             z = 1.0 / whole;
-            sum_up(R{}, 1);
+            slot = 1;
+            sum_up(R{}, slot);
             rest = whole > 0.0;            // nothing may be left of p beside q: then from p
+            if (!rest) slot = 2;
         }
-        for (int slot = 2; !rest; slot = 1) {
+        for (; !rest; slot = 1) {
             sum_up(W{}, slot);
             if (whole > 0.0 || d < 0) break;
             d = -1;                        // the refused draft had all the mass (u was not below one): from p too
@@ -520,10 +517,22 @@ __global__ void __launch_bounds__(DRAW_THREADS, 1) verify_draw_kernel(const __gr
         // inside [0, whole) even if u is not inside [0, 1)
         double target = fmax((double)u_sample * whole, 0.0);
         if (!(target < whole)) target = __longlong_as_double(__double_as_longlong(whole) - 1);
-        if (start <= target && end > target) {
-            double upto = start;
-            uint32_t s = 0, bl = b0;
-            while (bl + seg_blocks < b1 && !(upto + segments[warp][s] > target)) upto += segments[warp][s++], bl += seg_blocks;
+        // The CTA, its warp and the warp's segment that hold the target: the lowest with mass whose running sum passes it.  Sums of the same numbers in another
+        // order differ by roundings, so a target beside a border may pass none of those that have mass; then it is the last of them, and every level has one.
+        auto pick = [&](double mass, double upto) {   // a lane an entry; each warp that asks comes to the same answer
+            const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0), over = __ballot_sync(0xffffffffu, mass > 0.0 && upto > target);
+            return over ? __ffs(over) - 1 : 31 - __clz(some);
+        };
+        auto ahead_of = [&](double upto, int at, double first) { return at ? __shfl_sync(0xffffffffu, upto, at - 1) : first; };
+        const double of_cta = lane < size ? slots[slot][lane] : 0.0, of_warp = lane < DRAW_WARPS ? warp_sums[lane] : 0.0;
+        const double in_row = warp_scan(of_cta, lane), before = ahead_of(in_row, (int)rank, 0.0), in_cta = before + warp_scan(of_warp, lane);
+        const bool here = pick(of_cta, in_row) == (int)rank;
+        if (here && pick(of_warp, in_cta) == (int)warp) {
+            const uint32_t n_seg = (b1 - b0 + seg_blocks - 1) / seg_blocks;
+            const double of_seg = lane < n_seg ? segments[warp][lane] : 0.0, start = ahead_of(in_cta, (int)warp, before), in_run = start + warp_scan(of_seg, lane);
+            const int s = pick(of_seg, in_run);
+            double upto = ahead_of(in_run, s, start);
+            uint32_t bl = b0 + (uint32_t)s * seg_blocks;
             int hit = -1, last = -1;
             for (; bl < b1 && hit < 0; ++bl) {
                 float x[4], q[4];
@@ -551,11 +560,11 @@ __global__ void __launch_bounds__(DRAW_THREADS, 1) verify_draw_kernel(const __gr
                 if (over) hit = __shfl_sync(0xffffffffu, at, __ffs(over) - 1);
                 upto += __shfl_sync(0xffffffffu, sum, 31);
             }
-            if (lane == 0) found = hit >= 0 ? hit : last;   // none by a rounding: the run's last token with any mass
+            if (lane == 0) found = hit >= 0 ? hit : last;   // none by a rounding: the run's last token with any mass (the segment has some)
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0 && found >= 0) p.tokens[(uint64_t)b * p.rows + taken] = found;   // one run of the cluster's holds the target
+    if (threadIdx.x == 0 && found >= 0) p.tokens[(uint64_t)b * p.rows + taken] = found;   // one warp of the cluster's found it
     if (rank == 0) {
         if (threadIdx.x == 0) {
             p.n_accepted[b] = ok ? taken : -1 - taken;

@@ -676,3 +676,35 @@ def test_attention_of_some_hundred_rows_a_head(case):
                                   (56, 7, 56, 8, 64, 1300, 246, "bf16", "rows"), (42, 60, 8, 8, 64, 1853, 300, "f16", "heads")], ids=str)
 def test_attention_of_prefix_and_own_items_that_fill_up_each_other(case):
     test_attention_against_the_definition(case)
+
+
+# ---- draws at the ends of what has mass -----------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("B,V", [(300, 20000), (100, 32001), (20, 40000), (2, 151936), (30, 300)])
+def test_verify_u_of_one_draws_the_last_token_with_mass(B, V, dt):
+    # Rows that end in tokens without mass, as a masked vocabulary does: some of them inside one warp's run, some over many.  The last token's weight
+    # is some 1e-9 of the row's at least, a sum's roundings 1e-13, so u = 1 (and more) can only mean that token.
+    for seed in range(4):
+        g = rng(seed * 10 + V)
+        x = torch.randn(B, 2, V, device="cuda", generator=g).mul_(2).to(DT[dt])
+        last = (torch.rand(B, device="cuda", generator=g) * V).long().clamp(min=3)
+        last[::5] = V - 1 - torch.arange(len(last[::5]), device="cuda") % 5
+        last.clamp_(min=3, max=V - 1)
+        x.masked_fill_((torch.arange(V, device="cuda") > last[:, None])[:, None], -math.inf)
+        us = torch.ones(B, device="cuda")
+        us[::7] = 1.5
+        us[1] = math.inf
+        none = torch.empty(B, 0, device="cuda")
+        n, tok = pkg.verify_drafts(x[:, :1], none.to(torch.int32), none, us)
+        assert (n == 0).all() and torch.equal(tok[:, 0].long(), last)
+        # behind a refused draft without distributions, and from what is left beside one: q holds all of p from `last` on, token `before` is the last with a rest
+        d = torch.zeros(B, 1, device="cuda", dtype=torch.int32)
+        never = torch.full((B, 1), 1.0, device="cuda")
+        n, tok = pkg.verify_drafts(x, d, never, us)
+        assert (n == 0).all() and torch.equal(tok[:, 0].long(), last)
+        p = torch.softmax(x[:, :1].double(), -1)
+        before = (last // 2).clamp(min=1)
+        q = torch.where(torch.arange(V, device="cuda") > before[:, None, None], p * 2, p * 0.5).float()
+        q[:, 0, 0] = 1.0
+        n, tok = pkg.verify_drafts(x, d, never, us, draft_probs=q)
+        assert (n == 0).all() and torch.equal(tok[:, 0].long(), before)
