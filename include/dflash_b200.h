@@ -306,8 +306,9 @@ dfl_status dfl_prefix_attention(int32_t device, const dfl_prefix_attention_args*
  * the whole.  n_accepted_out[b] = drafts that stand; tokens_out[b] = those drafts, the drawn token, then -1.
  * Where a row that the decision reads is no distribution (a NaN or +inf logit, all -inf, a negative, infinite or
  * NaN temperature), n_accepted_out[b] = -1 - row and every token is -1.  A draft outside [0, vocab) does not stand.
- * u in [0, 1); a u_sample outside counts as the nearest number inside (1: the last token with mass).  draft_probs finite and not negative.  The sums that draw a token are in 64 bits, so the token is
- * the one that the definition gives.  n_drafts 0..DFL_MAX_VERIFY_DRAFTS, 1 <= vocab < 2^31; dtype of the logits: DFL_F32,
+ * u in [0, 1); a u_sample outside counts as the nearest number inside (1: the last token with mass).  draft_probs finite and not negative.  Sums that a draft
+ * near its border is judged by, and those that draw a token, are in 64 bits (within some 1e-13 of themselves), so counts and tokens
+ * are those that the definition gives.  n_drafts 0..DFL_MAX_VERIFY_DRAFTS, 1 <= vocab < 2^31; dtype of the logits: DFL_F32,
  * DFL_F16 or DFL_BF16. */
 #define DFL_MAX_VERIFY_DRAFTS 255
 typedef struct dfl_verify_drafts_args {

@@ -7,7 +7,8 @@
 // Two launches.  The first reads every row that it cannot rule out once and leaves (max, sum, index of the first maximum) of each piece of it: bound
 // by the bytes of the logits, f32 sums.  In the second a cluster of one to sixteen CTAs a request puts the pieces together, decides, and goes over
 // the one row that the draw needs again, in 64 bits: a border between two tokens is met by a sum that is 1e-9 off once in a few thousand draws
-// (vocabulary 151 936), by one that is 1e-13 off practically never, and the token is to be the definition's.
+// (vocabulary 151 936), by one that is 1e-13 off practically never, and the token is to be the definition's.  So are the drafts that stand: where u q lies
+// so near to p that the f32 sums do not tell, the cluster adds that row up in 64 bits ahead of the decision.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -137,8 +138,13 @@ __device__ __forceinline__ double weight_of(const Expo& f, float x) {
 struct Row {
     float top;
     int32_t first;
-    int stands;   // the draft behind this row's tokens: 1 stands, 0 does not (or there is none), -1 the row is no distribution
+    int stands;   // the draft behind this row's tokens: 1 stands, 0 does not (or there is none), -1 the row is no distribution, NEAR the f32 sums do not tell
 };
+constexpr int NEAR = 2;
+// How far Z may be off, in relation to itself, by the first kernel's f32 sums.  An exponent a = log2 of 1 / w is off by four roundings of 2^-24 of itself
+// (difference, log2 e, quotient, product), its power by ln 2 times as much; weighted by p, a is log2 V <= 31 at most (its mean is p's entropy less log2 Z): 86
+// units of 2^-24.  Two ex2 of 2^-22 each: 8.  Sums of at most 65, 5 and 5 steps and a product: 76.  Together 170 units; 2^-16 are 256.
+constexpr double Z_OFF = 1.0 / 65536.0;
 // by a whole warp: puts a row's pieces together and tests its draft.  Both kernels come to the same answer: no product in it is left to the
 // compiler to fuse or not.
 template <typename T>
@@ -170,9 +176,9 @@ __device__ __forceinline__ Row row_of(const VerifyParams& p, uint32_t b, uint32_
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     first = __reduce_min_sync(0xffffffffu, first);
     const double w = weight_of(ex, x);
-    const double pd = t > 0.f ? w / sum : (d == first ? 1.0 : 0.0);
+    const double pd = t > 0.f ? w / sum : (d == first ? 1.0 : 0.0), uq = __dmul_rn((double)u, (double)q);   // a product of two f32 is exact
     const bool ok = t >= 0.f && t < INFINITY && top > -INFINITY && top < INFINITY && sum == sum;
-    return Row{top, first, !ok ? -1 : tested && (double)u * (double)q < pd ? 1 : 0};
+    return Row{top, first, !ok ? -1 : !tested ? 0 : t > 0.f && pd > 0.0 && fabs(uq - pd) <= pd * Z_OFF ? NEAR : uq < pd ? 1 : 0};
 }
 __device__ __forceinline__ int drafts_of(const VerifyParams& p, uint32_t b) {
     const int K = (int)p.rows - 1, n = p.n_draft ? p.n_draft[b] : K;
@@ -354,7 +360,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) verify_pieces_kernel(const __gr
                 asm volatile("fence.acq_rel.gpu;" ::: "memory");
                 const float t = temperature_of(p, b);
                 const Row row = row_of<T>(p, b, r, drafts_of(p, b), t, scale_of(t), tab);
-                if (lane == 0 && row.stands != 1) atomicMax(&stops[b], (uint32_t)(STOP_BASE - (int)r));
+                if (lane == 0 && row.stands <= 0) atomicMax(&stops[b], (uint32_t)(STOP_BASE - (int)r));
             }
         }
     }
@@ -399,7 +405,7 @@ __global__ void __launch_bounds__(DRAW_THREADS, 1) verify_draw_kernel(const __gr
     const double tab = pow2_table();
     pdl_wait();
     cg::cluster_group cluster = cg::this_cluster();
-    __shared__ double slots[3][DRAW_CLUSTER];
+    __shared__ double slots[2][DRAW_CLUSTER];   // used in turn: who writes one again has met everybody behind their reading of it
     __shared__ double warp_sums[DRAW_WARPS];
     __shared__ double segments[DRAW_WARPS][DRAW_SEGMENTS];
     __shared__ Row rows[DFL_MAX_VERIFY_DRAFTS + 1];
@@ -411,32 +417,40 @@ __global__ void __launch_bounds__(DRAW_THREADS, 1) verify_draw_kernel(const __gr
     const double scale = scale_of(t);
     if (threadIdx.x == 0) found = -1;
     cluster.barrier_arrive();
-    // a warp a row, four rows a warp at a time until one decides
-    int taken = 0;
-    for (int r0 = 0; r0 <= n; r0 += DRAW_WARPS) {
-        if (r0 + (int)warp <= n) {
-            const Row row = row_of<T>(p, b, r0 + warp, n, t, scale, tab);
-            if (lane == 0) rows[r0 + warp] = row;
+    // on to the first row whose draft does not stand for certain: a warp a row at a time
+    int taken = 0, judged = 0;
+    auto look = [&]() {
+        while (true) {
+            while (taken < min(judged, n) && rows[taken].stands == 1) ++taken;
+            if (taken < judged) return;
+            if (judged + (int)warp <= n) {
+                const Row r = row_of<T>(p, b, judged + warp, n, t, scale, tab);
+                if (lane == 0) rows[judged + warp] = r;
+            }
+            __syncthreads();
+            judged += DRAW_WARPS;
         }
-        __syncthreads();
-        const int end = min(n, r0 + DRAW_WARPS - 1);
-        while (taken < end && rows[taken].stands == 1) ++taken;
-        if (rows[taken].stands != 1 || taken == n) break;
-        ++taken;
-    }
-    const Row row = rows[taken];
-    const bool refused = taken < n, ok = row.stands >= 0;
+    };
+    look();
+    Row row = rows[taken];
     cluster.barrier_wait();   // every CTA of the cluster has started
-    if (ok && t > 0.f) {
-        int d = refused && !p.probs ? p.drafts[(uint64_t)b * K + taken] : -1;   // the token that has no weight
-        const T* x_row = static_cast<const T*>(p.logits) + b * p.x_b + taken * p.x_r;
-        const float* q_row = p.probs + b * p.q_b + taken * p.q_r;
-        const bool x_vec = reinterpret_cast<uintptr_t>(x_row) % (4 * sizeof(T)) == 0, q_vec = reinterpret_cast<uintptr_t>(q_row) % 16 == 0;
+    if (row.stands >= 0 && t > 0.f) {
+        int d = -1;           // the token that has no weight
+        const T* x_row;
+        const float* q_row;
+        bool x_vec, q_vec;
+        Expo ex;
+        auto settle = [&]() {
+            x_row = static_cast<const T*>(p.logits) + b * p.x_b + taken * p.x_r;
+            q_row = p.probs + b * p.q_b + taken * p.q_r;
+            x_vec = reinterpret_cast<uintptr_t>(x_row) % (4 * sizeof(T)) == 0, q_vec = reinterpret_cast<uintptr_t>(q_row) % 16 == 0;
+            ex = expo(row.top, scale, tab);
+        };
+        settle();
         // the row in vocabulary order over the cluster's warps: a run of `count` segments of `seg` tokens each
         const uint32_t n_warps = size * DRAW_WARPS;
         const uint32_t blocks = (p.vocab + 127) / 128, per = (blocks + n_warps - 1) / n_warps, seg_blocks = (per + 2 * DRAW_SEGMENTS - 1) / (2 * DRAW_SEGMENTS) * 2;
         const uint32_t b0 = min(blocks, (rank * DRAW_WARPS + warp) * per), b1 = min(blocks, b0 + per);   // blocks of 128 tokens, four a lane
-        const Expo ex = expo(row.top, scale, tab);
         double z = 1.0;
         // two kinds of weight: w, without the refused draft's (kind W), and max(p - q, 0) (kind R)
         using W = std::false_type;
@@ -499,70 +513,86 @@ __global__ void __launch_bounds__(DRAW_THREADS, 1) verify_draw_kernel(const __gr
             cluster.sync();
             whole = __shfl_sync(0xffffffffu, warp_scan(lane < size ? slots[slot][lane] : 0.0, lane), size - 1);
         };
-        bool rest = refused && p.probs;   // drawn from the residual
-        int slot = 2;
-        if (rest) {
-            sum_up(W{}, 0);
-            z = 1.0 / whole;
-            slot = 1;
-            sum_up(R{}, slot);
-            rest = whole > 0.0;            // nothing may be left of p beside q: then from p
-            if (!rest) slot = 2;
-        }
-        for (; !rest; slot = 1) {
-            sum_up(W{}, slot);
-            if (whole > 0.0 || d < 0) break;
-            d = -1;                        // the refused draft had all the mass (u was not below one): from p too
-        }
-        // inside [0, whole) even if u is not inside [0, 1)
-        double target = fmax((double)u_sample * whole, 0.0);
-        if (!(target < whole)) target = __longlong_as_double(__double_as_longlong(whole) - 1);
-        // The CTA, its warp and the warp's segment that hold the target: the lowest with mass whose running sum passes it.  Sums of the same numbers in another
-        // order differ by roundings, so a target beside a border may pass none of those that have mass; then it is the last of them, and every level has one.
-        auto pick = [&](double mass, double upto) {   // a lane an entry; each warp that asks comes to the same answer
-            const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0), over = __ballot_sync(0xffffffffu, mass > 0.0 && upto > target);
-            return over ? __ffs(over) - 1 : 31 - __clz(some);
-        };
-        auto ahead_of = [&](double upto, int at, double first) { return at ? __shfl_sync(0xffffffffu, upto, at - 1) : first; };
-        const double of_cta = lane < size ? slots[slot][lane] : 0.0, of_warp = lane < DRAW_WARPS ? warp_sums[lane] : 0.0;
-        const double in_row = warp_scan(of_cta, lane), before = ahead_of(in_row, (int)rank, 0.0), in_cta = before + warp_scan(of_warp, lane);
-        const bool here = pick(of_cta, in_row) == (int)rank;
-        if (here && pick(of_warp, in_cta) == (int)warp) {
-            const uint32_t n_seg = (b1 - b0 + seg_blocks - 1) / seg_blocks;
-            const double of_seg = lane < n_seg ? segments[warp][lane] : 0.0, start = ahead_of(in_cta, (int)warp, before), in_run = start + warp_scan(of_seg, lane);
-            const int s = pick(of_seg, in_run);
-            double upto = ahead_of(in_run, s, start);
-            uint32_t bl = b0 + (uint32_t)s * seg_blocks;
-            int hit = -1, last = -1;
-            for (; bl < b1 && hit < 0; ++bl) {
-                float x[4], q[4];
-                double w[4];
-                if (rest) {
-                    fetch(R{}, bl, x, q);
-                    weights(R{}, bl, x, q, w);
+        // Whether a row is added up to judge its draft or to draw, every CTA comes to it alike: all have the same pieces.
+        bool rest = false, all = false;   // drawn from the residual; from p behind a refused draft too
+        int slot = 1;
+        while (row.stands >= 0) {
+            const bool near = row.stands == NEAR, refused = taken < n && !all;
+            d = !near && refused && !p.probs ? p.drafts[(uint64_t)b * K + taken] : -1;
+            sum_up(W{}, slot ^= 1);
+            if (near) {
+                const int draft = p.drafts[(uint64_t)b * K + taken];
+                const double uq = __dmul_rn((double)p.u_accept[(uint64_t)b * K + taken], p.probs ? (double)q_row[draft] : 1.0);
+                if (uq < weight_of(ex, logit<T>(x_row, draft)) / whole) {
+                    ++taken;
+                    look();
+                    row = rows[taken];
+                    settle();
                 } else {
-                    fetch(W{}, bl, x, q);
-                    weights(W{}, bl, x, q, w);
+                    row.stands = 0;
                 }
-                const double own = (w[0] + w[1]) + (w[2] + w[3]), sum = warp_scan(own, lane);
-                double run = upto + (sum - own);
-                int at = -1, some = -1;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    run += w[e];
-                    if (w[e] > 0.0) {
-                        some = (int)(bl * 128 + lane * 4 + e);
-                        if (at < 0 && run > target) at = some;
-                    }
-                }
-                const unsigned over = __ballot_sync(0xffffffffu, at >= 0);
-                last = max(last, __reduce_max_sync(0xffffffffu, some));
-                if (over) hit = __shfl_sync(0xffffffffu, at, __ffs(over) - 1);
-                upto += __shfl_sync(0xffffffffu, sum, 31);
+                continue;
             }
-            if (lane == 0) found = hit >= 0 ? hit : last;   // none by a rounding: the run's last token with any mass (the segment has some)
+            if (refused && p.probs) {
+                z = 1.0 / whole;
+                sum_up(R{}, slot ^= 1);
+                rest = whole > 0.0;
+            }
+            if (rest || (whole > 0.0 && !(refused && p.probs)) || !refused) break;
+            all = true;   // nothing is left of p beside q, or the refused draft had all the mass (u was not below one): from p itself
+        }
+        if (row.stands >= 0) {
+            // inside [0, whole) even if u is not inside [0, 1)
+            double target = fmax((double)u_sample * whole, 0.0);
+            if (!(target < whole)) target = __longlong_as_double(__double_as_longlong(whole) - 1);
+            // The CTA, its warp and the warp's segment that hold the target: the lowest with mass whose running sum passes it.  Sums of the same numbers in another
+            // order differ by roundings, so a target beside a border may pass none of those that have mass; then it is the last of them, and every level has one.
+            auto pick = [&](double mass, double upto) {   // a lane an entry; each warp that asks comes to the same answer
+                const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0), over = __ballot_sync(0xffffffffu, mass > 0.0 && upto > target);
+                return over ? __ffs(over) - 1 : 31 - __clz(some);
+            };
+            auto ahead_of = [&](double upto, int at, double first) { return at ? __shfl_sync(0xffffffffu, upto, at - 1) : first; };
+            const double of_cta = lane < size ? slots[slot][lane] : 0.0, of_warp = lane < DRAW_WARPS ? warp_sums[lane] : 0.0;
+            const double in_row = warp_scan(of_cta, lane), before = ahead_of(in_row, (int)rank, 0.0), in_cta = before + warp_scan(of_warp, lane);
+            const bool here = pick(of_cta, in_row) == (int)rank;
+            if (here && pick(of_warp, in_cta) == (int)warp) {
+                const uint32_t n_seg = (b1 - b0 + seg_blocks - 1) / seg_blocks;
+                const double of_seg = lane < n_seg ? segments[warp][lane] : 0.0, start = ahead_of(in_cta, (int)warp, before), in_run = start + warp_scan(of_seg, lane);
+                const int s = pick(of_seg, in_run);
+                double upto = ahead_of(in_run, s, start);
+                uint32_t bl = b0 + (uint32_t)s * seg_blocks;
+                int hit = -1, last = -1;
+                for (; bl < b1 && hit < 0; ++bl) {
+                    float x[4], q[4];
+                    double w[4];
+                    if (rest) {
+                        fetch(R{}, bl, x, q);
+                        weights(R{}, bl, x, q, w);
+                    } else {
+                        fetch(W{}, bl, x, q);
+                        weights(W{}, bl, x, q, w);
+                    }
+                    const double own = (w[0] + w[1]) + (w[2] + w[3]), sum = warp_scan(own, lane);
+                    double run = upto + (sum - own);
+                    int at = -1, some = -1;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        run += w[e];
+                        if (w[e] > 0.0) {
+                            some = (int)(bl * 128 + lane * 4 + e);
+                            if (at < 0 && run > target) at = some;
+                        }
+                    }
+                    const unsigned over = __ballot_sync(0xffffffffu, at >= 0);
+                    last = max(last, __reduce_max_sync(0xffffffffu, some));
+                    if (over) hit = __shfl_sync(0xffffffffu, at, __ffs(over) - 1);
+                    upto += __shfl_sync(0xffffffffu, sum, 31);
+                }
+                if (lane == 0) found = hit >= 0 ? hit : last;   // none by a rounding: the run's last token with any mass (the segment has some)
+            }
         }
     }
+    const bool ok = row.stands >= 0;
     __syncthreads();
     if (threadIdx.x == 0 && found >= 0) p.tokens[(uint64_t)b * p.rows + taken] = found;   // one warp of the cluster's found it
     if (rank == 0) {

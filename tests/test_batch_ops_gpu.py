@@ -708,3 +708,30 @@ def test_verify_u_of_one_draws_the_last_token_with_mass(B, V, dt):
         q[:, 0, 0] = 1.0
         n, tok = pkg.verify_drafts(x, d, never, us, draft_probs=q)
         assert (n == 0).all() and torch.equal(tok[:, 0].long(), before)
+
+
+# ---- drafts beside the border of standing and falling ---------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("B,K,V,sharp", [(64, 3, 151936, 2.0), (6, 3, 151936, 1.0), (40, 15, 32001, 0.3), (12, 7, 1000, 3.0), (5, 255, 777, 1.0)])
+def test_verify_drafts_a_step_of_f32_beside_the_border(B, K, V, sharp, probs, dt):
+    # u q(d) is one of the f32 numbers around p(d), within 2^-23 of it: far from it for a sum in 64 bits (1e-13), nothing for one in 32 (some 1e-7)
+    g = rng(V + B)
+    dev = {"device": "cuda", "generator": g}
+    x = (torch.randn(B, K + 1, V, **dev) * sharp).to(DT[dt])
+    t = torch.rand(B, **dev) + 0.5
+    d = torch.randint(0, V, (B, K), **dev).to(torch.int32)
+    p = torch.softmax(x.double() / t.double()[:, None, None], -1)[:, :K].gather(2, d.long()[..., None])[..., 0]
+    ua = torch.rand(B, K, **dev) * 0.6 + 0.3
+    goal = p / ua.double() if probs else p
+    near = goal.float()
+    steps = torch.randint(0, 4, (B, K), **dev)
+    near = torch.where(steps == 0, torch.nextafter(near, torch.ones_like(near)), torch.where(steps > 1, torch.nextafter(near, torch.zeros_like(near)), near))
+    q = None
+    if probs:
+        q = torch.softmax(torch.randn(B, K, V, **dev), -1)
+        q.scatter_(2, d.long()[..., None], near[..., None])
+    else:
+        ua = near
+    n, _ = verify_check(x, d, ua, torch.rand(B, **dev), q, None, t)
+    assert n.max() > 1 and n.min() < K     # some stand, some fall
