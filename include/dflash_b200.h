@@ -298,7 +298,7 @@ dfl_status dfl_prefix_attention(int32_t device, const dfl_prefix_attention_args*
 /* Verification of drafted tokens against the target's probabilities from given random numbers, on the device
  * (dfl_accept_prefix is the host's, with its own generator and filters).  Row i of request b's logits
  * [n_drafts + 1][vocab] is the target's distribution behind its first i drafts: p_i = softmax(logits / T), T =
- * temperature[b] (NULL = 1); T == 0 puts all mass on the largest logit, ties to the lowest token.  Draft i
+ * temperature[b] (NULL = 1; a positive one counts as at least 2^-122 and at most 2^122); T == 0 puts all mass on the largest logit, ties to the lowest token.  Draft i
  * (i < n_draft[b], NULL = n_drafts) stands while u_accept[b][i] * q_i(d_i) < p_i(d_i), where q_i is
  * draft_probs[b][i] or, when that is NULL, all mass on the draft.  Behind the last draft that stands one token
  * is drawn: from the residual max(p - q, 0) of the first refused draft (from p itself should that be empty),

@@ -54,7 +54,11 @@ template <> __device__ __forceinline__ float logit<float>(const void* base, int6
 template <> __device__ __forceinline__ float logit<__half>(const void* base, int64_t at) { return __half2float(static_cast<const __half*>(base)[at]); }
 template <> __device__ __forceinline__ float logit<__nv_bfloat16>(const void* base, int64_t at) { return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at]); }
 
-__device__ __forceinline__ float temperature_of(const VerifyParams& p, uint32_t b) { return p.temperature ? p.temperature[b] : 1.f; }
+// Between 2^-122 and 2^122, where 32 log2 e / T and a difference of two logits over T keep their places in f32; what is no temperature stays as it is.
+__device__ __forceinline__ float temperature_of(const VerifyParams& p, uint32_t b) {
+    const float t = p.temperature ? p.temperature[b] : 1.f;
+    return t > 0.f && t < INFINITY ? fminf(fmaxf(t, 0x1p-122f), 0x1p122f) : t;
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -94,7 +98,7 @@ struct Expo {
 __device__ __forceinline__ double pow2_table() { return exp2((double)(threadIdx.x & 31) * 0.03125); }
 // 32 / (T ln 2); T = 0 is never asked for
 __device__ __forceinline__ double scale_of(float t) { return t > 0.f ? 32.0 * 1.4426950408889634 / (double)t : 0.0; }
-__device__ __forceinline__ Expo expo(float top, double scale, double tab) { return Expo{(double)top, scale, tab, top, fminf((float)scale, 3e38f)}; }
+__device__ __forceinline__ Expo expo(float top, double scale, double tab) { return Expo{(double)top, scale, tab, top, (float)scale}; }
 template <int N>
 __device__ __forceinline__ void weights_of(const Expo& f, const float* x, double (&w)[N]) {
     constexpr double L = 0.02166084939249829;   // ln 2 / 32
@@ -192,7 +196,7 @@ __device__ __forceinline__ int drafts_of(const VerifyParams& p, uint32_t b) {
 // piece is done its draft is tested, and where it falls the rows behind are spared.
 struct ItemInfo {   // what the producer found out about a piece
     uint32_t b, r, piece, head, v0, n, tail;   // n vectors from v0 on, `head` logits ahead of the row's first vector, the last ones from `tail` on
-    float c;                                   // log2 e / T, finite: 0 * c has to stay 0
+    float c;                                   // log2 e / T
     int32_t greedy, end;
 };
 
@@ -245,7 +249,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) verify_pieces_kernel(const __gr
                 f.v0 = f.piece * (PIECE / VE);
                 f.n = f.v0 < n_vec ? min(n_vec - f.v0, PIECE / VE) : 0;
                 const float t = temperature_of(p, f.b);
-                f.c = t > 0.f ? fminf(1.44269504f / t, 3e38f) : 1.f;
+                f.c = t > 0.f ? 1.44269504f / t : 1.f;
                 f.greedy = t == 0.f;
             }
             while (true) {

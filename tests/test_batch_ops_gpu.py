@@ -735,3 +735,22 @@ def test_verify_drafts_a_step_of_f32_beside_the_border(B, K, V, sharp, probs, dt
         ua = near
     n, _ = verify_check(x, d, ua, torch.rand(B, **dev), q, None, t)
     assert n.max() > 1 and n.min() < K     # some stand, some fall
+
+
+# ---- temperatures at the ends of f32 --------------------------------------------------------------------------------
+@pytest.mark.parametrize("probs", [False, True])
+def test_verify_temperatures_at_the_ends_of_f32_count_as_the_nearest_usable(probs):
+    # logits of the temperature's own size, so that the weights are neither equal nor zero: subnormal ones under the smallest, huge ones under the largest
+    B, K, V = 8, 2, 3001
+    low, high = 2.0 ** -122, 2.0 ** 122
+    t = torch.tensor([1e-45, 1e-40, 1.1e-38, low, high, 2e37, 3.4e38, 1.0], device="cuda")
+    for seed in range(3):
+        x, d, ua, us, q = verify_case(B, K, V, "f32", probs, seed)
+        x = (x * t.clamp(low, high)[:, None, None].double()).float()
+        x[6, :, 5:9] = torch.finfo(torch.float32).min
+        got = pkg.verify_drafts(x, d, ua, us, draft_probs=q, temperature=t)
+        want = verify_ref(x, d, ua, us, q, None, t.clamp(low, high))
+        assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+        # logits far apart: a row's largest alone, and all alike
+        x = x / t.clamp(low, high)[:, None, None]
+        verify_check(x, d, ua, us, q, None, t)
