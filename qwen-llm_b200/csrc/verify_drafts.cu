@@ -612,18 +612,15 @@ __global__ void __launch_bounds__(DRAW_THREADS, 1) verify_draw_kernel(const __gr
 
 struct Split {
     uint32_t n_pieces;
-    bool tickets;
-    uint64_t piece_bytes, ticket_bytes;
+    uint64_t piece_bytes, ticket_bytes;   // counters have a place wherever a draft can fall, so that the size is the same on every device
 };
 Split split_of(const dfl_verify_drafts_args* a) {
     const uint32_t piece = ST_BYTES / (a->dtype == DFL_F32 ? 4 : 2);
     Split s;
     s.n_pieces = (uint32_t)((a->vocab + piece - 1) / piece);
     const uint64_t rows = (uint64_t)a->batch * (a->n_drafts + 1);
-    // Sparing rows pays with more pieces than the rings hold at once.  The counters have to be cleared, a launch of 2 us.
-    s.tickets = a->n_drafts > 0 && rows * s.n_pieces > 2 * 148 * ST_SLOTS;
     s.piece_bytes = (rows * s.n_pieces * sizeof(Piece) + 255) / 256 * 256;
-    s.ticket_bytes = s.tickets ? (rows + a->batch) * sizeof(uint32_t) : 0;
+    s.ticket_bytes = a->n_drafts > 0 ? (rows + a->batch) * sizeof(uint32_t) : 0;
     return s;
 }
 
@@ -713,7 +710,8 @@ extern "C" dfl_status dfl_verify_drafts(int32_t device, const dfl_verify_drafts_
     const Split s = split_of(a);
     p.batch = a->batch, p.rows = a->n_drafts + 1, p.vocab = (uint32_t)a->vocab, p.n_pieces = s.n_pieces;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (s.tickets) {
+    // Sparing rows pays with twice as many pieces as the rings hold at once.  The counters have to be cleared, a launch of 2 us.
+    if (a->n_drafts > 0 && (uint64_t)p.batch * p.rows * p.n_pieces > 2ull * sm_count() * ST_SLOTS) {
         p.tickets = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a->workspace) + s.piece_bytes);
         DFL_CUDA(cudaMemsetAsync(p.tickets, 0, s.ticket_bytes, st));
     }

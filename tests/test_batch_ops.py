@@ -171,3 +171,13 @@ MORE_REFUSED = [
 @pytest.mark.parametrize("make,entry,change,status", MORE_REFUSED, ids=["%s-%s" % (e[4:], "-".join(c)) for _, e, c, _ in MORE_REFUSED])
 def test_refused_addresses_and_strides(make, entry, change, status):
     test_refused_before_anything_runs(make, entry, change, status)
+
+
+def test_verify_workspace_has_room_for_its_counters_whatever_the_machine():
+    # whether rows are counted depends on how many SMs there are; the size, asked for without a device, does not
+    f = C.CFUNCTYPE(C.c_int32, C.c_int32, C.c_void_p, C.c_void_p)(("dfl_verify_drafts_workspace", pkg.lib()))
+    for batch, drafts, vocab in ((1, 0, 1000), (1, 1, 10), (3, 15, 151936), (30, 7, 32000), (128, 7, 151936), (500, 0, 151936)):
+        need = C.c_uint64()
+        pkg.check(f(0, C.byref(verify_args(batch=batch, n_drafts=drafts, vocab=vocab)), C.byref(need)))
+        rows, pieces = batch * (drafts + 1), -(-vocab // 8192)
+        assert need.value == -(-rows * pieces * 16 // 256) * 256 + (4 * (rows + batch) if drafts else 0)
