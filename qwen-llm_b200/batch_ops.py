@@ -1,7 +1,8 @@
 """Operators for a batch of requests that continue one prompt, over torch CUDA tensors.
 
 Mirrors dfl_qk_norm_rope, dfl_prefix_attention and dfl_verify_drafts (include/dflash_b200.h): shapes, dtypes and strides are
-read off the tensors, outputs and workspaces come from torch's allocator on the call's stream, nothing waits for the GPU.
+read off the tensors, outputs and workspaces come from torch's allocator on the call's stream, nothing waits for the GPU.  With `stream` the work goes to
+that stream: it has to be ordered behind what the inputs come from, and whoever reads the outputs behind it, as with torch.cuda.stream().
 torch is imported with the first call only; the rest of the package does not need it.
 """
 import contextlib
@@ -140,13 +141,18 @@ def _no_grad(torch, *tensors):
 
 
 @contextlib.contextmanager
-def _current(torch, dev, stream):
-    """The device, and the stream where one is given, as torch's current ones: what is allocated inside belongs to that stream."""
+def _current(torch, dev, stream, tensors):
+    """The device, and the stream where one is given, as torch's current ones: what is allocated inside belongs to that stream, and the memory of the
+    tensors that the call was given goes to no other one before the stream has passed the call."""
     with torch.cuda.device(dev):
         if stream is not None and stream.device.index != dev:
             raise ValueError(f"stream on {stream.device}, tensors on cuda:{dev}")
         with torch.cuda.stream(stream):
             yield
+        if stream is not None:
+            for x in tensors:
+                if x is not None:
+                    x.record_stream(stream)
 
 
 def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, interleaved=False, q_weight=None, k_weight=None, eps=1e-6,
@@ -158,7 +164,7 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
     L, torch, check, dtypes, raw = _fns()
     dev = _device(q, "q", 3, "[tokens, heads, dim]")
     if stream is not None or torch.cuda.current_device() != dev:
-        with _current(torch, dev, stream):
+        with _current(torch, dev, stream, (q, k, positions, q_weight, k_weight, q_out, k_out, k_rows, v, v_out)):
             return qk_norm_rope(q, k, positions, theta=theta, rotary_dim=rotary_dim, sections=sections, interleaved=interleaved, q_weight=q_weight,
                                 k_weight=k_weight, eps=eps, q_out=q_out, k_out=k_out, k_rows=k_rows, v=v, v_out=v_out)
     shape, dt, f32 = q.shape, q.dtype, torch.float32
@@ -216,7 +222,7 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
     L, torch, check, dtypes, raw = _fns()
     dev = _device(q, "q", 4, "[batch, tokens, heads, dim]")
     if stream is not None or torch.cuda.current_device() != dev:
-        with _current(torch, dev, stream):
+        with _current(torch, dev, stream, (q, prefix_k, prefix_v, own_k, own_v, own_len, q_len, out)):
             return prefix_attention(q, prefix_k, prefix_v, own_k, own_v, own_len, q_len=q_len, scale=scale, out=out)
     shape, dt = q.shape, q.dtype
     B, n, hq, D = shape
@@ -257,7 +263,7 @@ def verify_drafts(logits, drafts, u_accept, u_sample, *, draft_probs=None, n_dra
     L, torch, check, dtypes, raw = _fns()
     dev = _device(logits, "logits", 3, "[batch, drafts + 1, vocab]")
     if stream is not None or torch.cuda.current_device() != dev:
-        with _current(torch, dev, stream):
+        with _current(torch, dev, stream, (logits, drafts, u_accept, u_sample, draft_probs, n_draft, temperature)):
             return verify_drafts(logits, drafts, u_accept, u_sample, draft_probs=draft_probs, n_draft=n_draft, temperature=temperature)
     shape, f32, i32 = logits.shape, torch.float32, torch.int32
     B, R, V = shape

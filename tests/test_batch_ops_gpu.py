@@ -754,3 +754,34 @@ def test_verify_temperatures_at_the_ends_of_f32_count_as_the_nearest_usable(prob
         # logits far apart: a row's largest alone, and all alike
         x = x / t.clamp(low, high)[:, None, None]
         verify_check(x, d, ua, us, q, None, t)
+
+
+# ---- memory on other streams ----------------------------------------------------------------------------------------
+def test_tensors_given_with_a_stream_stay_theirs_until_it_has_passed():
+    # made on the current stream, used on another, dropped at once: their memory may not go to the next tensor before the other stream has read it
+    side = torch.cuda.Stream()
+    q, pk, pv, ok, ov = attn_case(4, 8, 16, 2, 128, 3000, 64, "bf16")
+    own_len = torch.tensor([8, 64, 33, 20], device="cuda", dtype=torch.int32)
+    pos = torch.arange(32, device="cuda", dtype=torch.int32)
+    x, d, ua, us, p = verify_case(4, 3, 60000, "f32", True)
+    calls = [
+        (lambda a, **kw: pkg.prefix_attention(*a, **kw), (q, pk, pv, ok, ov, own_len)),
+        (lambda a, **kw: pkg.qk_norm_rope(a[0], a[1], a[2], theta=1e4, v=a[3], **kw), (q.reshape(32, 16, 128), pk[:32].clone(), pos, pv[:32].clone())),
+        (lambda a, **kw: pkg.verify_drafts(*a[:4], draft_probs=a[4], **kw), (x, d, ua, us, p)),
+    ]
+    for call, tensors in calls:
+        as_tuple = lambda r: r if isinstance(r, tuple) else (r,)
+        want = [y.clone() for y in as_tuple(call(tensors))]
+        torch.cuda.synchronize()
+        given = [y.clone() for y in tensors]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)      # some 10 ms
+        got = as_tuple(call(given, stream=side))
+        sizes = [(y.shape, y.dtype) for y in given]
+        del given
+        over = [torch.zeros(s, dtype=t, device="cuda") for s, t in sizes]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        del over
