@@ -133,7 +133,7 @@ def _dense(x, name, shape, dtype, dev):
 
 
 def _no_grad(torch, *tensors):
-    """The operators have no backward pass: a result that autograd would take for a constant is refused."""
+    """The operators have no backward pass: a result that autograd would take for a constant is refused, and an output that it tracks."""
     if torch.is_grad_enabled():
         for x in tensors:
             if x is not None and x.requires_grad:
@@ -193,7 +193,7 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
         rows, _ = _take(k_rows, "k_rows", (T,), torch.int64, dev)
         if k_out is None or (v is not None and v_out is None):
             raise ValueError("k_rows: needs k_out (and v_out)")
-    _no_grad(torch, q, k, v, q_weight, k_weight)
+    _no_grad(torch, q, k, v, q_weight, k_weight, q_out, k_out, v_out)
     if q_out is None:
         q_out = torch.empty(shape, dtype=dt, device=q.device)
     out_dt = q_out.dtype
@@ -239,7 +239,7 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
         ov_p, ov_s = _take(own_v, "own_v", (B, cap, hk, D), dt, dev)
         lens, _ = _take(own_len, "own_len", (B,), torch.int32, dev)
     q_lens = 0 if q_len is None else _take(q_len, "q_len", (B,), torch.int32, dev)[0]
-    _no_grad(torch, q, prefix_k, prefix_v, own_k, own_v)
+    _no_grad(torch, q, prefix_k, prefix_v, own_k, own_v, out)
     if out is None:
         out = (torch.empty if q_len is None else torch.zeros)(shape, dtype=dt, device=q.device)
     o_p, o_s = _take_out(out, "out", shape, dt, dev)

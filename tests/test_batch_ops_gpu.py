@@ -785,3 +785,21 @@ def test_tensors_given_with_a_stream_stay_theirs_until_it_has_passed():
         for a, b in zip(got, want):
             assert torch.equal(a, b)
         del over
+
+
+# ---- torch's bookkeeping ---------------------------------------------------------------------------------------------
+def wrapper_inputs(dt="f16"):
+    q, pk, pv, ok, ov = attn_case(2, 3, 4, 2, 64, 100, 8, dt)
+    pos = torch.arange(6, device="cuda", dtype=torch.int32)
+    return q, pk, pv, ok, ov, torch.tensor([8, 5], device="cuda", dtype=torch.int32), q.reshape(6, 4, 64), pk[:6], pv[:6], pos
+
+
+def test_wrappers_refuse_outputs_that_require_gradients():
+    q, pk, pv, ok, ov, own_len, flat, k, v, pos = wrapper_inputs()
+    leaf = lambda x: torch.zeros_like(x).requires_grad_()
+    for call in (lambda: pkg.prefix_attention(q, pk, pv, out=leaf(q)), lambda: pkg.qk_norm_rope(flat, k, pos, theta=1e4, q_out=leaf(flat)),
+                 lambda: pkg.qk_norm_rope(flat, k, pos, theta=1e4, k_out=leaf(k)), lambda: pkg.qk_norm_rope(flat, k, pos, theta=1e4, v=v, v_out=leaf(v))):
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            call()
+        with torch.no_grad():
+            call()
