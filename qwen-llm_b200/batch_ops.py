@@ -133,11 +133,16 @@ def _dense(x, name, shape, dtype, dev):
 
 
 def _no_grad(torch, *tensors):
-    """The operators have no backward pass: a result that autograd would take for a constant is refused, and an output that it tracks."""
+    """The operators have no derivatives: a result that autograd would take for a constant is refused, and an output that it tracks."""
     if torch.is_grad_enabled():
         for x in tensors:
             if x is not None and x.requires_grad:
                 raise RuntimeError("no backward pass: call it under torch.no_grad() or on detached tensors")
+    fw = torch.autograd.forward_ad
+    if fw._current_level >= 0:   # inside a dual_level(); no_grad() does not reach that
+        for x in tensors:
+            if x is not None and fw.unpack_dual(x).tangent is not None:
+                raise RuntimeError("no forward-mode derivative: a tensor has a tangent")
 
 
 @contextlib.contextmanager

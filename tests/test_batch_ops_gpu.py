@@ -803,3 +803,22 @@ def test_wrappers_refuse_outputs_that_require_gradients():
             call()
         with torch.no_grad():
             call()
+
+
+def test_wrappers_refuse_tangents():
+    import torch.autograd.forward_ad as fw
+    q, pk, pv, ok, ov, own_len, flat, k, v, pos = wrapper_inputs()
+    logits, u = torch.zeros(2, 2, 10, device="cuda"), torch.zeros(2, 1, device="cuda")
+    with fw.dual_level(), torch.no_grad():     # forward mode is not what no_grad() turns off
+        dual = lambda x: fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: pkg.prefix_attention(dual(q), pk, pv), lambda: pkg.prefix_attention(q, pk, dual(pv)), lambda: pkg.prefix_attention(q, pk, pv, ok, dual(ov), own_len),
+                     lambda: pkg.prefix_attention(q, pk, pv, out=dual(torch.empty_like(q))), lambda: pkg.qk_norm_rope(dual(flat), k, pos, theta=1e4),
+                     lambda: pkg.qk_norm_rope(flat, k, pos, theta=1e4, k_weight=dual(torch.ones(64, device="cuda"))), lambda: pkg.qk_norm_rope(flat, k, pos, theta=1e4, v=dual(v)),
+                     lambda: pkg.qk_norm_rope(flat, k, pos, theta=1e4, q_out=dual(torch.empty_like(flat))), lambda: pkg.verify_drafts(dual(logits), u.int(), u, u[:, 0].contiguous())):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+        pkg.prefix_attention(q, pk, pv)        # without tangents as ever
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: pkg.prefix_attention(x, pk, pv), (q,), (torch.ones_like(q),))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: pkg.prefix_attention(x, pk, pv))(q[None])
