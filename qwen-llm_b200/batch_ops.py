@@ -60,7 +60,7 @@ _FNS = None
 
 
 def _fns():
-    """The library's entry points with their argument types, torch, the status check, dtype codes, and the handle of a device's current stream."""
+    """The library's entry points with their argument types, torch, the status check, dtype codes, the handle of a device's current stream, and autograd's notice."""
     global _FNS
     if _FNS is None:
         import torch
@@ -75,7 +75,9 @@ def _fns():
         dtypes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
         # the handle without a Stream object around it, where torch has that: 0.1 us instead of 2.3
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
-        _FNS = (L, torch, check, dtypes, raw)
+        # says to autograd that a caller's tensors have changed, so that a graph that saved one of them does not take it for what it was
+        written = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
+        _FNS = (L, torch, check, dtypes, raw, written)
     return _FNS
 
 
@@ -102,7 +104,7 @@ def _extents(x, name, dims, what):
 
 
 # Calls of a few microseconds on the device are bounded by the checks here, so a tensor is asked for each of its properties once and looked at closely
-# only when it is out of line: norm and rotation of one token take the host 12 us a call, 9 of them here.
+# only when it is out of line: norm and rotation of one token take the host 13 us a call, 10 of them here.
 def _take(x, name, shape, dtype, dev):
     """(address, strides) of a tensor that has this shape and dtype, lies on device number `dev` and is contiguous in its last dimension."""
     s = x.stride()
@@ -166,7 +168,7 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
     an axis), and the store of the K (and V) rows: at row t, or at k_rows[t] (int64) of k_out / v_out [rows, Hkv, D], rows outside of which
     are dropped.  Weights are f32 [D].  Outputs that are not given are new tensors of q's dtype.  Returns (q_out, k_out) or, with v, (q_out,
     k_out, v_out)."""
-    L, torch, check, dtypes, raw = _fns()
+    L, torch, check, dtypes, raw, written = _fns()
     dev = _device(q, "q", 3, "[tokens, heads, dim]")
     if stream is not None or torch.cuda.current_device() != dev:
         with _current(torch, dev, stream, (q, k, positions, q_weight, k_weight, q_out, k_out, k_rows, v, v_out)):
@@ -198,7 +200,8 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
         rows, _ = _take(k_rows, "k_rows", (T,), torch.int64, dev)
         if k_out is None or (v is not None and v_out is None):
             raise ValueError("k_rows: needs k_out (and v_out)")
-    _no_grad(torch, q, k, v, q_weight, k_weight, q_out, k_out, v_out)
+    given = (q_out, k_out, v_out)
+    _no_grad(torch, q, k, v, q_weight, k_weight, *given)
     if q_out is None:
         q_out = torch.empty(shape, dtype=dt, device=q.device)
     out_dt = q_out.dtype
@@ -217,6 +220,7 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
                    1 if interleaved else 0, theta, eps, 0, q_p, k_p, v_p, q_s[0], q_s[1], k_s[0], k_s[1], v_s[0], v_s[1], wq, wk, pos_p, axis_stride, rows,
                    n_rows, qo_p, ko_p, vo_p, qo_s[0], qo_s[1], ko_s[0], ko_s[1], vo_s[0], vo_s[1])
     check(L.dfl_qk_norm_rope(dev, a, raw(dev)))
+    written([x for x in given if x is not None])
     return (q_out, k_out) if v is None else (q_out, k_out, v_out)
 
 
@@ -224,7 +228,7 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
     """Attention of a batch over one shared prefix and each request's own rows: q [B, n, Hq, D], prefix_k / prefix_v [P, Hkv, D], own_k / own_v
     [B, cap, Hkv, D] of which own_len[b] (int32) are in use, the block's own rows the last of them.  q_len (int32 [B]): how many of a request's n
     queries exist (all when None); output rows behind them are left as they were (zero in a new tensor).  scale: 1 / sqrt(D) when None."""
-    L, torch, check, dtypes, raw = _fns()
+    L, torch, check, dtypes, raw, written = _fns()
     dev = _device(q, "q", 4, "[batch, tokens, heads, dim]")
     if stream is not None or torch.cuda.current_device() != dev:
         with _current(torch, dev, stream, (q, prefix_k, prefix_v, own_k, own_v, own_len, q_len, out)):
@@ -245,6 +249,7 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
         lens, _ = _take(own_len, "own_len", (B,), torch.int32, dev)
     q_lens = 0 if q_len is None else _take(q_len, "q_len", (B,), torch.int32, dev)[0]
     _no_grad(torch, q, prefix_k, prefix_v, own_k, own_v, out)
+    given = out
     if out is None:
         out = (torch.empty if q_len is None else torch.zeros)(shape, dtype=dt, device=q.device)
     o_p, o_s = _take_out(out, "out", shape, dt, dev)
@@ -257,6 +262,8 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
         work = q.new_empty(size // 2)   # of 16-bit elements
         a = a[:-_WORK.size] + _WORK.pack(work.data_ptr(), size)
     check(L.dfl_prefix_attention(dev, a, raw(dev)))
+    if given is not None:
+        written((given,))
     return out
 
 
@@ -265,7 +272,7 @@ def verify_drafts(logits, drafts, u_accept, u_sample, *, draft_probs=None, n_dra
     (n_accepted int32 [B], tokens int32 [B, K + 1], -1 behind the drawn token).  u_accept [B, K] and u_sample [B] are f32 in [0, 1).
     draft_probs f32 [B, K, V]: the distributions the drafts were drawn from (None: each draft had all the mass); n_draft int32 [B]: drafts that
     exist; temperature f32 [B]: 0 is greedy.  n_accepted[b] = -1 - row where that row is no distribution."""
-    L, torch, check, dtypes, raw = _fns()
+    L, torch, check, dtypes, raw, _ = _fns()
     dev = _device(logits, "logits", 3, "[batch, drafts + 1, vocab]")
     if stream is not None or torch.cuda.current_device() != dev:
         with _current(torch, dev, stream, (logits, drafts, u_accept, u_sample, draft_probs, n_draft, temperature)):

@@ -822,3 +822,18 @@ def test_wrappers_refuse_tangents():
         torch.func.jvp(lambda x: pkg.prefix_attention(x, pk, pv), (q,), (torch.ones_like(q),))
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda x: pkg.prefix_attention(x, pk, pv))(q[None])
+
+
+def test_a_saved_tensor_that_is_written_over_is_noticed():
+    q, pk, pv, ok, ov, own_len, flat, k, v, pos = wrapper_inputs("bf16")
+    for name, call in (("out", lambda x: pkg.prefix_attention(q, pk, pv, out=x)), ("q_out", lambda x: pkg.qk_norm_rope(flat, k, pos, theta=1e4, q_out=x)),
+                       ("k_out", lambda x: pkg.qk_norm_rope(flat, k, pos, theta=1e4, k_out=x)), ("v_out", lambda x: pkg.qk_norm_rope(flat, k, pos, theta=1e4, v=v, v_out=x))):
+        x = torch.ones_like({"out": q, "q_out": flat, "k_out": k, "v_out": v}[name])
+        w = torch.ones_like(x).requires_grad_()
+        y = (x * w).sum()                      # saves x
+        before = x._version
+        with torch.no_grad():
+            call(x)
+        assert x._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
