@@ -165,9 +165,9 @@ def _current(torch, dev, stream, tensors):
 def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, interleaved=False, q_weight=None, k_weight=None, eps=1e-6,
                  q_out=None, k_out=None, k_rows=None, v=None, v_out=None, stream=None):
     """Per-head RMS norm of q [T, Hq, D] and k [T, Hkv, D], rotation by `positions` (int32 [T], or [axes, T] with `sections` frequencies to
-    an axis), and the store of the K (and V) rows: at row t, or at k_rows[t] (int64) of k_out / v_out [rows, Hkv, D], rows outside of which
-    are dropped.  Weights are f32 [D].  Outputs that are not given are new tensors of q's dtype.  Returns (q_out, k_out) or, with v, (q_out,
-    k_out, v_out)."""
+    an axis), and the store of the K (and V) rows: at row t of k_out / v_out, which have as many at least, or at k_rows[t] (int64) of k_out / v_out
+    [rows, Hkv, D], rows outside of which are dropped.  Weights are f32 [D].  Outputs that are not given are new tensors of q_out's dtype, and that one of
+    q's.  Returns (q_out, k_out) or, with v, (q_out, k_out, v_out)."""
     L, torch, check, dtypes, raw, written = _fns()
     dev = _device(q, "q", 3, "[tokens, heads, dim]")
     if stream is not None or torch.cuda.current_device() != dev:
@@ -215,7 +215,9 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
         v_p, v_s = _take(v, "v", kv_shape, dt, dev)
         if v_out is None:
             v_out = torch.empty(kv_shape, dtype=out_dt, device=q.device)
-        vo_p, vo_s = _take_out(v_out, "v_out", (n_rows, hk, D), out_dt, dev)
+        v_rows = n_rows if k_rows is not None else _extents(v_out, "v_out", 3, "[rows, heads, dim]")[0]
+        vo_p, vo_s = _take_out(v_out, "v_out", (v_rows, hk, D), out_dt, dev)
+        n_rows = min(n_rows, v_rows)
     a = _ROPE.pack(_dtype(dtypes, q, "q"), _dtype(dtypes, q_out, "q_out"), T, hq, hk, D, rotary_dim, axes, *sections, *(0,) * (MAX_ROPE_AXES - axes),
                    1 if interleaved else 0, theta, eps, 0, q_p, k_p, v_p, q_s[0], q_s[1], k_s[0], k_s[1], v_s[0], v_s[1], wq, wk, pos_p, axis_stride, rows,
                    n_rows, qo_p, ko_p, vo_p, qo_s[0], qo_s[1], ko_s[0], ko_s[1], vo_s[0], vo_s[1])

@@ -837,3 +837,20 @@ def test_a_saved_tensor_that_is_written_over_is_noticed():
         assert x._version > before
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.backward()
+
+
+# ---- which arguments go together ------------------------------------------------------------------------------------
+def test_rope_new_v_rows_beside_a_longer_k_out():
+    q, k, v, pos, sections, (wq, wk) = rope_case(9, 4, 2, 64, 64, 1, False, "bf16")
+    want = pkg.qk_norm_rope(q, k, pos, theta=1e4, sections=sections, q_weight=wq, k_weight=wk, v=v)
+    k_out, v_out = (torch.full((12, 2, 64), 5.0, device="cuda", dtype=torch.bfloat16) for _ in "kv")
+    got = pkg.qk_norm_rope(q, k, pos, theta=1e4, sections=sections, q_weight=wq, k_weight=wk, v=v, k_out=k_out)
+    assert got[1] is k_out and got[2].shape == (9, 2, 64) and torch.equal(got[2], want[2]) and torch.equal(k_out[:9], want[1]) and (k_out[9:] == 5).all()
+    got = pkg.qk_norm_rope(q, k, pos, theta=1e4, sections=sections, q_weight=wq, k_weight=wk, v=v, v_out=v_out)
+    assert got[2] is v_out and torch.equal(v_out[:9], want[2]) and torch.equal(got[1], want[1]) and (v_out[9:] == 5).all()
+    # rows by number: both outputs are one cache
+    rows = torch.arange(9, device="cuda")
+    with pytest.raises(ValueError, match="v_out: shape"):
+        pkg.qk_norm_rope(q, k, pos, theta=1e4, sections=sections, v=v, k_out=k_out, v_out=v_out[:11], k_rows=rows)
+    with pytest.raises(pkg.DflError, match="fewer output rows than tokens"):
+        pkg.qk_norm_rope(q, k, pos, theta=1e4, sections=sections, v=v, v_out=v_out[:8])
