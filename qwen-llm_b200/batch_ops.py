@@ -218,6 +218,8 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
         v_rows = n_rows if k_rows is not None else _extents(v_out, "v_out", 3, "[rows, heads, dim]")[0]
         vo_p, vo_s = _take_out(v_out, "v_out", (v_rows, hk, D), out_dt, dev)
         n_rows = min(n_rows, v_rows)
+    elif v_out is not None:
+        raise ValueError("v_out: without v")
     a = _ROPE.pack(_dtype(dtypes, q, "q"), _dtype(dtypes, q_out, "q_out"), T, hq, hk, D, rotary_dim, axes, *sections, *(0,) * (MAX_ROPE_AXES - axes),
                    1 if interleaved else 0, theta, eps, 0, q_p, k_p, v_p, q_s[0], q_s[1], k_s[0], k_s[1], v_s[0], v_s[1], wq, wk, pos_p, axis_stride, rows,
                    n_rows, qo_p, ko_p, vo_p, qo_s[0], qo_s[1], ko_s[0], ko_s[1], vo_s[0], vo_s[1])
@@ -249,6 +251,8 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
         ok_p, ok_s = _take(own_k, "own_k", (B, cap, hk, D), dt, dev)
         ov_p, ov_s = _take(own_v, "own_v", (B, cap, hk, D), dt, dev)
         lens, _ = _take(own_len, "own_len", (B,), torch.int32, dev)
+    elif own_v is not None or own_len is not None:
+        raise ValueError("own_v, own_len: without own_k")
     q_lens = 0 if q_len is None else _take(q_len, "q_len", (B,), torch.int32, dev)[0]
     _no_grad(torch, q, prefix_k, prefix_v, own_k, own_v, out)
     given = out

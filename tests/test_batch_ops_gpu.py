@@ -854,3 +854,14 @@ def test_rope_new_v_rows_beside_a_longer_k_out():
         pkg.qk_norm_rope(q, k, pos, theta=1e4, sections=sections, v=v, k_out=k_out, v_out=v_out[:11], k_rows=rows)
     with pytest.raises(pkg.DflError, match="fewer output rows than tokens"):
         pkg.qk_norm_rope(q, k, pos, theta=1e4, sections=sections, v=v, v_out=v_out[:8])
+
+
+def test_wrappers_refuse_arguments_that_nothing_would_read():
+    q, pk, pv, ok, ov, own_len, flat, k, v, pos = wrapper_inputs()
+    for extra in (dict(own_v=ov), dict(own_len=own_len), dict(own_v=ov, own_len=own_len)):
+        with pytest.raises(ValueError, match="without own_k"):
+            pkg.prefix_attention(q, pk, pv, **extra)
+    with pytest.raises(ValueError, match="own_k: needs own_v and own_len"):
+        pkg.prefix_attention(q, pk, pv, ok, ov)
+    with pytest.raises(ValueError, match="v_out: without v"):
+        pkg.qk_norm_rope(flat, k, pos, theta=1e4, v_out=torch.empty_like(v))
