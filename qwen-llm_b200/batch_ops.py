@@ -251,8 +251,8 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
         ok_p, ok_s = _take(own_k, "own_k", (B, cap, hk, D), dt, dev)
         ov_p, ov_s = _take(own_v, "own_v", (B, cap, hk, D), dt, dev)
         lens, _ = _take(own_len, "own_len", (B,), torch.int32, dev)
-    elif own_v is not None or own_len is not None:
-        raise ValueError("own_v, own_len: without own_k")
+    elif own_v is not None:   # (own_len alone is clamped to the rows there are: none)
+        raise ValueError("own_v: without own_k")
     q_lens = 0 if q_len is None else _take(q_len, "q_len", (B,), torch.int32, dev)[0]
     _no_grad(torch, q, prefix_k, prefix_v, own_k, own_v, out)
     given = out

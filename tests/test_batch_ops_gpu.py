@@ -858,9 +858,10 @@ def test_rope_new_v_rows_beside_a_longer_k_out():
 
 def test_wrappers_refuse_arguments_that_nothing_would_read():
     q, pk, pv, ok, ov, own_len, flat, k, v, pos = wrapper_inputs()
-    for extra in (dict(own_v=ov), dict(own_len=own_len), dict(own_v=ov, own_len=own_len)):
-        with pytest.raises(ValueError, match="without own_k"):
+    for extra in (dict(own_v=ov), dict(own_v=ov, own_len=own_len)):
+        with pytest.raises(ValueError, match="own_v: without own_k"):
             pkg.prefix_attention(q, pk, pv, **extra)
+    assert torch.equal(pkg.prefix_attention(q, pk, pv, own_len=own_len), pkg.prefix_attention(q, pk, pv))   # clamped to the rows there are: none
     with pytest.raises(ValueError, match="own_k: needs own_v and own_len"):
         pkg.prefix_attention(q, pk, pv, ok, ov)
     with pytest.raises(ValueError, match="v_out: without v"):
