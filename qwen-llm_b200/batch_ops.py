@@ -200,8 +200,7 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
         rows, _ = _take(k_rows, "k_rows", (T,), torch.int64, dev)
         if k_out is None or (v is not None and v_out is None):
             raise ValueError("k_rows: needs k_out (and v_out)")
-    given = (q_out, k_out, v_out)
-    _no_grad(torch, q, k, v, q_weight, k_weight, *given)
+    _no_grad(torch, q, k, v, q_weight, k_weight, q_out, k_out, v_out)
     if q_out is None:
         q_out = torch.empty(shape, dtype=dt, device=q.device)
     out_dt = q_out.dtype
@@ -224,8 +223,9 @@ def qk_norm_rope(q, k, positions, *, theta, rotary_dim=None, sections=None, inte
                    1 if interleaved else 0, theta, eps, 0, q_p, k_p, v_p, q_s[0], q_s[1], k_s[0], k_s[1], v_s[0], v_s[1], wq, wk, pos_p, axis_stride, rows,
                    n_rows, qo_p, ko_p, vo_p, qo_s[0], qo_s[1], ko_s[0], ko_s[1], vo_s[0], vo_s[1])
     check(L.dfl_qk_norm_rope(dev, a, raw(dev)))
-    written([x for x in given if x is not None])
-    return (q_out, k_out) if v is None else (q_out, k_out, v_out)
+    outs = (q_out, k_out) if v is None else (q_out, k_out, v_out)
+    written(outs)
+    return outs
 
 
 def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None, *, q_len=None, scale=None, out=None, stream=None):
@@ -255,7 +255,6 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
         raise ValueError("own_v: without own_k")
     q_lens = 0 if q_len is None else _take(q_len, "q_len", (B,), torch.int32, dev)[0]
     _no_grad(torch, q, prefix_k, prefix_v, own_k, own_v, out)
-    given = out
     if out is None:
         out = (torch.empty if q_len is None else torch.zeros)(shape, dtype=dt, device=q.device)
     o_p, o_s = _take_out(out, "out", shape, dt, dev)
@@ -268,8 +267,7 @@ def prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None
         work = q.new_empty(size // 2)   # of 16-bit elements
         a = a[:-_WORK.size] + _WORK.pack(work.data_ptr(), size)
     check(L.dfl_prefix_attention(dev, a, raw(dev)))
-    if given is not None:
-        written((given,))
+    written((out,))
     return out
 
 
