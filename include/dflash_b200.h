@@ -223,13 +223,14 @@ dfl_status dfl_argmax_top2_static(int32_t device, const float* logits_dev, int32
  * dimensions from rotary_dim on keep y (the layout of the model's own attention layers).  With several axes
  * (time, height, width) sections[a] frequencies belong to axis a and their sum is rotary_dim / 2: one block of
  * frequencies behind the other, or (interleaved) frequency j to axis a = j mod n_axes while j < n_axes *
- * sections[a], and to axis 0 otherwise.  Angles are exact for every int32 position (negative ones too).
+ * sections[a], and to axis 0 otherwise.  Angles are within 2^-22 rad for every int32 position (negative ones too).
  * kv_rows != NULL: token t's K and V rows go to row kv_rows[t] of k_out / v_out; tokens whose row is negative or
  * at least n_kv_out_rows store none (their query is still written); no two tokens may name the same row.
  * kv_rows == NULL: row t, and n_kv_out_rows is at least n_tokens.  v == NULL or n_kv_heads == 0: no V rows.
  * An output may be its own input's buffer when types and strides are the same and kv_rows is NULL.
- * src_dtype, dst_dtype: DFL_F32, DFL_F16 or DFL_BF16; head_dim 2..512, rotary_dim even and at most head_dim; theta >= 1;
- * sums and angles in f32 or better, one rounding to dst_dtype.  n_tokens == 0 enqueues nothing. */
+ * src_dtype, dst_dtype: DFL_F32, DFL_F16 or DFL_BF16; head_dim 2..512, rotary_dim even and at most head_dim; theta
+ * >= 1 and eps >= 0, both finite; n_tokens below 2^31, at most 65 536 query heads and as many KV heads; sums and
+ * angles in f32 or better, one rounding to dst_dtype.  n_tokens == 0 enqueues nothing. */
 #define DFL_MAX_ROPE_AXES 3
 typedef struct dfl_qk_norm_rope_args {
     int32_t src_dtype, dst_dtype;
@@ -265,11 +266,13 @@ dfl_status dfl_qk_norm_rope(int32_t device, const dfl_qk_norm_rope_args* args, v
  * the device (own_len is clamped to [0, own_capacity], q_len to [0, n_tokens]), so a captured call follows
  * them.  Cache rows behind own_len, and the queries of absent tokens, may hold anything; a NaN or infinity in a V
  * row that exists may reach every row of the request (a prefix row: of the batch) in the heads that read it.
- * dtype: DFL_F16 or DFL_BF16 for all tensors; head_dim 64, 128 or 256; n_q_heads a multiple of n_kv_heads, at
- * most 64 query heads a KV head; prefix_len and own_capacity below 2^30; addresses and strides multiples of 16
- * bytes.  own_len may be NULL when own_capacity is 0.  Scores, softmax and sums in f32; the weights of a tile
- * are rounded to dtype for the product with V, as is the result.  Every wait on the device is bounded; should one
- * run out, the output rows it concerns are NaN.  batch, n_tokens 0: enqueues nothing. */
+ * dtype: DFL_F16 or DFL_BF16 for all tensors; head_dim 64, 128 or 256; n_q_heads a multiple of n_kv_heads, at most
+ * 64 query heads a KV head; prefix_len and own_capacity below 2^30, batch * n_tokens * n_q_heads below 2^31; scale
+ * positive and finite; addresses and strides multiples of 16 bytes, strides below 2^39 bytes and those of K and V
+ * not zero (each key has a place of its own: K and V expanded over heads or requests are refused).  own_len may be
+ * NULL when own_capacity is 0.  Scores, softmax and sums in f32; the weights of a tile are rounded to dtype for the
+ * product with V, as is the result.  Every wait on the device is bounded; should one run out, the output rows it
+ * concerns are NaN.  batch, n_tokens 0: enqueues nothing. */
 typedef struct dfl_prefix_attention_args {
     int32_t dtype;
     uint32_t batch, n_tokens, n_q_heads, n_kv_heads, head_dim;
@@ -296,20 +299,21 @@ dfl_status dfl_prefix_attention_workspace(int32_t device, const dfl_prefix_atten
 dfl_status dfl_prefix_attention(int32_t device, const dfl_prefix_attention_args* args, void* stream);
 
 /* Verification of drafted tokens against the target's probabilities from given random numbers, on the device
- * (dfl_accept_prefix is the host's, with its own generator and filters).  Row i of request b's logits
- * [n_drafts + 1][vocab] is the target's distribution behind its first i drafts: p_i = softmax(logits / T), T =
- * temperature[b] (NULL = 1; a positive one counts as at least 2^-122 and at most 2^122); T == 0 puts all mass on the largest logit, ties to the lowest token.  Draft i
- * (i < n_draft[b], NULL = n_drafts) stands while u_accept[b][i] * q_i(d_i) < p_i(d_i), where q_i is
- * draft_probs[b][i] or, when that is NULL, all mass on the draft.  Behind the last draft that stands one token
- * is drawn: from the residual max(p - q, 0) of the first refused draft (from p itself should that be empty),
- * or from p of the last row when all stand - the lowest token whose cumulated mass exceeds u_sample[b] times
- * the whole.  n_accepted_out[b] = drafts that stand; tokens_out[b] = those drafts, the drawn token, then -1.
- * Where a row that the decision reads is no distribution (a NaN or +inf logit, all -inf, a negative, infinite or
- * NaN temperature), n_accepted_out[b] = -1 - row and every token is -1.  A draft outside [0, vocab) does not stand.
- * u in [0, 1); a u_sample outside counts as the nearest number inside (1: the last token with mass).  draft_probs finite and not negative.  Sums that a draft
- * near its border is judged by, and those that draw a token, are in 64 bits (within some 1e-13 of themselves), so counts and tokens
- * are those that the definition gives.  n_drafts 0..DFL_MAX_VERIFY_DRAFTS, 1 <= vocab < 2^31; dtype of the logits: DFL_F32,
- * DFL_F16 or DFL_BF16. */
+ * (dfl_accept_prefix is the host's, with its own generator and filters).  Row i of request b's logits [n_drafts +
+ * 1][vocab] is the target's distribution behind its first i drafts: p_i = softmax(logits / T), T = temperature[b]
+ * (NULL = 1; a positive one counts as at least 2^-122 and at most 2^122); T == 0 puts all mass on the largest
+ * logit, ties to the lowest token.  Draft i (i < n_draft[b], NULL = n_drafts) stands while u_accept[b][i] *
+ * q_i(d_i) < p_i(d_i), where q_i is draft_probs[b][i] or, when that is NULL, all mass on the draft.  Behind the
+ * last draft that stands one token is drawn: from the residual max(p - q, 0) of the first refused draft (from p
+ * itself should that be empty), or from p of the last row when all stand - the lowest token whose cumulated mass
+ * exceeds u_sample[b] times the whole.  n_accepted_out[b] = drafts that stand; tokens_out[b] = those drafts, the
+ * drawn token, then -1. Where a row that the decision reads is no distribution (a NaN or +inf logit, all -inf, a
+ * negative, infinite or NaN temperature), n_accepted_out[b] = -1 - row and every token is -1.  A draft outside [0,
+ * vocab) does not stand. u in [0, 1); a u_sample outside counts as the nearest number inside.  Filters (top-k,
+ * top-p, min-p) are the caller's: a logit of -inf has no mass.  draft_probs finite and not negative.  Sums that a draft near its border is judged by, and those that
+ * draw a token, are in 64 bits (within some 1e-13 of themselves), so counts and tokens are those that the
+ * definition gives.  n_drafts 0..DFL_MAX_VERIFY_DRAFTS, 1 <= vocab < 2^31, batch up to 2^24, fewer than 2^31 pieces
+ * (begun 32 KB of a row) in batch * (n_drafts + 1) rows; dtype of the logits: DFL_F32, DFL_F16 or DFL_BF16. */
 #define DFL_MAX_VERIFY_DRAFTS 255
 typedef struct dfl_verify_drafts_args {
     int32_t dtype;

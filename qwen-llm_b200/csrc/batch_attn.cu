@@ -15,9 +15,9 @@
 // One persistent CTA an SM; S = Q K^T and O += P V on the tensor cores (tcgen05, both accumulators and P in tensor memory), K and V tiles by
 // TMA into a ring.  Two warpgroups of softmax threads (thread = row), one MMA issuer, one producer.  A step is a key tile.
 //   * head widths 64 and 128: two streams, each with its warpgroup, score buffer and accumulator, half a step apart, so that one's products run under the
-//     other's exponentials.  They take a row tile each; of an item with at most 128 rows every other key tile (two parts of a row then: joining them in
-//     the CTA took 119 us where the second kernel takes 113, 64 requests of a token over 32 768 + 1024 keys); or, with enough such items, an item
-//     each, so that their starts and ends coincide (105 us).  P goes out in two halves, the first half's product runs under the second half's exponentials.  (Two buffers of 64 keys a stream
+//     other's exponentials.  They take a row tile each; of an item with at most 128 rows every other key tile (two parts of a row then, which the
+//     second kernel joins: 112 us for 64 requests of a token over 32 768 + 1024 keys, 6 more where the CTA joined them itself); or, with enough such items, an
+//     item each, so that their starts and ends coincide (98 us).  P goes out in two halves, the first half's product runs under the second half's exponentials.  (Two buffers of 64 keys a stream
 //     instead were slower: the product of a 64-key tile reads Q from shared memory as often as that of a 128-key tile, 192 bytes a clock.)
 //   * 256: the output takes half of tensor memory, there is one stream with two score buffers; the warpgroups take a half of each key tile's columns,
 //     agree on the maximum through shared memory and scale and write a half of the output's columns each.
@@ -195,10 +195,10 @@ __device__ __forceinline__ Item item_of(const BatchAttnParams& p, uint32_t idx, 
 // The items of a CTA, `first` and then those behind `idx`.  The search costs the hot loop some registers, 3 % of the time, so it is three kernels:
 //   * PLAIN: every gridDim.x-th.
 //   * RANKS: where requests may lack whole row blocks (the host does not know their lengths) every gridDim.x-th of the items that have rows: a warp looks 32
-//     of them over at a time.  By number alone some CTAs get seven items and others five: 4 prompts of 1024 to 2048 tokens over 8192 keys took 951 us
-//     instead of 828.
+//     of them over at a time.  By number alone some CTAs get seven items and others five: 4 prompts of 1024 to 2048 tokens over 8192 keys take 930 us
+//     instead of 875.
 //   * EARLY: every gridDim.x-th of the prefix's and then of the own ones, of which the CTAs that had a prefix item less than the others take some ahead (see
-//     plan(): 30 requests of 8 tokens, heads of 256, over 12 001 keys 62.7 us without, 57.0 with; 56 of 7 tokens over 2506 keys 84 and 74).
+//     plan(): 30 requests of 8 tokens, heads of 256, over 12 001 keys 61 to 68 us without, 57 to 61 with; 56 of 7 tokens over 2506 keys 62 to 69 and 59 to 66).
 enum Walk { PLAIN, RANKS, EARLY };
 template <int D, Walk WALK>
 __device__ __forceinline__ uint32_t item_behind(const BatchAttnParams& p, bool first, uint32_t idx) {
@@ -303,8 +303,7 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
     pdl_prologue();
-    // The roles are the arms of one chain and each sets its registers itself.  (With the issue and the producer in a second chain behind the softmax arm, width
-    // 256 took 74 us where it takes 64: 30 requests of 8 tokens, 16 heads over 2 KV heads, prefix of 12 001 keys.)
+    // The roles are the arms of one chain and each sets its registers itself.
     if (warp < 8) {
         // ================= softmax: thread = row =================
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BA_REGS_SOFTMAX));
@@ -390,6 +389,8 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                     uint32_t w[32];
                     uint64_t sum2[2] = {0, 0}, mc2 = 0;
                     const uint64_t c2 = pack2(c, c);
+                    // Weights are rounded to T, the type that the second product takes beside V; the sum has them unrounded.  Half a step each makes the result's
+                    // error 1.2 to 1.4 times that of its own rounding (with f32 weights it would be 1).
                     auto weight = [&](int j, int k) {
                         float a, e;
                         unpack2(fma2(pack2(s[j + 2 * k], s[j + 2 * k + 1]), c2, mc2), a, e);
@@ -404,7 +405,8 @@ batch_attn_t5_kernel(const __grid_constant__ BatchAttnParams p, const __grid_con
                     };
                     refer();
                     float t4[4] = {s[0], s[1], s[2], s[3]};
-                    // (Width 256 makes none before there is a maximum, 65.5 -> 61.3 us; at 128 the same took 5 % longer, 840 -> 895 us for four prompts.)
+                    // (Width 256 makes none before there is a maximum: 60 us instead of 64, 30 requests of 8 tokens over 12 001 keys; at 128 the same takes 3 %
+                    // longer, 900 us instead of 875 for four prompts over 8192 keys.)
                     const bool blank = C::SPLIT && u == 0;
                     if (blank) {
 #pragma unroll
