@@ -866,3 +866,32 @@ def test_wrappers_refuse_arguments_that_nothing_would_read():
         pkg.prefix_attention(q, pk, pv, ok, ov)
     with pytest.raises(ValueError, match="v_out: without v"):
         pkg.qk_norm_rope(flat, k, pos, theta=1e4, v_out=torch.empty_like(v))
+
+
+def test_a_call_with_a_stream_inside_a_capture():
+    q, pk, pv, ok, ov = attn_case(3, 4, 8, 2, 128, 900, 32, "f16")
+    own_len = torch.tensor([4, 32, 11], device="cuda", dtype=torch.int32)
+    x, d, ua, us, _ = verify_case(3, 3, 5000, "f32", False)
+    want = pkg.prefix_attention(q, pk, pv, ok, ov, own_len), *pkg.verify_drafts(x, d, ua, us)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        got = pkg.prefix_attention(q * 1, pk, pv, ok, ov, own_len, stream=side), *pkg.verify_drafts(x * 1, d, ua, us, stream=side)   # inputs made inside and dropped
+        torch.cuda.current_stream().wait_stream(side)
+    for y in got:
+        y.zero_()
+    for _ in range(3):
+        graph.replay()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def test_wrappers_under_inference_mode():
+    q, pk, pv, ok, ov, own_len, flat, k, v, pos = wrapper_inputs()
+    want = pkg.prefix_attention(q, pk, pv, ok, ov, own_len), *pkg.qk_norm_rope(flat, k, pos, theta=1e4, v=v)
+    outs = torch.empty_like(q), torch.empty_like(flat), torch.empty_like(k), torch.empty_like(v)     # made outside, as a cache is
+    with torch.inference_mode():
+        for kept in (outs, [torch.empty_like(x) for x in outs]):
+            got = pkg.prefix_attention(q, pk, pv, ok, ov, own_len, out=kept[0]), *pkg.qk_norm_rope(flat, k, pos, theta=1e4, v=v, q_out=kept[1], k_out=kept[2], v_out=kept[3])
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
